@@ -8,6 +8,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <algorithm>
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <unordered_set>
@@ -411,6 +412,13 @@ int finish(Device& d, CError* err, int exec_code, const char* what) {
   if (g_blocking && d.status_host->code != 0) {
     d.last_status = *d.status_host;
     std::memset(d.status_host, 0, sizeof(GemmStatus));
+    if (d.last_status.code == gonn::kStatusBadIndex) {
+      static const char* const kinds[] = {"token", "teacher token", "label"};
+      set_error(err, "%s: %s %d of row %u is outside the vocabulary.", what,
+                kinds[d.last_status.where < 3 ? d.last_status.where : 0], int(d.last_status.kblock),
+                d.last_status.tile);
+      return -3;
+    }
     // a kernel that gave up may have left split-K arrival counters half counted
     cudaMemsetAsync(d.splitk_counters, 0, kSplitKSlots * 4, d.stream);
     set_error(err,
@@ -1818,6 +1826,449 @@ int gonngpu_linear_backward(GPUPtr xPtr, GPUPtr wPtr, GPUPtr dyPtr, GPUPtr actOu
   }
   const int frc = finish(d, err && rc == 0 ? err : nullptr, -6, "linear backward");
   return rc ? rc : frc;
+}
+
+// ---- rows of logits: log probabilities, distillation ----------------------------------
+namespace {
+// A buffer as a call uses it: at least `count` elements of `size` bytes from its start.
+struct Use {
+  Buffer* b;
+  size_t bytes;
+};
+bool fits(const Buffer* b, long rows, long cols, size_t size) {
+  return (unsigned __int128)rows * (unsigned __int128)cols * size <= b->bytes;
+}
+bool overlap(const Use& a, const Use& b) {
+  if (!a.b || !b.b || !a.bytes || !b.bytes) return false;
+  const char *pa = reinterpret_cast<const char*>(a.b->dptr), *pb = reinterpret_cast<const char*>(b.b->dptr);
+  return pa < pb + b.bytes && pb < pa + a.bytes;
+}
+// -2: buffers on different devices, -3: an output overlaps an input or another output, -1: no
+// device, -6: an upload failed, 0: inputs are resident.  NULL handles are skipped.
+int prepare_buffers(const char* what, std::initializer_list<Use> ins, std::initializer_list<Use> outs,
+                    CError* err) {
+  const int dev = ins.begin()->b->device;
+  for (const auto* list : {&ins, &outs})
+    for (const Use& u : *list)
+      if (u.b && u.b->device != dev) {
+        set_error(err, "%s: buffers live on different devices.", what);
+        return -2;
+      }
+  for (const Use* o = outs.begin(); o != outs.end(); ++o) {
+    bool bad = false;
+    for (const Use& i : ins) bad = bad || overlap(*o, i);
+    for (const Use* q = outs.begin(); q != o; ++q) bad = bad || overlap(*o, *q);
+    if (bad) {
+      set_error(err, "%s: a result buffer must not overlap another buffer of the call.", what);
+      return -3;
+    }
+  }
+  if (ensure_device(dev, err)) return -1;
+  Device& d = g_dev[dev];
+  for (const Use& u : ins)
+    if (u.b && !make_resident(d, u.b)) {
+      cudaGetLastError();
+      set_error(err, "%s: host to device copy failed.", what);
+      return -6;
+    }
+  return 0;
+}
+// A handle that may be NULL; false when it is neither NULL nor a live buffer.
+bool optional_buffer(GPUPtr p, Buffer** out) {
+  *out = p ? as_buffer(p) : nullptr;
+  return !p || *out;
+}
+// Results that do not cover the whole buffer must not hide an upload that is still to come.
+bool keep_rest(Device& d, const Use& u) {
+  return !u.b || u.bytes >= u.b->bytes || make_resident(d, u.b);
+}
+constexpr long kMaxVocab = (1l << 31) - 1;
+}  // namespace
+
+int gonngpu_token_logprobs(GPUPtr logitsPtr, long rows, long vocab, long ld, GPUPtr tokensPtr, long n_tokens,
+                           GPUPtr logprobsPtr, GPUPtr entropyPtr, int top_n, GPUPtr topTokensPtr,
+                           GPUPtr topLogprobsPtr, CError* err) {
+  static const char* const what = "token log probabilities";
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  if (rows <= 0 || vocab <= 0 || vocab > kMaxVocab || rows > kMaxVocab || ld < vocab || n_tokens < 0 ||
+      n_tokens > kMaxVocab || top_n < 0 || top_n > gonn::kMaxTop || top_n > vocab) {
+    set_error(err, "%s: bad dimensions: rows %ld, vocabulary %ld, row pitch %ld, %ld tokens, %d alternatives "
+                   "(at most %d, and no more than the vocabulary).", what, rows, vocab, ld, n_tokens, top_n,
+              gonn::kMaxTop);
+    return -3;
+  }
+  Buffer *x = as_buffer(logitsPtr), *tokens, *lp, *entropy, *top, *top_lp;
+  if (!x || !optional_buffer(tokensPtr, &tokens) || !optional_buffer(logprobsPtr, &lp) ||
+      !optional_buffer(entropyPtr, &entropy) || !optional_buffer(topTokensPtr, &top) ||
+      !optional_buffer(topLogprobsPtr, &top_lp)) {
+    set_error(err, "%s: invalid buffer pointers.", what);
+    return -2;
+  }
+  if ((n_tokens > 0 && (!tokens || !lp)) || (top_n > 0 && (!top || !top_lp)) ||
+      (n_tokens == 0 && top_n == 0 && !entropy)) {
+    set_error(err, "%s: a result is asked for without its buffers, or none is.", what);
+    return -2;
+  }
+  const size_t used = (size_t(rows - 1) * ld + vocab) * 4;
+  if ((unsigned __int128)(rows - 1) * (unsigned __int128)ld * 4 + size_t(vocab) * 4 > x->bytes ||
+      (n_tokens && (!fits(tokens, rows, n_tokens, 4) || !fits(lp, rows, n_tokens, 4))) ||
+      (entropy && !fits(entropy, rows, 1, 4)) ||
+      (top_n && (!fits(top, rows, top_n, 4) || !fits(top_lp, rows, top_n, 4)))) {
+    set_error(err, "%s: a buffer is smaller than its stated matrix.", what);
+    return -3;
+  }
+  const size_t given_bytes = size_t(rows) * n_tokens * 4, top_bytes = size_t(rows) * top_n * 4;
+  const Use u_tokens{n_tokens ? tokens : nullptr, given_bytes}, u_lp{n_tokens ? lp : nullptr, given_bytes},
+      u_entropy{entropy, size_t(rows) * 4}, u_top{top_n ? top : nullptr, top_bytes},
+      u_top_lp{top_n ? top_lp : nullptr, top_bytes};
+  if (int rc = prepare_buffers(what, {{x, used}, u_tokens}, {u_lp, u_entropy, u_top, u_top_lp}, err)) return rc;
+  Device& d = g_dev[x->device];
+  for (const Use& u : {u_lp, u_entropy, u_top, u_top_lp})
+    if (!keep_rest(d, u)) {
+      cudaGetLastError();
+      set_error(err, "%s: host to device copy failed.", what);
+      return -6;
+    }
+  gonn::LogprobArgs a;
+  a.x = x->dptr;
+  a.rows = uint64_t(rows);
+  a.vocab = uint64_t(vocab);
+  a.ld = uint64_t(ld);
+  a.n_tokens = uint32_t(n_tokens);
+  a.top_n = uint32_t(top_n);
+  if (n_tokens) {
+    a.tokens = reinterpret_cast<const int*>(tokens->dptr);
+    a.logprobs = lp->dptr;
+  }
+  if (entropy) a.entropy = entropy->dptr;
+  if (top_n) {
+    a.top_tokens = reinterpret_cast<int*>(top->dptr);
+    a.top_logprobs = top_lp->dptr;
+  }
+  a.status = d.status_dev;
+  if (gonn::launch_token_logprobs(a, d.sm_count, d.stream) != cudaSuccess) {
+    set_error(err, "%s: launch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
+    return -4;
+  }
+  ++g_stats[3];
+  for (const Use& u : {u_lp, u_entropy, u_top, u_top_lp})
+    if (u.b) wrote(u.b);
+  return finish(d, err, -6, what);
+}
+
+namespace {
+struct DistillCall {
+  GPUPtr logits;
+  long rows, vocab, ld;
+  GPUPtr teacher_tokens, teacher_logits;
+  int top_n;
+  GPUPtr labels;
+  float temperature, soft_weight;
+  GPUPtr loss, stats, grad_loss;
+  float grad_scale;
+  GPUPtr grad;
+  long ld_grad;
+};
+
+int distill_core(gonn::DistillPass pass, const char* what, const DistillCall& c, CError* err) {
+  using gonn::DistillPass;
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  if (c.rows <= 0 || c.vocab <= 0 || c.vocab > kMaxVocab || c.rows > kMaxVocab || c.ld < c.vocab ||
+      c.top_n < 0 || c.top_n > gonn::kMaxTop || (pass != DistillPass::Forward && c.ld_grad < c.vocab)) {
+    set_error(err, "%s: bad dimensions: rows %ld, vocabulary %ld, row pitch %ld, %d teacher logits (at most %d).",
+              what, c.rows, c.vocab, c.ld, c.top_n, gonn::kMaxTop);
+    return -3;
+  }
+  // written so that a NaN is refused too
+  if (!(c.temperature >= 1e-6f && c.temperature <= 1e6f) || !(c.soft_weight >= 0.f && c.soft_weight <= 1.f) ||
+      !(c.grad_scale - c.grad_scale == 0.f)) {
+    set_error(err, "%s: the temperature must lie in [1e-6, 1e6], the soft weight in [0, 1], and the gradient "
+                   "scale must be finite.", what);
+    return -3;
+  }
+  Buffer *x = as_buffer(c.logits), *tt, *tl, *labels, *loss, *stats, *gl, *grad;
+  if (!x || !optional_buffer(c.teacher_tokens, &tt) || !optional_buffer(c.teacher_logits, &tl) ||
+      !optional_buffer(c.labels, &labels) || !optional_buffer(c.loss, &loss) ||
+      !optional_buffer(c.stats, &stats) || !optional_buffer(c.grad_loss, &gl) ||
+      !optional_buffer(c.grad, &grad)) {
+    set_error(err, "%s: invalid buffer pointers.", what);
+    return -2;
+  }
+  const bool soft = c.soft_weight > 0.f, hard = c.soft_weight < 1.f;
+  const bool want_loss = pass != DistillPass::Backward, want_grad = pass != DistillPass::Forward;
+  if ((soft && (c.top_n == 0 || !tt || !tl)) || (hard && !labels) || (want_loss && !loss) ||
+      (pass == DistillPass::Backward && !stats) || (want_grad && !grad)) {
+    set_error(err, "%s: a soft weight above 0 needs the teacher's tokens and logits, one below 1 the labels, and "
+                   "every result its buffer.", what);
+    return -2;
+  }
+  if (!soft) tt = tl = nullptr;
+  if (!hard) labels = nullptr;
+  const uint32_t top = soft ? uint32_t(c.top_n) : 0;
+  auto pitched = [&](long ld) {
+    return (unsigned __int128)(c.rows - 1) * (unsigned __int128)ld * 4 + size_t(c.vocab) * 4;
+  };
+  if (pitched(c.ld) > x->bytes || (want_grad && pitched(c.ld_grad) > grad->bytes) ||
+      (soft && (!fits(tt, c.rows, top, 4) || !fits(tl, c.rows, top, 4))) ||
+      (labels && !fits(labels, c.rows, 1, 4)) || (loss && !fits(loss, c.rows, 1, 4)) ||
+      (stats && !fits(stats, c.rows, 3, 4)) || (gl && !fits(gl, c.rows, 1, 4))) {
+    set_error(err, "%s: a buffer is smaller than its stated matrix.", what);
+    return -3;
+  }
+  const bool in_place = want_grad && grad->dptr == x->dptr;
+  if (in_place && c.ld_grad != c.ld) {
+    set_error(err, "%s: a gradient in the place of the logits must have their row pitch.", what);
+    return -3;
+  }
+  const size_t n4 = size_t(c.rows) * 4;
+  const Use u_x{x, size_t(pitched(c.ld))}, u_tt{tt, n4 * top}, u_tl{tl, n4 * top}, u_lab{labels, n4},
+      u_gl{want_grad ? gl : nullptr, n4}, u_loss{want_loss ? loss : nullptr, n4},
+      u_grad{want_grad ? grad : nullptr, want_grad ? size_t(pitched(c.ld_grad)) : 0};
+  const Use stats_in{pass == DistillPass::Backward ? stats : nullptr, n4 * 3};
+  const Use stats_out{pass == DistillPass::Forward ? stats : nullptr, n4 * 3};
+  // in place, the gradient may cover the logits and nothing else
+  const Use x_in{x, in_place ? 0 : u_x.bytes};
+  if (int rc = prepare_buffers(what, {x_in, u_tt, u_tl, u_lab, u_gl, stats_in}, {u_loss, stats_out, u_grad}, err))
+    return rc;
+  Device& d = g_dev[x->device];
+  bool resident = true;
+  for (const Use& u : {u_loss, stats_out})
+    resident = resident && keep_rest(d, u);
+  // columns between the vocabulary and the row pitch stay as they were
+  if (u_grad.b && (c.ld_grad != c.vocab || !keep_rest(d, u_grad))) resident = resident && make_resident(d, grad);
+  if (!resident) {
+    cudaGetLastError();
+    set_error(err, "%s: host to device copy failed.", what);
+    return -6;
+  }
+  gonn::DistillArgs a;
+  a.x = x->dptr;
+  a.rows = uint64_t(c.rows);
+  a.vocab = uint64_t(c.vocab);
+  a.ld = uint64_t(c.ld);
+  a.top_n = top;
+  if (soft) {
+    a.teacher_tokens = reinterpret_cast<const int*>(tt->dptr);
+    a.teacher_logits = tl->dptr;
+  }
+  if (labels) a.labels = reinterpret_cast<const int*>(labels->dptr);
+  a.temperature = c.temperature;
+  a.soft_weight = c.soft_weight;
+  if (want_loss) a.loss = loss->dptr;
+  if (stats_out.b) a.stats = stats->dptr;
+  if (stats_in.b) a.stats_in = stats->dptr;
+  if (want_grad) {
+    if (gl) a.grad_loss = gl->dptr;
+    a.grad_scale = c.grad_scale;
+    a.grad = grad->dptr;
+    a.ld_grad = uint64_t(c.ld_grad);
+  }
+  a.status = d.status_dev;
+  if (gonn::launch_distill(pass, a, d.sm_count, d.stream) != cudaSuccess) {
+    set_error(err, "%s: launch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
+    return -4;
+  }
+  ++g_stats[3];
+  for (const Use& u : {u_loss, stats_out, u_grad})
+    if (u.b) wrote(u.b);
+  return finish(d, err, -6, what);
+}
+}  // namespace
+
+int gonngpu_distill_forward(GPUPtr logits, long rows, long vocab, long ld, GPUPtr teacherTokens,
+                            GPUPtr teacherLogits, int top_n, GPUPtr labels, float temperature,
+                            float soft_weight, GPUPtr loss, GPUPtr stats, CError* err) {
+  return distill_core(gonn::DistillPass::Forward, "distillation forward",
+                      {logits, rows, vocab, ld, teacherTokens, teacherLogits, top_n, labels, temperature,
+                       soft_weight, loss, stats, nullptr, 1.f, nullptr, 0}, err);
+}
+int gonngpu_distill_backward(GPUPtr logits, long rows, long vocab, long ld, GPUPtr teacherTokens,
+                             GPUPtr teacherLogits, int top_n, GPUPtr labels, float temperature,
+                             float soft_weight, GPUPtr stats, GPUPtr gradLoss, float grad_scale, GPUPtr grad,
+                             long ldGrad, CError* err) {
+  return distill_core(gonn::DistillPass::Backward, "distillation backward",
+                      {logits, rows, vocab, ld, teacherTokens, teacherLogits, top_n, labels, temperature,
+                       soft_weight, nullptr, stats, gradLoss, grad_scale, grad, ldGrad}, err);
+}
+int gonngpu_distill_step(GPUPtr logits, long rows, long vocab, long ld, GPUPtr teacherTokens,
+                         GPUPtr teacherLogits, int top_n, GPUPtr labels, float temperature,
+                         float soft_weight, GPUPtr gradLoss, float grad_scale, GPUPtr loss, GPUPtr grad,
+                         long ldGrad, CError* err) {
+  return distill_core(gonn::DistillPass::Step, "distillation step",
+                      {logits, rows, vocab, ld, teacherTokens, teacherLogits, top_n, labels, temperature,
+                       soft_weight, loss, nullptr, gradLoss, grad_scale, grad, ldGrad}, err);
+}
+
+// ---- microscaled 4-bit operands --------------------------------------------------------
+namespace {
+constexpr long kMaxDim = (1l << 31) - 1;
+bool packed_ok(const Buffer* b, long rows, long cols) {
+  return gonn::Mxfp4Layout(uint64_t(rows), uint64_t(cols)).bytes <= b->bytes;
+}
+bool dims_ok(long rows, long cols) {
+  // the second bound keeps every byte count of a matrix within 63 bits
+  return rows > 0 && cols > 0 && rows <= kMaxDim && cols <= kMaxDim && rows <= (1l << 60) / cols;
+}
+// The packed form is read in 16-byte pieces; memory that a caller wrapped can start anywhere.
+bool aligned16(const Buffer* b) { return (reinterpret_cast<uintptr_t>(b->dptr) & 15u) == 0; }
+}  // namespace
+
+long gonngpu_mxfp4_bytes(long rows, long cols) {
+  if (!dims_ok(rows, cols)) return -3;
+  return long(gonn::Mxfp4Layout(uint64_t(rows), uint64_t(cols)).bytes);
+}
+
+int gonngpu_mxfp4_quantize(GPUPtr srcPtr, long rows, long cols, int transposed, GPUPtr packedPtr, CError* err) {
+  static const char* const what = "MXFP4 quantisation";
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  if (!dims_ok(rows, cols)) {
+    set_error(err, "%s: bad dimensions %ld x %ld.", what, rows, cols);
+    return -3;
+  }
+  Buffer *src = as_buffer(srcPtr), *packed = as_buffer(packedPtr);
+  if (!src || !packed) {
+    set_error(err, "%s: invalid buffer pointers.", what);
+    return -2;
+  }
+  const long r = transposed ? cols : rows, c = transposed ? rows : cols;
+  if (!fits(src, rows, cols, 4) || !packed_ok(packed, r, c) || !aligned16(packed)) {
+    set_error(err, "%s: a buffer is smaller than its matrix of %ld x %ld (gonngpu_mxfp4_bytes), or the packed "
+                   "matrix does not start on 16 bytes.", what, rows, cols);
+    return -3;
+  }
+  const Use out{packed, size_t(gonn::Mxfp4Layout(uint64_t(r), uint64_t(c)).bytes)};
+  if (int rc = prepare_buffers(what, {{src, size_t(rows) * cols * 4}}, {out}, err)) return rc;
+  Device& d = g_dev[src->device];
+  if (!keep_rest(d, out)) {
+    cudaGetLastError();
+    set_error(err, "%s: host to device copy failed.", what);
+    return -6;
+  }
+  if (gonn::launch_mxfp4_quantize(src->dptr, uint64_t(rows), uint64_t(cols), transposed != 0, packed->dptr,
+                                  d.stream) != cudaSuccess) {
+    set_error(err, "%s: launch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
+    return -4;
+  }
+  ++g_stats[3];
+  wrote(packed);
+  return finish(d, err, -6, what);
+}
+
+int gonngpu_mxfp4_dequantize(GPUPtr packedPtr, long rows, long cols, GPUPtr dstPtr, CError* err) {
+  static const char* const what = "MXFP4 dequantisation";
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  if (!dims_ok(rows, cols)) {
+    set_error(err, "%s: bad dimensions %ld x %ld.", what, rows, cols);
+    return -3;
+  }
+  Buffer *packed = as_buffer(packedPtr), *dst = as_buffer(dstPtr);
+  if (!packed || !dst) {
+    set_error(err, "%s: invalid buffer pointers.", what);
+    return -2;
+  }
+  if (!fits(dst, rows, cols, 4) || !packed_ok(packed, rows, cols) || !aligned16(packed)) {
+    set_error(err, "%s: a buffer is smaller than its matrix of %ld x %ld (gonngpu_mxfp4_bytes), or the packed "
+                   "matrix does not start on 16 bytes.", what, rows, cols);
+    return -3;
+  }
+  const Use out{dst, size_t(rows) * cols * 4};
+  if (int rc = prepare_buffers(what, {{packed, size_t(gonngpu_mxfp4_bytes(rows, cols))}}, {out}, err)) return rc;
+  Device& d = g_dev[packed->device];
+  if (!keep_rest(d, out)) {
+    cudaGetLastError();
+    set_error(err, "%s: host to device copy failed.", what);
+    return -6;
+  }
+  if (gonn::launch_mxfp4_dequantize(packed->dptr, uint64_t(rows), uint64_t(cols), dst->dptr, d.stream) !=
+      cudaSuccess) {
+    set_error(err, "%s: launch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
+    return -4;
+  }
+  ++g_stats[3];
+  wrote(dst);
+  return finish(d, err, -6, what);
+}
+
+namespace {
+// Both products: `a` is the packed matrix [m, k], or with `a_float` the float32 one, which is
+// quantised into library scratch first.
+int mxfp4_product(const char* what, GPUPtr aPtr, bool a_float, long m, GPUPtr bPtr, long n, long k, GPUPtr biasPtr,
+                  int act, float act_param, GPUPtr cPtr, CError* err) {
+  std::lock_guard<std::recursive_mutex> lk(g_mu);
+  if (!dims_ok(m, k) || !dims_ok(n, k) || !dims_ok(m, n)) {
+    set_error(err, "%s: bad dimensions: %ld x %ld by %ld x %ld.", what, m, k, n, k);
+    return -3;
+  }
+  Buffer *a = as_buffer(aPtr), *b = as_buffer(bPtr), *c = as_buffer(cPtr), *bias;
+  if (!a || !b || !c || !optional_buffer(biasPtr, &bias)) {
+    set_error(err, "%s: invalid buffer pointers.", what);
+    return -2;
+  }
+  if (!(a_float ? fits(a, m, k, 4) : packed_ok(a, m, k) && aligned16(a)) || !packed_ok(b, n, k) ||
+      !aligned16(b) || !fits(c, m, n, 4) || (bias && !fits(bias, n, 1, 4))) {
+    set_error(err, "%s: a buffer is smaller than its matrix (%ld x %ld by %ld x %ld; gonngpu_mxfp4_bytes), or a "
+                   "packed matrix does not start on 16 bytes.", what, m, k, n, k);
+    return -3;
+  }
+  const gonn::Mxfp4Layout la{uint64_t(m), uint64_t(k)}, lb{uint64_t(n), uint64_t(k)};
+  const Use out{c, size_t(m) * n * 4};
+  if (int rc = prepare_buffers(what, {{a, a_float ? size_t(m) * k * 4 : size_t(la.bytes)}, {b, size_t(lb.bytes)},
+                                      {bias, size_t(n) * 4}}, {out}, err))
+    return rc;
+  Device& d = g_dev[c->device];
+  if (!keep_rest(d, out)) {
+    cudaGetLastError();
+    set_error(err, "%s: host to device copy failed.", what);
+    return -6;
+  }
+  gonn::Mxfp4Product p;
+  p.a = a->dptr;
+  p.b = b->dptr;
+  p.M = uint64_t(m);
+  p.N = uint64_t(n);
+  p.K = uint64_t(k);
+  p.c = c->dptr;
+  p.bias = bias ? bias->dptr : nullptr;
+  p.act = act;
+  p.act_param = act_param;
+  void* scratch = nullptr;
+  if (a_float) {
+    if (pool_alloc(c->device, &scratch, la.bytes) != cudaSuccess) {
+      cudaGetLastError();
+      set_error(err, "%s: could not allocate the packed operand.", what);
+      return -5;
+    }
+    if (gonn::launch_mxfp4_quantize(a->dptr, uint64_t(m), uint64_t(k), false, scratch, d.stream) != cudaSuccess) {
+      set_error(err, "%s: launch failed: %s", what, cudaGetErrorString(cudaGetLastError()));
+      pool_free(c->device, scratch, la.bytes);
+      return -4;
+    }
+    ++g_stats[3];
+    p.a = scratch;
+  }
+  const char* msg = gonn::launch_mxfp4_product(p, d.status_dev, d.sm_count, d.stream);
+  // whoever gets the scratch next is queued behind this product on the same stream
+  if (scratch) pool_free(c->device, scratch, la.bytes);
+  if (msg) {
+    cudaGetLastError();
+    set_error(err, "%s: %s", what, msg);
+    return -4;
+  }
+  ++g_stats[3];
+  ++g_stats[4];
+  wrote(c);
+  return finish(d, err, -6, what);
+}
+}  // namespace
+
+int gonngpu_mxfp4_matmul(GPUPtr a, long m, GPUPtr b, long n, long k, GPUPtr bias, int activation_type,
+                         float activation_param, GPUPtr c, CError* err) {
+  return mxfp4_product("MXFP4 product", a, false, m, b, n, k, bias, activation_type, activation_param, c, err);
+}
+int gonngpu_mxfp4_linear(GPUPtr x, long batch, long in_size, GPUPtr weights, long out_size, GPUPtr bias,
+                         int activation_type, float activation_param, GPUPtr y, CError* err) {
+  return mxfp4_product("MXFP4 linear", x, true, batch, weights, out_size, in_size, bias, activation_type,
+                       activation_param, y, err);
 }
 
 int gonngpu_column_sum(GPUPtr inPtr, long rows, long cols, GPUPtr outPtr, CError* err) {

@@ -147,6 +147,79 @@ void launch_softmax(const float* in_or_grad, const float* act, float* out, uint6
 // *out = min(*out, smallest i with b[i] == 0); the caller presets *out to ~0.
 void launch_first_zero(const float* b, uint64_t n, unsigned long long* out, cudaStream_t stream);
 
+// ---- row statistics over logits: log probabilities and distillation ----------------
+// Status code of a row's index that lies outside the vocabulary (`where`: INDEX_TOKEN,
+// INDEX_TEACHER or INDEX_LABEL, `tile`: the row, `kblock`: the index).
+constexpr uint32_t kStatusBadIndex = 7;
+enum IndexKind : uint32_t { INDEX_TOKEN = 0, INDEX_TEACHER = 1, INDEX_LABEL = 2 };
+constexpr int kMaxTop = 128;  // top alternatives of a row; a teacher's logits of a row
+
+struct LogprobArgs {
+  const float* x = nullptr;  // logits [rows, vocab], row pitch ld
+  uint64_t rows = 0, vocab = 0, ld = 0;
+  const int* tokens = nullptr;  // [rows, n_tokens] or null
+  uint32_t n_tokens = 0, top_n = 0;
+  float* logprobs = nullptr;      // [rows, n_tokens]
+  float* entropy = nullptr;       // [rows] or null
+  int* top_tokens = nullptr;      // [rows, top_n]
+  float* top_logprobs = nullptr;  // [rows, top_n]
+  GemmStatus* status = nullptr;
+};
+cudaError_t launch_token_logprobs(const LogprobArgs& a, int sm_count, cudaStream_t stream);
+
+struct DistillArgs {
+  const float* x = nullptr;  // the student's logits [rows, vocab], row pitch ld
+  uint64_t rows = 0, vocab = 0, ld = 0;
+  const int* teacher_tokens = nullptr;  // [rows, top_n]
+  const float* teacher_logits = nullptr;
+  uint32_t top_n = 0;
+  const int* labels = nullptr;  // [rows] or null
+  float temperature = 1.f, soft_weight = 1.f;
+  float* loss = nullptr;             // [rows] (forward, step)
+  float* stats = nullptr;            // [rows, 3]: max, sum e^((x-max)/T), sum e^(x-max)
+  const float* stats_in = nullptr;   // the same, read by the backward
+  const float* grad_loss = nullptr;  // [rows] or null
+  float grad_scale = 1.f;
+  float* grad = nullptr;  // [rows, vocab], row pitch ld_grad; may be x itself
+  uint64_t ld_grad = 0;
+  GemmStatus* status = nullptr;
+};
+// forward: loss (and stats); backward: grad from stats_in; step: loss and grad.
+enum class DistillPass : int { Forward = 0, Backward = 1, Step = 2 };
+cudaError_t launch_distill(DistillPass pass, const DistillArgs& a, int sm_count, cudaStream_t stream);
+
+// ---- microscaled 4-bit operands (MXFP4) ---------------------------------------------
+// A packed matrix [rows, cols]: blocks of 32 along a row share a scale 2^e; an element is an
+// e2m1 code.  The codes come first, two a byte (the even column in the low half), rows of
+// blocks*16 bytes; the scales follow at scale_offset, one byte e + 127 each (255: the block
+// holds a NaN or an infinity), in tiles of 128 rows x 4 blocks: byte
+// (row % 32) * 16 + (row % 128) / 32 * 4 + block % 4 of tile (row / 128, block / 4), the order in
+// which the tensor cores' scale memory takes them.  Scales outside the matrix are 0.
+struct Mxfp4Layout {
+  uint64_t rows, cols, blocks, groups, row_bytes, scale_offset, bytes;
+  Mxfp4Layout(uint64_t r, uint64_t c)
+      : rows(r), cols(c), blocks((c + 31) / 32), groups((blocks + 3) / 4), row_bytes(blocks * 16),
+        scale_offset((r * row_bytes + 511) / 512 * 512),
+        bytes(scale_offset + (r + 127) / 128 * groups * 512) {}
+};
+// src [rows, cols] float32 (dense) -> packed matrix of src, or with `transposed` of its transpose.
+cudaError_t launch_mxfp4_quantize(const float* src, uint64_t rows, uint64_t cols, bool transposed,
+                                  void* packed, cudaStream_t stream);
+// packed matrix [rows, cols] -> float32 (dense).
+cudaError_t launch_mxfp4_dequantize(const void* packed, uint64_t rows, uint64_t cols, float* dst,
+                                    cudaStream_t stream);
+struct Mxfp4Product {
+  const void* a = nullptr;  // packed [M, K]
+  const void* b = nullptr;  // packed [N, K]
+  uint64_t M = 0, N = 0, K = 0;
+  float* c = nullptr;           // [M, N] float32, dense
+  const float* bias = nullptr;  // [N] or null
+  int act = ACT_NONE;
+  float act_param = 0.f;
+};
+// C = act(A . B^T + bias).  Returns nullptr on success, else a static message.
+const char* launch_mxfp4_product(const Mxfp4Product& p, GemmStatus* status, int sm_count, cudaStream_t stream);
+
 // ---- replication of B over NVSwitch (row-sharded product) --------------------------
 // Control words every rank keeps at the same offset of its symmetric buffer.  arrived[s] is
 // the last epoch whose data is complete in slot s of this GPU (written by the owner);

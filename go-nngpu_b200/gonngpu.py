@@ -101,6 +101,23 @@ SIGNATURES = {
     "gonngpu_shard_plan": (_c_int, [_c_long, _c_int, _c_int, ctypes.POINTER(_c_long), ctypes.POINTER(_c_long)]),
     "gonngpu_linear_backward": (
         _c_int, [_vp, _vp, _vp, _vp, _c_long, _c_long, _c_long, _vp, _vp, _vp, _errp]),
+    "gonngpu_token_logprobs": (
+        _c_int, [_vp, _c_long, _c_long, _c_long, _vp, _c_long, _vp, _vp, _c_int, _vp, _vp, _errp]),
+    "gonngpu_distill_forward": (
+        _c_int, [_vp, _c_long, _c_long, _c_long, _vp, _vp, _c_int, _vp, _c_float, _c_float, _vp, _vp, _errp]),
+    "gonngpu_distill_backward": (
+        _c_int, [_vp, _c_long, _c_long, _c_long, _vp, _vp, _c_int, _vp, _c_float, _c_float, _vp, _vp, _c_float,
+                 _vp, _c_long, _errp]),
+    "gonngpu_distill_step": (
+        _c_int, [_vp, _c_long, _c_long, _c_long, _vp, _vp, _c_int, _vp, _c_float, _c_float, _vp, _c_float, _vp,
+                 _vp, _c_long, _errp]),
+    "gonngpu_mxfp4_bytes": (_c_long, [_c_long, _c_long]),
+    "gonngpu_mxfp4_quantize": (_c_int, [_vp, _c_long, _c_long, _c_int, _vp, _errp]),
+    "gonngpu_mxfp4_dequantize": (_c_int, [_vp, _c_long, _c_long, _vp, _errp]),
+    "gonngpu_mxfp4_matmul": (
+        _c_int, [_vp, _c_long, _vp, _c_long, _c_long, _vp, _c_int, _c_float, _vp, _errp]),
+    "gonngpu_mxfp4_linear": (
+        _c_int, [_vp, _c_long, _c_long, _vp, _c_long, _vp, _c_int, _c_float, _vp, _errp]),
     "gonngpu_column_sum": (_c_int, [_vp, _c_long, _c_long, _vp, _errp]),
     "gonngpu_alloc_device_buffer": (_c_int, [_c_long, ctypes.POINTER(_vp), _errp]),
     "gonngpu_wrap_device_memory": (_c_int, [_vp, _c_long, ctypes.POINTER(_vp), _errp]),
@@ -177,6 +194,11 @@ class Buffer:
         return cls(h, a.nbytes, a)
 
     @classmethod
+    def from_host_int32(cls, array):
+        """The same over int32 data (token numbers, labels)."""
+        return cls.from_host(np.ascontiguousarray(array, dtype=np.int32).view(np.float32))
+
+    @classmethod
     def empty(cls, nbytes):
         h, err = _vp(), CError()
         _check(lib().gonngpu_alloc_device_buffer(int(nbytes), ctypes.byref(h), ctypes.byref(err)), err)
@@ -216,6 +238,16 @@ class Buffer:
     def retrieve_into(self, out):
         err = CError()
         _check(lib().retrieve_gpu_buffer_data(self.handle, _np_ptr(out), out.nbytes, ctypes.byref(err)), err)
+
+    def retrieve_int32(self, shape):
+        out = np.empty(shape, dtype=np.int32)
+        self.retrieve_into(out)
+        return out
+
+    def retrieve_bytes(self):
+        out = np.empty(self.nbytes, dtype=np.uint8)
+        self.retrieve_into(out)
+        return out
 
     def device_address(self):
         return lib().gonngpu_device_address(self.handle)
@@ -410,6 +442,79 @@ def batch_matmul(a, b, c, batch, m, n, k):
     err = CError()
     _check(lib().perform_batch_matmul_optimized(a.handle, b.handle, c.handle, batch, m, n, k, None,
                                                 ctypes.byref(err)), err)
+
+
+def _handle(buffer):
+    return buffer.handle if buffer is not None else None
+
+
+def token_logprobs(logits, rows, vocab, tokens=None, n_tokens=0, logprobs=None, entropy=None, top_n=0,
+                   top_tokens=None, top_logprobs=None, ld=None):
+    """Log probabilities of given tokens, entropy and top alternatives of every row of logits."""
+    err = CError()
+    _check(lib().gonngpu_token_logprobs(
+        logits.handle, rows, vocab, vocab if ld is None else ld, _handle(tokens), n_tokens, _handle(logprobs),
+        _handle(entropy), top_n, _handle(top_tokens), _handle(top_logprobs), ctypes.byref(err)), err)
+
+
+def distill_forward(logits, rows, vocab, teacher_tokens, teacher_logits, top_n, labels, temperature, soft_weight,
+                    loss, stats=None, ld=None):
+    err = CError()
+    _check(lib().gonngpu_distill_forward(
+        logits.handle, rows, vocab, vocab if ld is None else ld, _handle(teacher_tokens), _handle(teacher_logits),
+        top_n, _handle(labels), temperature, soft_weight, _handle(loss), _handle(stats), ctypes.byref(err)), err)
+
+
+def distill_backward(logits, rows, vocab, teacher_tokens, teacher_logits, top_n, labels, temperature, soft_weight,
+                     stats, grad, grad_loss=None, grad_scale=1.0, ld=None, ld_grad=None):
+    err = CError()
+    _check(lib().gonngpu_distill_backward(
+        logits.handle, rows, vocab, vocab if ld is None else ld, _handle(teacher_tokens), _handle(teacher_logits),
+        top_n, _handle(labels), temperature, soft_weight, _handle(stats), _handle(grad_loss), grad_scale,
+        _handle(grad), vocab if ld_grad is None else ld_grad, ctypes.byref(err)), err)
+
+
+def distill_step(logits, rows, vocab, teacher_tokens, teacher_logits, top_n, labels, temperature, soft_weight,
+                 loss, grad, grad_loss=None, grad_scale=1.0, ld=None, ld_grad=None):
+    """Loss and gradient of a training step in one pass over the logits."""
+    err = CError()
+    _check(lib().gonngpu_distill_step(
+        logits.handle, rows, vocab, vocab if ld is None else ld, _handle(teacher_tokens), _handle(teacher_logits),
+        top_n, _handle(labels), temperature, soft_weight, _handle(grad_loss), grad_scale, _handle(loss),
+        _handle(grad), vocab if ld_grad is None else ld_grad, ctypes.byref(err)), err)
+
+
+def mxfp4_bytes(rows, cols):
+    n = lib().gonngpu_mxfp4_bytes(rows, cols)
+    if n < 0:
+        raise GonnError(n, "bad dimensions of a packed matrix")
+    return n
+
+
+def mxfp4_quantize(src, rows, cols, transposed, packed):
+    """float32 [rows, cols] -> packed 4-bit matrix, of its transpose with `transposed`."""
+    err = CError()
+    _check(lib().gonngpu_mxfp4_quantize(src.handle, rows, cols, int(transposed), packed.handle, ctypes.byref(err)),
+           err)
+
+
+def mxfp4_dequantize(packed, rows, cols, dst):
+    err = CError()
+    _check(lib().gonngpu_mxfp4_dequantize(packed.handle, rows, cols, dst.handle, ctypes.byref(err)), err)
+
+
+def mxfp4_matmul(a, m, b, n, k, c, bias=None, act=ACT_NONE, act_param=0.0):
+    """C[m, n] = act(A . B^T + bias) for packed A [m, k] and B [n, k]."""
+    err = CError()
+    _check(lib().gonngpu_mxfp4_matmul(a.handle, m, b.handle, n, k, _handle(bias), act, act_param, c.handle,
+                                      ctypes.byref(err)), err)
+
+
+def mxfp4_linear(x, batch, in_size, weights, out_size, bias, act, act_param, y):
+    """y = act(Q(x) . W^T + bias) for packed weights [out_size, in_size]."""
+    err = CError()
+    _check(lib().gonngpu_mxfp4_linear(x.handle, batch, in_size, weights.handle, out_size, _handle(bias), act,
+                                      act_param, y.handle, ctypes.byref(err)), err)
 
 
 def column_sum(inp, rows, cols, out):

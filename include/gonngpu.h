@@ -385,6 +385,101 @@ GONNGPU_API int gonngpu_matmul_f16_static_scratch(const float *a, long aRows, lo
 GONNGPU_API int gonngpu_linear_backward(GPUPtr x, GPUPtr w, GPUPtr dy, GPUPtr actOut, long batch, long in_size,
                             long out_size, GPUPtr dx, GPUPtr dw, GPUPtr db, CError *err);
 
+/* ---- rows of logits: log probabilities and distillation ---------------------
+ * No counterpart in the reference; they stand beside its row softmax
+ * (perform_activation_softmax_2d_*).  Logits are float32 [rows, vocab] with a
+ * row pitch of `ld` >= vocab elements; token and label buffers hold int32.  A
+ * logit of -inf is a masked token (probability 0).  A row that holds a NaN or
+ * +inf gives NaN (alternatives: token -1).  Token numbers below 0 mean "none"; one that is not
+ * below vocab is treated as none (a log probability: NaN) and reported: -3, by
+ * this call in blocking mode, else by gonngpu_synchronize.  Result buffers must
+ * not overlap other buffers of the call.  Errors: -1 device, -2 bad or missing
+ * buffer, -3 dimensions, sizes, parameters or token numbers, -4 launch, -6
+ * execution. */
+
+/* At most this many alternatives, or teacher logits, per row. */
+#define GONNGPU_MAX_TOP 128
+
+/* Under softmax(logits[r]):
+ *   logprobs[r,t]  = log p(tokens[r,t]), t < n_tokens; 0 where the token is
+ *                    none, -inf where it is masked
+ *   entropy[r]     = -sum p log p (NULL: not wanted; 0 for a row that is masked
+ *                    as a whole)
+ *   top_tokens[r,k], top_logprobs[r,k] = the top_n largest logits in descending
+ *                    order, equal ones by ascending token, with their log
+ *                    probabilities.  Masked tokens follow the others, as -inf.
+ * `tokens` and `logprobs` may be NULL when n_tokens is 0, the last two when
+ * top_n is 0 (top_n <= min(vocab, GONNGPU_MAX_TOP)). */
+GONNGPU_API int gonngpu_token_logprobs(GPUPtr logits, long rows, long vocab, long ld, GPUPtr tokens,
+                           long n_tokens, GPUPtr logprobs, GPUPtr entropy, int top_n,
+                           GPUPtr top_tokens, GPUPtr top_logprobs, CError *err);
+
+/* Distillation of a student's logits x from a teacher's top logits z:
+ *   q = softmax(z / T) over the row's teacher tokens, p_T = softmax(x / T), p = softmax(x)
+ *   loss[r] = w T^2 sum_k q_k (log q_k - log p_T[token_k]) + (1 - w) (-log p[label])
+ *   grad[r,j] = g_r (w T (p_T[j] - sum_{k: token_k = j} q_k) + (1 - w) (p[j] - [j = label]))
+ * with T = temperature, w = soft_weight in [0, 1] and g_r = grad_scale * gradLoss[r]
+ * (gradLoss NULL: 1).  Teacher entries whose token is none or whose logit is
+ * -inf are left out; a row without any, or without a label, lacks that term; a
+ * row whose logits are all masked has loss and gradient 0.  A token may be
+ * named twice: the entries add up.  A NaN or +inf among a row's logits or teacher
+ * logits makes its loss and gradient NaN.  The teacher's buffers ([rows, top_n]) may be
+ * NULL when w is 0, the labels ([rows]) when w is 1.  Any constant may be added
+ * to a row of z, so log probabilities (gonngpu_token_logprobs) serve as well.
+ *
+ * forward writes loss and, unless NULL, stats[r] = {max x, sum e^((x-max)/T),
+ * sum e^(x-max)}, which the backward takes; step does both in one pass over the
+ * logits.  `grad` may be `logits` itself (same row pitch); the columns between
+ * vocab and ldGrad stay as they were. */
+GONNGPU_API int gonngpu_distill_forward(GPUPtr logits, long rows, long vocab, long ld, GPUPtr teacherTokens,
+                            GPUPtr teacherLogits, int top_n, GPUPtr labels, float temperature,
+                            float soft_weight, GPUPtr loss, GPUPtr stats, CError *err);
+GONNGPU_API int gonngpu_distill_backward(GPUPtr logits, long rows, long vocab, long ld, GPUPtr teacherTokens,
+                             GPUPtr teacherLogits, int top_n, GPUPtr labels, float temperature,
+                             float soft_weight, GPUPtr stats, GPUPtr gradLoss, float grad_scale,
+                             GPUPtr grad, long ldGrad, CError *err);
+GONNGPU_API int gonngpu_distill_step(GPUPtr logits, long rows, long vocab, long ld, GPUPtr teacherTokens,
+                         GPUPtr teacherLogits, int top_n, GPUPtr labels, float temperature,
+                         float soft_weight, GPUPtr gradLoss, float grad_scale, GPUPtr loss, GPUPtr grad,
+                         long ldGrad, CError *err);
+
+/* ---- microscaled 4-bit operands (MXFP4) ---------------------------------------
+ * The next precision below the fp16 path; no counterpart in the reference.  A
+ * block of 32 elements along a row shares a scale 2^e, e = floor(log2 max|x|) - 2
+ * (at least -127), and keeps x / 2^e as a 4-bit code: sign and 0, .5, 1, 1.5, 2,
+ * 3, 4 or 6, nearest, ties to even, larger magnitudes as 6.  A block that holds a
+ * NaN or an infinity stands for NaN as a whole.
+ *
+ * A packed matrix [rows, cols] is one buffer of gonngpu_mxfp4_bytes(rows, cols)
+ * bytes, 16-byte aligned: rows of ceil(cols/32)*16 code bytes (the even column
+ * in a byte's low half), then, from the next multiple of 512 bytes, one scale
+ * byte e + 127 per block (255: NaN) in tiles of 128 rows x 4 blocks of 512 bytes,
+ * tile (row/128, block/4) row-major, byte (row%32)*16 + (row%128)/32*4 + block%4.
+ * Codes past the last column and scales outside the matrix are 0 (a packed
+ * matrix from elsewhere must keep to that: the product reads them).
+ * Errors: -1 device, -2 bad buffer, -3 dimensions, sizes or alignment, -4
+ * launch, -5 scratch allocation, -6 execution; gonngpu_mxfp4_bytes: -3. */
+GONNGPU_API long gonngpu_mxfp4_bytes(long rows, long cols);
+/* float32 src [rows, cols] -> packed [rows, cols], or, with `transposed` != 0, the
+ * packed matrix [cols, rows] of its transpose (a layer's weights [in, out],
+ * scaled in blocks along `in`, become the [out, in] operand of the products). */
+GONNGPU_API int gonngpu_mxfp4_quantize(GPUPtr src, long rows, long cols, int transposed, GPUPtr packed,
+                           CError *err);
+/* packed [rows, cols] -> float32, the values that the codes stand for (what the
+ * backward pass of a layer with 4-bit weights multiplies by). */
+GONNGPU_API int gonngpu_mxfp4_dequantize(GPUPtr packed, long rows, long cols, GPUPtr dst, CError *err);
+/* C[m,n] = act(A[m,k] . B[n,k]^T + bias[n]) for packed A and B, C float32;
+ * accumulated in 32 bits.  `bias` may be NULL; activation_type as for
+ * perform_fused_linear_activation (GONNGPU_ACT_NONE: identity). */
+GONNGPU_API int gonngpu_mxfp4_matmul(GPUPtr a, long m, GPUPtr b, long n, long k, GPUPtr bias,
+                         int activation_type, float activation_param, GPUPtr c, CError *err);
+/* The 4-bit form of perform_fused_linear_activation: x [batch, in_size] float32 is
+ * quantised (blocks along in_size) and multiplied by packed weights [out_size,
+ * in_size]; y [batch, out_size] float32. */
+GONNGPU_API int gonngpu_mxfp4_linear(GPUPtr x, long batch, long in_size, GPUPtr weights, long out_size,
+                         GPUPtr bias, int activation_type, float activation_param, GPUPtr y,
+                         CError *err);
+
 /* out[j] = sum_i in[i,j] (bias gradient, gpu/matrix/layers.go:281-294). */
 GONNGPU_API int gonngpu_column_sum(GPUPtr in, long rows, long cols, GPUPtr out, CError *err);
 
