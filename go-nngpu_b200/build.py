@@ -10,8 +10,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libgonngpu_cuda.so")
 SOURCES = ["gemm_sm100.cu", "hbm_kernels.cu", "elementwise.cu", "bridge.cu", "static_scratch.cu",
-           "replicate.cu", "logits.cu", "mxfp4.cu"]
-HEADERS = ["ptx.cuh", "kernels.h", "launch.cuh", "activation.cuh", "mxfp4.cuh", os.path.join("..", "..", "include", "gonngpu.h")]
+           "replicate.cu", "logits.cu", "mxfp4.cu", "mxfp4_gemm.cu"]
+HEADERS = ["ptx.cuh", "kernels.h", "launch.cuh", "activation.cuh", "mxfp4.cuh", "status.cuh", "tmap.h",
+           os.path.join("..", "..", "include", "gonngpu.h")]
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -28,6 +28,8 @@
 #include "kernels.h"
 #include "launch.cuh"
 #include "ptx.cuh"
+#include "status.cuh"
+#include "tmap.h"
 
 namespace gonn {
 
@@ -177,27 +179,6 @@ __device__ __forceinline__ void load_bf16_planes(uint32_t mn_major, const CUtens
                                                  int32_t tile, int32_t kb, uint32_t bar) {
   if (mn_major) ptx::tma_load_4d_pair(dst, m, 0, kb * 32, tile * 2, 0, bar);
   else ptx::tma_load_3d_pair(dst, m, kb * 32, tile * 128, 0, bar);
-}
-
-// Raises the CTA's abort flag; true for the one role that raised it.  Only that role reports:
-// the roles that leave because they SAW the flag would otherwise overwrite the cause with
-// their own, later, wait (the status words live in mapped host memory, where "write only if
-// still zero" cannot tell a report of a microsecond ago from none).
-__device__ __forceinline__ bool first_to_give_up(volatile uint32_t* abort_flag) {
-  return atomicExch(const_cast<uint32_t*>(abort_flag), 1u) == 0u;
-}
-
-__device__ __forceinline__ void report(GemmStatus* st, uint32_t code, uint32_t where,
-                                       uint32_t tile, uint32_t kb) {
-  // `st` may be page-locked host memory mapped into the device: plain stores
-  // only (the first reporter wins most of the time, which is all that is needed).
-  volatile GemmStatus* v = st;
-  if (v->code == 0u) {
-    v->where = where;
-    v->tile = tile;
-    v->kblock = kb;
-    v->code = code;
-  }
 }
 
 // alpha * acc + beta * C_in + bias, then the activation, for four neighbouring columns;
@@ -1919,6 +1900,21 @@ CUresult encode_cached(CUtensorMap* map, CUtensorMapDataType dtype, cuuint32_t r
 }
 
 EncodeTiledFn encode_tiled() { return encode_tiled_driver() ? &encode_cached : nullptr; }
+
+}  // namespace
+
+bool encode_tensor_map(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank, const void* base,
+                       const uint64_t* dims, const uint64_t* strides, const uint32_t* box,
+                       CUtensorMapSwizzle swizzle) {
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return rank <= 4 && encode_cached(map, dtype, rank, const_cast<void*>(base),
+                                    reinterpret_cast<const cuuint64_t*>(dims),
+                                    reinterpret_cast<const cuuint64_t*>(strides), box, estr,
+                                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+namespace {
 
 // 2-D map over a row-major plane: `inner` contiguous elements per row, `outer`
 // rows, boxes of (128 bytes, box_rows) written with the 128-byte swizzle.

@@ -1,7 +1,6 @@
-// Microscaled 4-bit operands (MXFP4: e2m1 codes, one power-of-two scale for 32 of them) and the
-// product on them, C = act(A . B^T + bias).  The next precision below the fp16 path, no
-// counterpart in the reference.
-#include "activation.cuh"
+// Microscaled 4-bit operands (MXFP4: e2m1 codes, one power-of-two scale for 32 of them):
+// quantisation and back.  The next precision below the fp16 path, no counterpart in the
+// reference; the product is in mxfp4_gemm.cu.
 #include "kernels.h"
 #include "launch.cuh"
 #include "mxfp4.cuh"
@@ -59,30 +58,6 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
   }
 }
 
-// One thread per output.
-__global__ void __launch_bounds__(256) product_kernel(const Mxfp4Product p, Mxfp4Layout la, Mxfp4Layout lb) {
-  ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
-  ptx::grid_dependency_wait();
-  const uint8_t* a = static_cast<const uint8_t*>(p.a);
-  const uint8_t* b = static_cast<const uint8_t*>(p.b);
-  for (uint64_t i = blockIdx.x * uint64_t(blockDim.x) + threadIdx.x; i < p.M * p.N;
-       i += uint64_t(gridDim.x) * blockDim.x) {
-    const uint64_t m = i / p.N, n = i % p.N;
-    float sum = 0.f;
-    for (uint64_t k = 0; k < la.blocks; ++k) {
-      float part = 0.f;  // exact: multiples of 1/4 below 2^11
-      for (int j = 0; j < 16; ++j) {
-        const uint32_t x = a[m * la.row_bytes + k * 16 + j], y = b[n * lb.row_bytes + k * 16 + j];
-        part += decode(x & 15u) * decode(y & 15u) + decode(x >> 4) * decode(y >> 4);
-      }
-      sum += part * scale_value(a[la.scale_offset + scale_at(m, k, la.groups)]) *
-             scale_value(b[lb.scale_offset + scale_at(n, k, lb.groups)]);
-    }
-    if (p.bias) sum += p.bias[n];
-    p.c[i] = apply_act(sum, p.act, p.act_param);
-  }
-}
-
 uint32_t grid_for(uint64_t items, uint32_t per_block, uint32_t most) {
   const uint64_t n = (items + per_block - 1) / per_block;
   return uint32_t(n < most ? n : most);
@@ -104,14 +79,6 @@ cudaError_t launch_mxfp4_dequantize(const void* packed, uint64_t rows, uint64_t 
   const Mxfp4Layout l(rows, cols);
   return launch_kernel(dequantize_kernel, dim3(grid_for(rows * cols, 256, 148 * 16)), dim3(256), 0, stream,
                        static_cast<const uint8_t*>(packed), l, dst);
-}
-
-const char* launch_mxfp4_product(const Mxfp4Product& p, GemmStatus*, int, cudaStream_t stream) {
-  const Mxfp4Layout la(p.M, p.K), lb(p.N, p.K);
-  if (launch_kernel(product_kernel, dim3(grid_for(p.M * p.N, 256, 148 * 16)), dim3(256), 0, stream, p, la, lb) !=
-      cudaSuccess)
-    return "launch failed";
-  return nullptr;
 }
 
 }  // namespace gonn

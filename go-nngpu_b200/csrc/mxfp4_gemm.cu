@@ -1,0 +1,539 @@
+// C = act(A . B^T + bias) on packed MXFP4 operands (layout: Mxfp4Layout in kernels.h), on the
+// block-scaled 4-bit form of the tensor cores (tcgen05.mma kind::mxf4): 64 of K an instruction,
+// one scale byte for 32 of K, both scales applied by the tensor core, fp32 accumulators in TMEM.
+//
+// The rows of B (a layer's outputs) are the rows of the instruction's result and the rows of A
+// (the batch) its columns: a warp that reads the accumulators holds 32 neighbouring outputs of
+// one batch row in each register, so that every store covers 128 contiguous bytes of C whatever N
+// and its alignment, and a batch of a few rows wastes columns of a narrow tile and not rows of a
+// tall one.
+//
+// Shared memory holds stages of 256 of K: 128 bytes of codes per row, fetched by TMA with the
+// 128-byte swizzle, and the scales of 128 rows as two tiles of 512 bytes, which tcgen05.cp moves
+// into TMEM right before the MMAs that read them.  Each stage has its own place for scales in
+// TMEM: it is written again only after the stage's barrier has seen the MMAs retire.
+#include <algorithm>
+#include <cstring>
+
+#include "activation.cuh"
+#include "kernels.h"
+#include "launch.cuh"
+#include "ptx.cuh"
+#include "status.cuh"
+#include "tmap.h"
+
+namespace gonn {
+
+namespace {
+
+constexpr uint32_t ROWS = 128;                 // rows of B in a CTA's tile
+constexpr uint32_t STAGE_K_BYTES = 128;        // code bytes of a row in a stage: 256 of K
+constexpr uint32_t STEPS = 4;                  // MMAs (64 of K) a stage
+constexpr uint32_t ROW_CODES = ROWS * STAGE_K_BYTES;
+constexpr uint32_t SCALE_TILE = 512;           // scales of 128 rows x 128 of K
+constexpr uint32_t SMEM_LIMIT = 227 * 1024;
+
+struct Params {
+  uint32_t M, N;          // rows of A (columns of the tile), rows of B (rows of the tile)
+  uint32_t tiles_n, tiles_m, num_tiles;
+  uint32_t kblocks, ksteps;          // stages and MMAs along K
+  uint32_t splits, kb_per_split;     // single-CTA kernel: work units of a tile along K
+  float* c;
+  const float* bias;
+  int act;
+  float act_param;
+  float* ws;              // partial sums of split tiles: [unit][column][128]
+  uint32_t* counters;     // one per tile, zero between launches
+  GemmStatus* status;
+};
+
+// Scales: no swizzle, groups of 8 rows of 16 bytes 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
+  return ptx::smem_desc(0, 0, 128) | uint64_t(addr >> 4);
+}
+// Codes: K-major, 128-byte swizzle, groups of 8 rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t code_desc(uint32_t addr) {
+  return ptx::smem_desc(2, 16, 1024) | uint64_t(addr >> 4);
+}
+
+__device__ __forceinline__ void wait_out(volatile uint32_t* abort_flag) {
+  if (!*abort_flag) return;
+  // a role gave up: give copies and MMAs in flight time to land
+  const uint64_t t0 = ptx::globaltimer_ns();
+  for (uint32_t i = 0; i < (1u << 16); ++i) {
+    if (ptx::globaltimer_ns() - t0 > 2000000ull) break;
+    __nanosleep(1000);
+  }
+}
+
+// ---- one CTA per tile of 128 outputs x BN batch rows, or per share of its K -------------
+// Warp 0 loads, warp 1 issues the MMAs, warps 2-5 read the accumulators out.
+constexpr uint32_t SINGLE_THREADS = 192;
+
+template <int BN, int STAGES>
+struct SingleShape {
+  static constexpr uint32_t COL_CODES = BN * STAGE_K_BYTES;
+  static constexpr uint32_t STAGE = ROW_CODES + COL_CODES + 4 * SCALE_TILE;
+  static constexpr uint32_t SMEM = STAGES * STAGE + 1024 + 256;
+  static constexpr uint32_t USED = BN + STAGES * 16;
+  static constexpr uint32_t TMEM = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+};
+
+template <int BN, int STAGES>
+__global__ void __launch_bounds__(SINGLE_THREADS)
+mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_constant__ CUtensorMap tm_row_scales,
+                    const __grid_constant__ CUtensorMap tm_cols, const __grid_constant__ CUtensorMap tm_col_scales,
+                    const __grid_constant__ Params p) {
+  using S = SingleShape<BN, STAGES>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
+  const uint32_t base = raw + pad;
+  const uint32_t bar_base = base + STAGES * S::STAGE;
+  auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (STAGES + s); };
+  const uint32_t done_bar = bar_base + 8u * (2 * STAGES);
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem_raw + pad + STAGES * S::STAGE + 8 * (2 * STAGES + 1));
+  uint32_t* tmem_slot = words;
+  volatile uint32_t* abort_flag = words + 1;
+  volatile uint32_t* last_flag = words + 2;
+
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t tile = blockIdx.x / p.splits, split = blockIdx.x - tile * p.splits;
+  const uint32_t tn = tile % p.tiles_n, tm = tile / p.tiles_n;
+  const uint32_t kb0 = split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.kblocks);
+
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    ptx::mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::prefetch_tmap(&tm_rows);
+    ptx::prefetch_tmap(&tm_row_scales);
+    ptx::prefetch_tmap(&tm_cols);
+    ptx::prefetch_tmap(&tm_col_scales);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(tmem_slot), S::TMEM);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  ptx::grid_dependency_release();
+  ptx::grid_dependency_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      for (uint32_t kb = kb0; kb < kb1; ++kb) {
+        if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
+          if (first_to_give_up(abort_flag)) report(p.status, 1, stage, tile, kb);
+          break;
+        }
+        const uint32_t fb = full_bar(stage), dst = base + stage * S::STAGE;
+        ptx::mbar_arrive_expect_tx(fb, S::STAGE);
+        ptx::tma_load_2d(dst, &tm_rows, int32_t(kb * STAGE_K_BYTES), int32_t(tn * ROWS), fb);
+        ptx::tma_load_2d(dst + ROW_CODES, &tm_cols, int32_t(kb * STAGE_K_BYTES), int32_t(tm * BN), fb);
+        const uint32_t scales = dst + ROW_CODES + S::COL_CODES;
+        ptx::tma_load_3d(scales, &tm_row_scales, 0, int32_t(kb * 2), int32_t(tn), fb);
+        // a tile narrower than 128 is the only one along M
+        ptx::tma_load_3d(scales + 2 * SCALE_TILE, &tm_col_scales, 0, int32_t(kb * 2),
+                         BN == 128 ? int32_t(tm) : 0, fb);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc0 = ptx::make_idesc_mxf4(ROWS, BN, 0), idesc1 = ptx::make_idesc_mxf4(ROWS, BN, 1);
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (uint32_t kb = kb0; kb < kb1; ++kb) {
+        if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag)) {
+          if (first_to_give_up(abort_flag)) report(p.status, 2, stage, tile, kb);
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        const uint32_t src = base + stage * S::STAGE, scales = src + ROW_CODES + S::COL_CODES;
+        const uint32_t ts = tmem + BN + stage * 16;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) ptx::tmem_cp_scales<false>(ts + j * 4, scale_desc(scales + j * SCALE_TILE));
+        const uint64_t da = code_desc(src), db = code_desc(src + ROW_CODES);
+        const uint32_t steps = min(STEPS, p.ksteps - kb * STEPS);
+        for (uint32_t k = 0; k < steps; ++k)
+          ptx::mma_mxf4<false>(tmem, da + k * 2, db + k * 2, (k & 1) ? idesc1 : idesc0, ts + (k >> 1) * 4,
+                               ts + 8 + (k >> 1) * 4, (kb > kb0 || k) ? 1u : 0u);
+        ptx::mma_commit(empty_bar(stage));
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (ok) ptx::mma_commit(done_bar);
+    }
+    __syncwarp();
+  } else {
+    const uint32_t quarter = warp & 3u;
+    bool ok = ptx::mbar_wait(done_bar, 0, abort_flag);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok && lane == 0 && first_to_give_up(abort_flag)) report(p.status, 3, 0, tile, 0);
+    ptx::tc_fence_after();
+    const uint32_t r = quarter * 32u + lane;       // row of the tile
+    const uint64_t n = uint64_t(tn) * ROWS + r;
+    const uint32_t m0 = tm * BN, cols = min(uint32_t(BN), p.M - m0);
+    const uint32_t taddr = tmem + ((quarter * 32u) << 16);
+    const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+    if (p.splits == 1) {
+#pragma unroll 1
+      for (uint32_t c0 = 0; ok && c0 < cols; c0 += 32) {
+        uint32_t v[32];
+        ptx::tmem_ld_32x32(taddr + c0, v);
+        ptx::tmem_ld_wait();
+        float* out = p.c + (uint64_t(m0) + c0) * p.N + n;
+#pragma unroll
+        for (uint32_t j = 0; j < 32; ++j)
+          if (c0 + j < cols && n < p.N) out[uint64_t(j) * p.N] = apply_act(__uint_as_float(v[j]) + bias, p.act, p.act_param);
+      }
+    } else {
+      // the unit that counts itself in last adds the partial sums in the order of the splits:
+      // the result does not depend on who that is.  (A warp that gave up still takes part in the
+      // barriers; its unit does not count, and the error clears the counters.)
+      float* part = p.ws + uint64_t(blockIdx.x) * BN * ROWS + r;
+#pragma unroll 1
+      for (uint32_t c0 = 0; ok && c0 < cols; c0 += 32) {
+        uint32_t v[32];
+        ptx::tmem_ld_32x32(taddr + c0, v);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (uint32_t j = 0; j < 32; ++j)
+          if (c0 + j < cols) __stcg(part + (c0 + j) * ROWS, __uint_as_float(v[j]));
+      }
+      __threadfence();
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (threadIdx.x == 64) {
+        const bool last = *abort_flag == 0 && atomicAdd(&p.counters[tile], 1u) + 1 == p.splits;
+        *last_flag = last;
+        if (last) p.counters[tile] = 0;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (*last_flag) {
+        __threadfence();
+        const float* all = p.ws + uint64_t(tile) * p.splits * BN * ROWS + r;
+        for (uint32_t c = 0; c < cols; ++c) {
+          float sum = 0.f;
+          for (uint32_t s = 0; s < p.splits; ++s) sum += __ldcg(all + (uint64_t(s) * BN + c) * ROWS);
+          if (n < p.N) p.c[(uint64_t(m0) + c) * p.N + n] = apply_act(sum + bias, p.act, p.act_param);
+        }
+      }
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  wait_out(abort_flag);
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, S::TMEM);
+  }
+}
+
+// ---- CTA pairs: 256 outputs x 256 batch rows, persistent ---------------------------------
+// Two CTAs share one MMA (M = 256): CTA r holds the codes of rows r*128.. of the tile's B and of
+// r*128.. of its A, the scales of its own rows of B and those of all 256 rows of A.  The single
+// 256-column accumulator leaves room in TMEM for every stage's scales; the eight warps that read
+// it out take it into registers at once and hand TMEM back before they store, so the next tile's
+// MMAs wait only for the read, while its loads have been running all the time.
+constexpr uint32_t PAIR_THREADS = 320;
+constexpr uint32_t PAIR_COLS = 256;
+constexpr uint32_t PAIR_STAGE = 2 * ROW_CODES + 6 * SCALE_TILE;
+constexpr uint32_t PAIR_STAGES = 6;
+constexpr uint32_t PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + 1024 + 256;
+static_assert(PAIR_SMEM <= SMEM_LIMIT && PAIR_COLS + PAIR_STAGES * 24 <= 512, "pair kernel resources");
+
+__device__ __forceinline__ void pair_tile(const Params& p, uint32_t t, uint32_t& tn, uint32_t& tm) {
+  // groups of 8 tiles of B sweep A together
+  const uint32_t per = 8 * p.tiles_m, g = t / per, first = g * 8;
+  const uint32_t wide = min(8u, p.tiles_n - first), r = t - g * per;
+  tn = first + r % wide;
+  tm = r / wide;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_constant__ CUtensorMap tm_row_scales,
+                  const __grid_constant__ CUtensorMap tm_cols, const __grid_constant__ CUtensorMap tm_col_scales,
+                  const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
+  const uint32_t base = raw + pad;
+  const uint32_t bar_base = base + PAIR_STAGES * PAIR_STAGE;
+  auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (PAIR_STAGES + s); };
+  const uint32_t tfull_bar = bar_base + 8u * (2 * PAIR_STAGES), tempty_bar = tfull_bar + 8u;
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem_raw + pad + PAIR_STAGES * PAIR_STAGE + 8 * (2 * PAIR_STAGES + 2));
+  uint32_t* tmem_slot = words;
+  volatile uint32_t* abort_flag = words + 1;
+
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();
+  const bool leader = rank == 0;
+  const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < PAIR_STAGES; ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    ptx::mbar_init(tfull_bar, 1);
+    ptx::mbar_init(tempty_bar, 16);  // the eight reading warps of both CTAs
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+  }
+  if (warp == 0 && lane == 0) {
+    ptx::prefetch_tmap(&tm_rows);
+    ptx::prefetch_tmap(&tm_row_scales);
+    ptx::prefetch_tmap(&tm_cols);
+    ptx::prefetch_tmap(&tm_col_scales);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::cluster_sync_all();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  ptx::grid_dependency_release();
+  ptx::grid_dependency_wait();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      bool alive = true;
+      for (uint32_t t = pair; alive && t < p.num_tiles; t += pairs) {
+        uint32_t tn, tm;
+        pair_tile(p, t, tn, tm);
+        for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
+          if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
+            if (first_to_give_up(abort_flag)) report(p.status, 1, stage, t, kb);
+            alive = false;
+            break;
+          }
+          if (leader) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * PAIR_STAGE);
+          const uint32_t fb = ptx::mapa_shared(full_bar(stage), 0), dst = base + stage * PAIR_STAGE;
+          ptx::tma_load_2d_pair(dst, &tm_rows, int32_t(kb * STAGE_K_BYTES), int32_t((tn * 2 + rank) * ROWS), fb);
+          ptx::tma_load_2d_pair(dst + ROW_CODES, &tm_cols, int32_t(kb * STAGE_K_BYTES),
+                                int32_t((tm * 2 + rank) * ROWS), fb);
+          const uint32_t scales = dst + 2 * ROW_CODES;
+          ptx::tma_load_3d_pair(scales, &tm_row_scales, 0, int32_t(kb * 2), int32_t(tn * 2 + rank), fb);
+          ptx::tma_load_3d_pair(scales + 2 * SCALE_TILE, &tm_col_scales, 0, int32_t(kb * 2), int32_t(tm * 2), fb);
+          if (++stage == PAIR_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (leader && lane == 0) {
+      constexpr uint32_t idesc0 = ptx::make_idesc_mxf4(256, PAIR_COLS, 0), idesc1 = ptx::make_idesc_mxf4(256, PAIR_COLS, 1);
+      uint32_t stage = 0, phase = 0, local = 0;
+      bool alive = true;
+      for (uint32_t t = pair; alive && t < p.num_tiles; t += pairs, ++local) {
+        if (!ptx::mbar_wait(tempty_bar, (local & 1u) ^ 1u, abort_flag)) {
+          if (first_to_give_up(abort_flag)) report(p.status, 2, 0x100u, t, 0);
+          break;
+        }
+        ptx::tc_fence_after();
+        for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
+          if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag)) {
+            if (first_to_give_up(abort_flag)) report(p.status, 2, stage, t, kb);
+            alive = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          const uint32_t src = base + stage * PAIR_STAGE, scales = src + 2 * ROW_CODES;
+          // per stage: 2 x 4 columns for the rows' scales, 2 x 8 for the columns' (128 + 128 rows)
+          const uint32_t ts = tmem + PAIR_COLS + stage * 24;
+#pragma unroll
+          for (uint32_t k = 0; k < 2; ++k) {
+            ptx::tmem_cp_scales<true>(ts + k * 4, scale_desc(scales + k * SCALE_TILE));
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+              ptx::tmem_cp_scales<true>(ts + 8 + k * 8 + h * 4, scale_desc(scales + (2 + h * 2 + k) * SCALE_TILE));
+          }
+          const uint64_t da = code_desc(src), db = code_desc(src + ROW_CODES);
+          const uint32_t steps = min(STEPS, p.ksteps - kb * STEPS);
+          for (uint32_t k = 0; k < steps; ++k)
+            ptx::mma_mxf4<true>(tmem, da + k * 2, db + k * 2, (k & 1) ? idesc1 : idesc0, ts + (k >> 1) * 4,
+                                ts + 8 + (k >> 1) * 8, (kb | k) ? 1u : 0u);
+          ptx::mma_commit_pair(empty_bar(stage), 3);
+          if (++stage == PAIR_STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (alive) ptx::mma_commit_pair(tfull_bar, 3);
+      }
+    }
+    __syncwarp();
+  } else {
+    const uint32_t quarter = warp & 3u, half = (warp - 2u) >> 2;
+    uint32_t local = 0;
+    for (uint32_t t = pair; t < p.num_tiles; t += pairs, ++local) {
+      uint32_t tn, tm;
+      pair_tile(p, t, tn, tm);
+      bool ok = ptx::mbar_wait(tfull_bar, local & 1u, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) {
+        if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 3, 0, t, 0);
+        break;
+      }
+      ptx::tc_fence_after();
+      uint32_t v[4][32];
+      const uint32_t taddr = tmem + ((quarter * 32u) << 16) + half * 128u;
+#pragma unroll
+      for (uint32_t c = 0; c < 4; ++c) ptx::tmem_ld_32x32(taddr + c * 32u, v[c]);
+      ptx::tmem_ld_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(tempty_bar, 0));
+      const uint64_t n = uint64_t(tn * 2 + rank) * ROWS + quarter * 32u + lane;
+      const uint32_t m0 = tm * PAIR_COLS + half * 128u;
+      const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+      if (n < p.N) {
+        float* out = p.c + uint64_t(m0) * p.N + n;
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c)
+#pragma unroll
+          for (uint32_t j = 0; j < 32; ++j)
+            if (m0 + c * 32 + j < p.M)
+              out[uint64_t(c * 32 + j) * p.N] = apply_act(__uint_as_float(v[c][j]) + bias, p.act, p.act_param);
+      }
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  wait_out(abort_flag);
+  __syncthreads();
+  ptx::cluster_sync_all();  // neither CTA leaves while the other can still signal or read it
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// ---- host side -----------------------------------------------------------------------
+// Codes as a byte matrix: boxes of 128 bytes x `box_rows` rows.
+bool code_map(CUtensorMap* map, const void* packed, const Mxfp4Layout& l, uint32_t box_rows) {
+  const uint64_t dims[2] = {l.row_bytes, l.rows}, strides[1] = {l.row_bytes};
+  const uint32_t box[2] = {STAGE_K_BYTES, box_rows};
+  return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, packed, dims, strides, box,
+                           CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// Scale tiles of 512 bytes: boxes of 2 along K x `tall` along the rows.
+bool scale_map(CUtensorMap* map, const void* packed, const Mxfp4Layout& l, uint32_t tall) {
+  const uint64_t dims[3] = {SCALE_TILE / 4, l.groups, (l.rows + 127) / 128};
+  const uint64_t strides[2] = {SCALE_TILE, l.groups * SCALE_TILE};
+  const uint32_t box[3] = {SCALE_TILE / 4, 2, tall};
+  return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3,
+                           static_cast<const uint8_t*>(packed) + l.scale_offset, dims, strides, box,
+                           CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <auto KERN>
+bool allow_smem(uint32_t bytes) {
+  static bool done[64] = {};  // per kernel and device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!done[dev & 63]) done[dev & 63] = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes)) == cudaSuccess;
+  return done[dev & 63];
+}
+
+template <int BN, int STAGES>
+const char* launch_single(const Mxfp4Product& q, const Mxfp4Layout& la, const Mxfp4Layout& lb, Params p,
+                          uint32_t units, cudaStream_t stream) {
+  CUtensorMap rows, row_scales, cols, col_scales;
+  if (!code_map(&rows, q.b, lb, ROWS) || !scale_map(&row_scales, q.b, lb, 1) || !code_map(&cols, q.a, la, BN) ||
+      !scale_map(&col_scales, q.a, la, 1))
+    return "cuTensorMapEncodeTiled failed";
+  constexpr auto kern = mxfp4_single_kernel<BN, STAGES>;
+  constexpr uint32_t smem = SingleShape<BN, STAGES>::SMEM;
+  static_assert(smem <= SMEM_LIMIT, "shared memory");
+  if (!allow_smem<kern>(smem)) return "cudaFuncSetAttribute(max dynamic shared memory) failed";
+  if (launch_kernel(kern, dim3(units), dim3(SINGLE_THREADS), smem, stream, rows, row_scales, cols, col_scales, p) !=
+      cudaSuccess)
+    return "product launch failed";
+  return nullptr;
+}
+
+}  // namespace
+
+const char* launch_mxfp4_product(const Mxfp4Product& q, GemmStatus* status, int sm_count, float* ws, size_t ws_bytes,
+                                 uint32_t* counters, uint32_t counter_slots, cudaStream_t stream) {
+  const Mxfp4Layout la(q.M, q.K), lb(q.N, q.K);
+  Params p{};
+  p.M = uint32_t(q.M);
+  p.N = uint32_t(q.N);
+  p.kblocks = uint32_t((lb.row_bytes + STAGE_K_BYTES - 1) / STAGE_K_BYTES);
+  p.ksteps = uint32_t((lb.blocks + 1) / 2);
+  p.splits = 1;
+  p.kb_per_split = p.kblocks;
+  p.c = q.c;
+  p.bias = q.bias;
+  p.act = q.act;
+  p.act_param = q.act_param;
+  p.status = status;
+  const uint64_t pair_tiles = ((q.N + 255) / 256) * ((q.M + 255) / 256);
+  if (pair_tiles >= 64) {
+    if (pair_tiles >= (1ull << 31)) return "too many tiles";
+    p.tiles_n = uint32_t((q.N + 255) / 256);
+    p.tiles_m = uint32_t((q.M + 255) / 256);
+    p.num_tiles = uint32_t(pair_tiles);
+    CUtensorMap rows, row_scales, cols, col_scales;
+    if (!code_map(&rows, q.b, lb, ROWS) || !scale_map(&row_scales, q.b, lb, 1) || !code_map(&cols, q.a, la, ROWS) ||
+        !scale_map(&col_scales, q.a, la, 2))
+      return "cuTensorMapEncodeTiled failed";
+    if (!allow_smem<mxfp4_pair_kernel>(PAIR_SMEM)) return "cudaFuncSetAttribute(max dynamic shared memory) failed";
+    const uint32_t pairs = std::min(uint32_t(sm_count) / 2, p.num_tiles);
+    if (launch_kernel(mxfp4_pair_kernel, dim3(2 * pairs), dim3(PAIR_THREADS), PAIR_SMEM, stream, rows, row_scales, cols,
+                      col_scales, p) != cudaSuccess)
+      return "product launch failed";
+    return nullptr;
+  }
+  const uint32_t bn = q.M <= 32 ? 32 : q.M <= 64 ? 64 : 128;
+  p.tiles_n = uint32_t((q.N + ROWS - 1) / ROWS);
+  p.tiles_m = uint32_t((q.M + bn - 1) / bn);
+  p.num_tiles = p.tiles_n * p.tiles_m;
+  // few tiles: share each one's K among several CTAs
+  uint32_t splits = std::max(1u, uint32_t(sm_count) / p.num_tiles);
+  splits = std::min(splits, p.kblocks);
+  if (p.num_tiles > counter_slots || uint64_t(p.num_tiles) * splits * bn * ROWS * 4 > ws_bytes) splits = 1;
+  p.kb_per_split = (p.kblocks + splits - 1) / splits;
+  p.splits = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;
+  p.ws = ws;
+  p.counters = counters;
+  const uint32_t units = p.num_tiles * p.splits;
+  return bn == 32   ? launch_single<32, 6>(q, la, lb, p, units, stream)
+         : bn == 64 ? launch_single<64, 4>(q, la, lb, p, units, stream)
+                    : launch_single<128, 4>(q, la, lb, p, units, stream);
+}
+
+}  // namespace gonn

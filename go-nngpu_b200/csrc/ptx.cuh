@@ -304,6 +304,37 @@ __device__ __forceinline__ void mma_commit_pair(uint32_t bar, uint16_t cta_mask)
       ::"r"(bar), "h"(cta_mask) : "memory");
 }
 
+// ------------------------------------------------- block-scaled 4-bit operands
+// 32 rows of 16 bytes from shared memory (descriptor) to 4 TMEM columns, the same in each of the
+// four 32-lane quarters: one tile of scales.  Ordered before the same thread's later MMAs.  With
+// `PAIR`, in both CTAs of the pair, each from its own shared memory.
+template <bool PAIR>
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// D[tmem] (+)= (A * scales) . (B * scales)^T on e2m1 operands, K = 64 a step, a scale for 32.
+template <bool PAIR>
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t sa_tmem, uint32_t sb_tmem, uint32_t accumulate) {
+  if (PAIR)
+    asm volatile(
+        "{\n\t"
+        ".reg .pred P;\n\t"
+        "setp.ne.b32 P, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], P;\n\t"
+        "}\n"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate) : "memory");
+  else
+    asm volatile(
+        "{\n\t"
+        ".reg .pred P;\n\t"
+        "setp.ne.b32 P, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], P;\n\t"
+        "}\n"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate) : "memory");
+}
+
 // ------------------------------------------------- system-scope flags, multicast stores
 // Flags that another GPU writes or reads (arrival of replicated data, acknowledgements).
 __device__ __forceinline__ uint32_t ld_acquire_sys(const uint32_t* p) {
@@ -370,6 +401,13 @@ __host__ __device__ constexpr uint64_t smem_desc(uint32_t layout, uint32_t lbo_b
                                                  uint32_t sbo_bytes) {
   return (uint64_t((lbo_bytes >> 4) & 0x3FFF) << 16) | (uint64_t((sbo_bytes >> 4) & 0x3FFF) << 32) |
          (uint64_t(1) << 46) | (uint64_t(layout) << 61);
+}
+// Instruction descriptor for kind::mxf4: [4,6) which byte pair of a scale word B takes, [7,10) and
+// [10,12) formats (1 = e2m1), [17,23) N >> 3, bit 23 scales are 2^e (ue8m0), [27,29) M >> 7,
+// [29,31) which byte pair A takes.  Both operands are K-major.
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(uint32_t m, uint32_t n, uint32_t pair_of_bytes) {
+  return ((pair_of_bytes * 2) << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | (1u << 23) | ((m >> 7) << 27) |
+         ((pair_of_bytes * 2) << 29);
 }
 // Instruction descriptor for kind::f16 / kind::tf32 with fp32 accumulation:
 //   [4,6) D format (1 = f32), [7,10) A format, [10,13) B format (0 f16, 1 bf16,

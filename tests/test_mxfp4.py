@@ -194,7 +194,8 @@ def activate(y, act, param):
 PRODUCTS = [(1, 1, 1), (1, 10, 784), (1, 1000, 4096), (2, 129, 100), (3, 64, 33), (4, 300, 2000), (5, 17, 31), (8, 512, 1024),
             (9, 130, 64), (16, 256, 300), (17, 100, 1000), (33, 65, 129), (64, 256, 256), (100, 1000, 784),
             (128, 128, 128), (129, 257, 513), (200, 300, 5000), (256, 256, 2048), (300, 515, 777), (512, 10, 1024),
-            (520, 1030, 260), (1000, 2000, 3000)]
+            (520, 1030, 260), (1000, 2000, 3000), (2048, 2048, 320), (2050, 2100, 1000), (257, 20000, 100),
+            (20001, 130, 600)]
 
 
 @pytest.mark.gpu
