@@ -2246,8 +2246,7 @@ int mxfp4_product(const char* what, GPUPtr aPtr, bool a_float, long m, GPUPtr bP
     ++g_stats[3];
     p.a = scratch;
   }
-  const char* msg = gonn::launch_mxfp4_product(p, d.status_dev, d.sm_count, d.splitk_ws, kSplitKBytes,
-                                               d.splitk_counters, kSplitKSlots, d.stream);
+  const char* msg = gonn::launch_mxfp4_product(p, d.status_dev, d.sm_count, d.stream);
   // whoever gets the scratch next is queued behind this product on the same stream
   if (scratch) pool_free(c->device, scratch, la.bytes);
   if (msg) {

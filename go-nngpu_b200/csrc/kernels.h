@@ -217,10 +217,8 @@ struct Mxfp4Product {
   int act = ACT_NONE;
   float act_param = 0.f;
 };
-// C = act(A . B^T + bias).  Returns nullptr on success, else a static message.  `ws` / `counters`
-// as in GemmTuning: partial sums of products with few tiles.
-const char* launch_mxfp4_product(const Mxfp4Product& p, GemmStatus* status, int sm_count, float* ws, size_t ws_bytes,
-                                 uint32_t* counters, uint32_t counter_slots, cudaStream_t stream);
+// C = act(A . B^T + bias).  Returns nullptr on success, else a static message.
+const char* launch_mxfp4_product(const Mxfp4Product& p, GemmStatus* status, int sm_count, cudaStream_t stream);
 
 // ---- replication of B over NVSwitch (row-sharded product) --------------------------
 // Control words every rank keeps at the same offset of its symmetric buffer.  arrived[s] is

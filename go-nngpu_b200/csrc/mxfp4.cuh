@@ -40,13 +40,11 @@ __device__ __forceinline__ uint32_t encode2(float lo, float hi) {
       : "f"(hi), "f"(lo));
   return r;
 }
-// The value of one code: 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives.  The two exponent bits
-// and the mantissa bit are those of a float with the exponent bias 126 - code 1 (0.5) alone is
-// subnormal in the code and not in the float.
+// The value of the code in the low four bits: 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives.  Moved
+// to the top of a float's exponent and mantissa the three bits read as that value times 2^-126
+// (code 1, like the code itself, as a subnormal number).
 __device__ __forceinline__ float decode(uint32_t code) {
-  const uint32_t mag = code & 7u;
-  const float v = mag < 2u ? 0.5f * float(mag) : __uint_as_float((mag << 22) + (126u << 23));
-  return (code & 8u) ? -v : v;
+  return __uint_as_float(((code & 7u) << 22) | ((code & 8u) << 28)) * 0x1p126f;
 }
 
 }  // namespace mxfp4

@@ -32,20 +32,44 @@ constexpr uint32_t STEPS = 4;                  // MMAs (64 of K) a stage
 constexpr uint32_t ROW_CODES = ROWS * STAGE_K_BYTES;
 constexpr uint32_t SCALE_TILE = 512;           // scales of 128 rows x 128 of K
 constexpr uint32_t SMEM_LIMIT = 227 * 1024;
+// The tensor core adds into its accumulators with truncation, so the error grows with the number
+// of MMAs: on blocks whose scales differ by 2^4 (one standard deviation) 1.8e-7 relative at K =
+// 4096, 6.0e-7 at 8192, 3.8e-6 at 16384, against 1.6e-7, 4.5e-7 and 1.2e-6 of float32 sums.  After
+// this many stages (4096 of K) the accumulators are therefore added to sums in registers, with
+// rounding to nearest, and start again.
+constexpr uint32_t CHUNK = 16;
 
 struct Params {
   uint32_t M, N;          // rows of A (columns of the tile), rows of B (rows of the tile)
   uint32_t tiles_n, tiles_m, num_tiles;
   uint32_t kblocks, ksteps;          // stages and MMAs along K
-  uint32_t splits, kb_per_split;     // single-CTA kernel: work units of a tile along K
+  uint32_t splits, kb_per_split;     // single-CTA kernel: CTAs (of one cluster) that share a tile's K
   float* c;
   const float* bias;
   int act;
   float act_param;
-  float* ws;              // partial sums of split tiles: [unit][column][128]
-  uint32_t* counters;     // one per tile, zero between launches
   GemmStatus* status;
 };
+
+// The epilogues are unrolled over their registers.  With the choice of activation inside every
+// copy the code outgrew the instruction cache: the 4096^3 product took 89 us, 59 us without its
+// stores.  So the two common cases are compiled apart and the rest is one out-of-line call.
+enum ActClass : int { IDENTITY = 0, RELU = 1, OTHER = 2 };
+__device__ __noinline__ float other_activation(float v, int act, float param) { return apply_act(v, act, param); }
+template <int CLASS>
+__device__ __forceinline__ float finish(const Params& p, float sum, float bias) {
+  const float v = sum + bias;
+  return CLASS == IDENTITY ? v : CLASS == RELU ? fmaxf(v, 0.f) : other_activation(v, p.act, p.act_param);
+}
+
+// Adds 32 accumulator columns to (or, the first time, puts them into) a thread's sums.
+__device__ __forceinline__ void take_columns(uint32_t taddr, float (&sum)[32], bool first) {
+  uint32_t v[32];
+  ptx::tmem_ld_32x32(taddr, v);
+  ptx::tmem_ld_wait();
+#pragma unroll
+  for (uint32_t j = 0; j < 32; ++j) sum[j] = first ? __uint_as_float(v[j]) : sum[j] + __uint_as_float(v[j]);
+}
 
 // Scales: no swizzle, groups of 8 rows of 16 bytes 128 bytes apart.
 __device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
@@ -66,8 +90,11 @@ __device__ __forceinline__ void wait_out(volatile uint32_t* abort_flag) {
   }
 }
 
-// ---- one CTA per tile of 128 outputs x BN batch rows, or per share of its K -------------
-// Warp 0 loads, warp 1 issues the MMAs, warps 2-5 read the accumulators out.
+// ---- one CTA per tile of 128 outputs x BN batch rows, or a cluster that shares its K ------
+// Warp 0 loads, warp 1 issues the MMAs, warps 2-5 read the accumulators out.  A product with few
+// tiles gives each tile to a cluster of up to 8 CTAs: each multiplies its share of K, leaves its
+// sums in its shared memory, and then adds up every `splits`-th column over all of them, in the
+// order of the shares.
 constexpr uint32_t SINGLE_THREADS = 192;
 
 template <int BN, int STAGES>
@@ -77,9 +104,10 @@ struct SingleShape {
   static constexpr uint32_t SMEM = STAGES * STAGE + 1024 + 256;
   static constexpr uint32_t USED = BN + STAGES * 16;
   static constexpr uint32_t TMEM = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+  static_assert(STAGES * STAGE >= BN * ROWS * 4, "the stages hold the sums of a share");
 };
 
-template <int BN, int STAGES>
+template <int BN, int STAGES, int CLASS>
 __global__ void __launch_bounds__(SINGLE_THREADS)
 mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_constant__ CUtensorMap tm_row_scales,
                     const __grid_constant__ CUtensorMap tm_cols, const __grid_constant__ CUtensorMap tm_col_scales,
@@ -92,11 +120,10 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
   const uint32_t bar_base = base + STAGES * S::STAGE;
   auto full_bar = [&](uint32_t s) { return bar_base + 8u * s; };
   auto empty_bar = [&](uint32_t s) { return bar_base + 8u * (STAGES + s); };
-  const uint32_t done_bar = bar_base + 8u * (2 * STAGES);
-  uint32_t* words = reinterpret_cast<uint32_t*>(smem_raw + pad + STAGES * S::STAGE + 8 * (2 * STAGES + 1));
+  const uint32_t tfull_bar = bar_base + 8u * (2 * STAGES), tempty_bar = tfull_bar + 8u;
+  uint32_t* words = reinterpret_cast<uint32_t*>(smem_raw + pad + STAGES * S::STAGE + 8 * (2 * STAGES + 2));
   uint32_t* tmem_slot = words;
   volatile uint32_t* abort_flag = words + 1;
-  volatile uint32_t* last_flag = words + 2;
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tile = blockIdx.x / p.splits, split = blockIdx.x - tile * p.splits;
@@ -108,7 +135,8 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
       ptx::mbar_init(full_bar(s), 1);
       ptx::mbar_init(empty_bar(s), 1);
     }
-    ptx::mbar_init(done_bar, 1);
+    ptx::mbar_init(tfull_bar, 1);
+    ptx::mbar_init(tempty_bar, 4);  // the reading warps
     *abort_flag = 0;
     ptx::fence_mbar_init();
     ptx::fence_proxy_async_smem();
@@ -155,89 +183,96 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc0 = ptx::make_idesc_mxf4(ROWS, BN, 0), idesc1 = ptx::make_idesc_mxf4(ROWS, BN, 1);
-      uint32_t stage = 0, phase = 0;
+    // The whole warp runs the loop and one lane issues: what the instructions take stays in
+    // uniform registers.
+    constexpr uint32_t idesc0 = ptx::make_idesc_mxf4(ROWS, BN, 0), idesc1 = ptx::make_idesc_mxf4(ROWS, BN, 1);
+    uint32_t stage = 0, phase = 0;
+    for (uint32_t kb = kb0; kb < kb1; ++kb) {
+      const uint32_t in_chunk = (kb - kb0) % CHUNK;
       bool ok = true;
-      for (uint32_t kb = kb0; kb < kb1; ++kb) {
-        if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag)) {
-          if (first_to_give_up(abort_flag)) report(p.status, 2, stage, tile, kb);
-          ok = false;
-          break;
-        }
-        ptx::tc_fence_after();
-        const uint32_t src = base + stage * S::STAGE, scales = src + ROW_CODES + S::COL_CODES;
-        const uint32_t ts = tmem + BN + stage * 16;
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) ptx::tmem_cp_scales<false>(ts + j * 4, scale_desc(scales + j * SCALE_TILE));
-        const uint64_t da = code_desc(src), db = code_desc(src + ROW_CODES);
-        const uint32_t steps = min(STEPS, p.ksteps - kb * STEPS);
-        for (uint32_t k = 0; k < steps; ++k)
-          ptx::mma_mxf4<false>(tmem, da + k * 2, db + k * 2, (k & 1) ? idesc1 : idesc0, ts + (k >> 1) * 4,
-                               ts + 8 + (k >> 1) * 4, (kb > kb0 || k) ? 1u : 0u);
-        ptx::mma_commit(empty_bar(stage));
-        if (++stage == STAGES) {
-          stage = 0;
-          phase ^= 1u;
-        }
+      if (in_chunk == 0) ok = ptx::mbar_wait(tempty_bar, ((kb - kb0) / CHUNK & 1u) ^ 1u, abort_flag);
+      ok = ok && ptx::mbar_wait(full_bar(stage), phase, abort_flag);
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 2, stage, tile, kb);
+        break;
       }
-      if (ok) ptx::mma_commit(done_bar);
+      ptx::tc_fence_after();
+      const uint32_t src = base + stage * S::STAGE, scales = src + ROW_CODES + S::COL_CODES;
+      const uint32_t ts = tmem + BN + stage * 16;
+      const uint64_t da = code_desc(src), db = code_desc(src + ROW_CODES), ds = scale_desc(scales);
+      const uint32_t steps = min(STEPS, p.ksteps - kb * STEPS);
+      if (ptx::elect_one()) {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) ptx::tmem_cp_scales<false>(ts + j * 4, ds + j * (SCALE_TILE >> 4));
+#pragma unroll
+        for (uint32_t k = 0; k < STEPS; ++k)
+          if (k < steps)
+            ptx::mma_mxf4<false>(tmem, da + k * 2, db + k * 2, (k & 1) ? idesc1 : idesc0, ts + (k >> 1) * 4,
+                                 ts + 8 + (k >> 1) * 4, (in_chunk || k) ? 1u : 0u);
+        ptx::mma_commit(empty_bar(stage));
+        if (in_chunk + 1 == CHUNK || kb + 1 == kb1) ptx::mma_commit(tfull_bar);
+      }
+      __syncwarp();
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1u;
+      }
     }
-    __syncwarp();
   } else {
     const uint32_t quarter = warp & 3u;
-    bool ok = ptx::mbar_wait(done_bar, 0, abort_flag);
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok && lane == 0 && first_to_give_up(abort_flag)) report(p.status, 3, 0, tile, 0);
-    ptx::tc_fence_after();
     const uint32_t r = quarter * 32u + lane;       // row of the tile
     const uint64_t n = uint64_t(tn) * ROWS + r;
     const uint32_t m0 = tm * BN, cols = min(uint32_t(BN), p.M - m0);
     const uint32_t taddr = tmem + ((quarter * 32u) << 16);
-    const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
-    if (p.splits == 1) {
-#pragma unroll 1
-      for (uint32_t c0 = 0; ok && c0 < cols; c0 += 32) {
-        uint32_t v[32];
-        ptx::tmem_ld_32x32(taddr + c0, v);
-        ptx::tmem_ld_wait();
-        float* out = p.c + (uint64_t(m0) + c0) * p.N + n;
+    const uint32_t chunks = (kb1 - kb0 + CHUNK - 1) / CHUNK;
+    float sum[BN / 32][32];
+    bool ok = true;
+    for (uint32_t ch = 0; ch < chunks; ++ch) {
+      ok = __all_sync(0xffffffffu, ptx::mbar_wait(tfull_bar, ch & 1u, abort_flag));
+      if (!ok) {
+        if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 3, 0, tile, ch);
+        break;
+      }
+      ptx::tc_fence_after();
 #pragma unroll
-        for (uint32_t j = 0; j < 32; ++j)
-          if (c0 + j < cols && n < p.N) out[uint64_t(j) * p.N] = apply_act(__uint_as_float(v[j]) + bias, p.act, p.act_param);
-      }
-    } else {
-      // the unit that counts itself in last adds the partial sums in the order of the splits:
-      // the result does not depend on who that is.  (A warp that gave up still takes part in the
-      // barriers; its unit does not count, and the error clears the counters.)
-      float* part = p.ws + uint64_t(blockIdx.x) * BN * ROWS + r;
-#pragma unroll 1
-      for (uint32_t c0 = 0; ok && c0 < cols; c0 += 32) {
-        uint32_t v[32];
-        ptx::tmem_ld_32x32(taddr + c0, v);
-        ptx::tmem_ld_wait();
+      for (uint32_t c = 0; c < BN / 32; ++c)
+        if (c * 32 < cols) take_columns(taddr + c * 32, sum[c], ch == 0);
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(tempty_bar);
+    }
+    if (ok && p.splits == 1 && n < p.N) {
+      const float bias = p.bias ? p.bias[n] : 0.f;
+      float* out = p.c + uint64_t(m0) * p.N + n;
 #pragma unroll
-        for (uint32_t j = 0; j < 32; ++j)
-          if (c0 + j < cols) __stcg(part + (c0 + j) * ROWS, __uint_as_float(v[j]));
-      }
-      __threadfence();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (threadIdx.x == 64) {
-        const bool last = *abort_flag == 0 && atomicAdd(&p.counters[tile], 1u) + 1 == p.splits;
-        *last_flag = last;
-        if (last) p.counters[tile] = 0;
-      }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (*last_flag) {
-        __threadfence();
-        const float* all = p.ws + uint64_t(tile) * p.splits * BN * ROWS + r;
-        for (uint32_t c = 0; c < cols; ++c) {
-          float sum = 0.f;
-          for (uint32_t s = 0; s < p.splits; ++s) sum += __ldcg(all + (uint64_t(s) * BN + c) * ROWS);
-          if (n < p.N) p.c[(uint64_t(m0) + c) * p.N + n] = apply_act(sum + bias, p.act, p.act_param);
-        }
+      for (uint32_t c = 0; c < BN; ++c, out += p.N)
+        if (c < cols) *out = finish<CLASS>(p, sum[c / 32][c % 32], bias);
+    } else if (ok && p.splits > 1) {
+      // every MMA of this CTA has retired and with it every read of the stages
+      float* part = reinterpret_cast<float*>(smem_raw + pad) + r;
+#pragma unroll
+      for (uint32_t c = 0; c < BN; ++c)
+        if (c < cols) part[c * ROWS] = sum[c / 32][c % 32];
+    }
+  }
+
+  if (p.splits > 1) {
+    __syncthreads();
+    ptx::cluster_sync_all();  // the sums of every share are in place
+    if (warp >= 2) {
+      const uint32_t r = (warp & 3u) * 32u + lane;
+      const uint64_t n = uint64_t(tn) * ROWS + r;
+      const uint32_t m0 = tm * BN, cols = min(uint32_t(BN), p.M - m0);
+      const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+#pragma unroll 1
+      for (uint32_t c = split; c < cols; c += p.splits) {
+        const uint32_t at = base + (c * ROWS + r) * 4;
+        float sum = 0.f;
+        for (uint32_t s = 0; s < p.splits; ++s) sum += ptx::ld_shared_cluster(ptx::mapa_shared(at, s));
+        if (n < p.N) p.c[(uint64_t(m0) + c) * p.N + n] = finish<CLASS>(p, sum, bias);
       }
     }
+    ptx::cluster_sync_all();  // no CTA leaves while another still reads its sums
   }
 
   ptx::tc_fence_before();
@@ -271,6 +306,7 @@ __device__ __forceinline__ void pair_tile(const Params& p, uint32_t t, uint32_t&
   tm = r / wide;
 }
 
+template <int CLASS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_constant__ CUtensorMap tm_row_scales,
                   const __grid_constant__ CUtensorMap tm_cols, const __grid_constant__ CUtensorMap tm_col_scales,
@@ -351,80 +387,95 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_cons
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (leader && lane == 0) {
+    // The whole warp runs the loop and one lane issues: what the instructions take stays in
+    // uniform registers.
+    if (leader) {
       constexpr uint32_t idesc0 = ptx::make_idesc_mxf4(256, PAIR_COLS, 0), idesc1 = ptx::make_idesc_mxf4(256, PAIR_COLS, 1);
-      uint32_t stage = 0, phase = 0, local = 0;
+      uint32_t stage = 0, phase = 0, drained = 1;
       bool alive = true;
-      for (uint32_t t = pair; alive && t < p.num_tiles; t += pairs, ++local) {
-        if (!ptx::mbar_wait(tempty_bar, (local & 1u) ^ 1u, abort_flag)) {
-          if (first_to_give_up(abort_flag)) report(p.status, 2, 0x100u, t, 0);
-          break;
-        }
-        ptx::tc_fence_after();
+      for (uint32_t t = pair; alive && t < p.num_tiles; t += pairs) {
+        uint32_t in_chunk = 0;
         for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
-          if (!ptx::mbar_wait(full_bar(stage), phase, abort_flag)) {
-            if (first_to_give_up(abort_flag)) report(p.status, 2, stage, t, kb);
+          bool ok = true;
+          if (in_chunk == 0) {
+            ok = ptx::mbar_wait(tempty_bar, drained, abort_flag);
+            drained ^= 1u;
+          }
+          ok = ok && ptx::mbar_wait(full_bar(stage), phase, abort_flag);
+          if (!__all_sync(0xffffffffu, ok)) {
+            if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 2, stage, t, kb);
             alive = false;
             break;
           }
           ptx::tc_fence_after();
-          const uint32_t src = base + stage * PAIR_STAGE, scales = src + 2 * ROW_CODES;
+          const uint32_t src = base + stage * PAIR_STAGE;
           // per stage: 2 x 4 columns for the rows' scales, 2 x 8 for the columns' (128 + 128 rows)
           const uint32_t ts = tmem + PAIR_COLS + stage * 24;
-#pragma unroll
-          for (uint32_t k = 0; k < 2; ++k) {
-            ptx::tmem_cp_scales<true>(ts + k * 4, scale_desc(scales + k * SCALE_TILE));
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h)
-              ptx::tmem_cp_scales<true>(ts + 8 + k * 8 + h * 4, scale_desc(scales + (2 + h * 2 + k) * SCALE_TILE));
-          }
-          const uint64_t da = code_desc(src), db = code_desc(src + ROW_CODES);
+          const uint64_t da = code_desc(src), db = code_desc(src + ROW_CODES), ds = scale_desc(src + 2 * ROW_CODES);
           const uint32_t steps = min(STEPS, p.ksteps - kb * STEPS);
-          for (uint32_t k = 0; k < steps; ++k)
-            ptx::mma_mxf4<true>(tmem, da + k * 2, db + k * 2, (k & 1) ? idesc1 : idesc0, ts + (k >> 1) * 4,
-                                ts + 8 + (k >> 1) * 8, (kb | k) ? 1u : 0u);
-          ptx::mma_commit_pair(empty_bar(stage), 3);
+          if (ptx::elect_one()) {
+#pragma unroll
+            for (uint32_t k = 0; k < 2; ++k) {
+              ptx::tmem_cp_scales<true>(ts + k * 4, ds + k * (SCALE_TILE >> 4));
+#pragma unroll
+              for (uint32_t h = 0; h < 2; ++h)
+                ptx::tmem_cp_scales<true>(ts + 8 + k * 8 + h * 4, ds + (2 + h * 2 + k) * (SCALE_TILE >> 4));
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < STEPS; ++k)
+              if (k < steps)
+                ptx::mma_mxf4<true>(tmem, da + k * 2, db + k * 2, (k & 1) ? idesc1 : idesc0, ts + (k >> 1) * 4,
+                                    ts + 8 + (k >> 1) * 8, (in_chunk || k) ? 1u : 0u);
+            ptx::mma_commit_pair(empty_bar(stage), 3);
+            if (in_chunk + 1 == CHUNK || kb + 1 == p.kblocks) ptx::mma_commit_pair(tfull_bar, 3);
+          }
+          __syncwarp();
+          if (++in_chunk == CHUNK) in_chunk = 0;
           if (++stage == PAIR_STAGES) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (alive) ptx::mma_commit_pair(tfull_bar, 3);
       }
     }
-    __syncwarp();
   } else {
     const uint32_t quarter = warp & 3u, half = (warp - 2u) >> 2;
-    uint32_t local = 0;
-    for (uint32_t t = pair; t < p.num_tiles; t += pairs, ++local) {
+    const uint32_t taddr = tmem + ((quarter * 32u) << 16) + half * 128u;
+    const uint32_t chunks = (p.kblocks + CHUNK - 1) / CHUNK;
+    uint32_t filled = 0;
+    for (uint32_t t = pair; t < p.num_tiles; t += pairs) {
       uint32_t tn, tm;
       pair_tile(p, t, tn, tm);
-      bool ok = ptx::mbar_wait(tfull_bar, local & 1u, abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
+      float sum[4][32];
+      bool ok = true;
+      for (uint32_t ch = 0; ch < chunks; ++ch) {
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(tfull_bar, filled, abort_flag));
+        filled ^= 1u;
+        if (!ok) break;
+        ptx::tc_fence_after();
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c) take_columns(taddr + c * 32u, sum[c], ch == 0);
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(tempty_bar, 0));
+      }
       if (!ok) {
         if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 3, 0, t, 0);
         break;
       }
-      ptx::tc_fence_after();
-      uint32_t v[4][32];
-      const uint32_t taddr = tmem + ((quarter * 32u) << 16) + half * 128u;
-#pragma unroll
-      for (uint32_t c = 0; c < 4; ++c) ptx::tmem_ld_32x32(taddr + c * 32u, v[c]);
-      ptx::tmem_ld_wait();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(tempty_bar, 0));
       const uint64_t n = uint64_t(tn * 2 + rank) * ROWS + quarter * 32u + lane;
       const uint32_t m0 = tm * PAIR_COLS + half * 128u;
-      const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+      float* out = p.c + uint64_t(m0) * p.N + n;
       if (n < p.N) {
-        float* out = p.c + uint64_t(m0) * p.N + n;
+        const float bias = p.bias ? p.bias[n] : 0.f;
+        if (m0 + 128 <= p.M) {
 #pragma unroll
-        for (uint32_t c = 0; c < 4; ++c)
+          for (uint32_t j = 0; j < 128; ++j, out += p.N) *out = finish<CLASS>(p, sum[j / 32][j % 32], bias);
+        } else {
 #pragma unroll
-          for (uint32_t j = 0; j < 32; ++j)
-            if (m0 + c * 32 + j < p.M)
-              out[uint64_t(c * 32 + j) * p.N] = apply_act(__uint_as_float(v[c][j]) + bias, p.act, p.act_param);
+          for (uint32_t j = 0; j < 128; ++j, out += p.N)
+            if (m0 + j < p.M) *out = finish<CLASS>(p, sum[j / 32][j % 32], bias);
+        }
       }
     }
   }
@@ -467,27 +518,41 @@ bool allow_smem(uint32_t bytes) {
   return done[dev & 63];
 }
 
-template <int BN, int STAGES>
-const char* launch_single(const Mxfp4Product& q, const Mxfp4Layout& la, const Mxfp4Layout& lb, Params p,
-                          uint32_t units, cudaStream_t stream) {
+template <int BN, int STAGES, int CLASS>
+const char* launch_single(const Mxfp4Product& q, const Mxfp4Layout& la, const Mxfp4Layout& lb, const Params& p,
+                          cudaStream_t stream) {
   CUtensorMap rows, row_scales, cols, col_scales;
   if (!code_map(&rows, q.b, lb, ROWS) || !scale_map(&row_scales, q.b, lb, 1) || !code_map(&cols, q.a, la, BN) ||
       !scale_map(&col_scales, q.a, la, 1))
     return "cuTensorMapEncodeTiled failed";
-  constexpr auto kern = mxfp4_single_kernel<BN, STAGES>;
+  constexpr auto kern = mxfp4_single_kernel<BN, STAGES, CLASS>;
   constexpr uint32_t smem = SingleShape<BN, STAGES>::SMEM;
   static_assert(smem <= SMEM_LIMIT, "shared memory");
   if (!allow_smem<kern>(smem)) return "cudaFuncSetAttribute(max dynamic shared memory) failed";
-  if (launch_kernel(kern, dim3(units), dim3(SINGLE_THREADS), smem, stream, rows, row_scales, cols, col_scales, p) !=
-      cudaSuccess)
+  if (launch_kernel_cluster(kern, p.splits, dim3(p.num_tiles * p.splits), dim3(SINGLE_THREADS), smem, stream, rows,
+                            row_scales, cols, col_scales, p) != cudaSuccess)
     return "product launch failed";
   return nullptr;
 }
 
-}  // namespace
+template <int CLASS>
+const char* launch_pair(const Mxfp4Product& q, const Mxfp4Layout& la, const Mxfp4Layout& lb, const Params& p,
+                        int sm_count, cudaStream_t stream) {
+  CUtensorMap rows, row_scales, cols, col_scales;
+  if (!code_map(&rows, q.b, lb, ROWS) || !scale_map(&row_scales, q.b, lb, 1) || !code_map(&cols, q.a, la, ROWS) ||
+      !scale_map(&col_scales, q.a, la, 2))
+    return "cuTensorMapEncodeTiled failed";
+  constexpr auto kern = mxfp4_pair_kernel<CLASS>;
+  if (!allow_smem<kern>(PAIR_SMEM)) return "cudaFuncSetAttribute(max dynamic shared memory) failed";
+  const uint32_t pairs = std::min(uint32_t(sm_count) / 2, p.num_tiles);
+  if (launch_kernel(kern, dim3(2 * pairs), dim3(PAIR_THREADS), PAIR_SMEM, stream, rows, row_scales, cols, col_scales,
+                    p) != cudaSuccess)
+    return "product launch failed";
+  return nullptr;
+}
 
-const char* launch_mxfp4_product(const Mxfp4Product& q, GemmStatus* status, int sm_count, float* ws, size_t ws_bytes,
-                                 uint32_t* counters, uint32_t counter_slots, cudaStream_t stream) {
+template <int CLASS>
+const char* launch_class(const Mxfp4Product& q, GemmStatus* status, int sm_count, cudaStream_t stream) {
   const Mxfp4Layout la(q.M, q.K), lb(q.N, q.K);
   Params p{};
   p.M = uint32_t(q.M);
@@ -502,38 +567,32 @@ const char* launch_mxfp4_product(const Mxfp4Product& q, GemmStatus* status, int 
   p.act_param = q.act_param;
   p.status = status;
   const uint64_t pair_tiles = ((q.N + 255) / 256) * ((q.M + 255) / 256);
+  if (pair_tiles >= (1ull << 30)) return "too many tiles";
   if (pair_tiles >= 64) {
-    if (pair_tiles >= (1ull << 31)) return "too many tiles";
     p.tiles_n = uint32_t((q.N + 255) / 256);
     p.tiles_m = uint32_t((q.M + 255) / 256);
     p.num_tiles = uint32_t(pair_tiles);
-    CUtensorMap rows, row_scales, cols, col_scales;
-    if (!code_map(&rows, q.b, lb, ROWS) || !scale_map(&row_scales, q.b, lb, 1) || !code_map(&cols, q.a, la, ROWS) ||
-        !scale_map(&col_scales, q.a, la, 2))
-      return "cuTensorMapEncodeTiled failed";
-    if (!allow_smem<mxfp4_pair_kernel>(PAIR_SMEM)) return "cudaFuncSetAttribute(max dynamic shared memory) failed";
-    const uint32_t pairs = std::min(uint32_t(sm_count) / 2, p.num_tiles);
-    if (launch_kernel(mxfp4_pair_kernel, dim3(2 * pairs), dim3(PAIR_THREADS), PAIR_SMEM, stream, rows, row_scales, cols,
-                      col_scales, p) != cudaSuccess)
-      return "product launch failed";
-    return nullptr;
+    return launch_pair<CLASS>(q, la, lb, p, sm_count, stream);
   }
   const uint32_t bn = q.M <= 32 ? 32 : q.M <= 64 ? 64 : 128;
   p.tiles_n = uint32_t((q.N + ROWS - 1) / ROWS);
   p.tiles_m = uint32_t((q.M + bn - 1) / bn);
   p.num_tiles = p.tiles_n * p.tiles_m;
-  // few tiles: share each one's K among several CTAs
-  uint32_t splits = std::max(1u, uint32_t(sm_count) / p.num_tiles);
-  splits = std::min(splits, p.kblocks);
-  if (p.num_tiles > counter_slots || uint64_t(p.num_tiles) * splits * bn * ROWS * 4 > ws_bytes) splits = 1;
+  // few tiles: share each one's K among the CTAs of a cluster
+  const uint32_t splits = std::min({std::max(1u, uint32_t(sm_count) / p.num_tiles), p.kblocks, 8u});
   p.kb_per_split = (p.kblocks + splits - 1) / splits;
   p.splits = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;
-  p.ws = ws;
-  p.counters = counters;
-  const uint32_t units = p.num_tiles * p.splits;
-  return bn == 32   ? launch_single<32, 6>(q, la, lb, p, units, stream)
-         : bn == 64 ? launch_single<64, 4>(q, la, lb, p, units, stream)
-                    : launch_single<128, 4>(q, la, lb, p, units, stream);
+  return bn == 32   ? launch_single<32, 6, CLASS>(q, la, lb, p, stream)
+         : bn == 64 ? launch_single<64, 4, CLASS>(q, la, lb, p, stream)
+                    : launch_single<128, 4, CLASS>(q, la, lb, p, stream);
+}
+
+}  // namespace
+
+const char* launch_mxfp4_product(const Mxfp4Product& q, GemmStatus* status, int sm_count, cudaStream_t stream) {
+  if (q.act == ACT_RELU) return launch_class<RELU>(q, status, sm_count, stream);
+  if (q.act >= ACT_RELU && q.act <= ACT_GELU) return launch_class<OTHER>(q, status, sm_count, stream);
+  return launch_class<IDENTITY>(q, status, sm_count, stream);
 }
 
 }  // namespace gonn
