@@ -8,6 +8,13 @@
 // (m, S, U) merge by
 //   m' = max(m1, m2),  S' = sum_i S_i e^(m_i-m'),  U' = sum_i e^(m_i-m') (U_i + (m_i-m') S_i).
 // log p(t) = (x_t - m) - log S, and the entropy is log S - U / S.
+//
+// Short rows (up to 1024 logits) are held in the registers of one warp.  Longer ones are streamed
+// by a block of 256 threads, 32 logits a thread in flight; few long rows are shared by the up to 8
+// blocks of a cluster, which merge what they found through distributed shared memory.  All merges
+// have a fixed order: results repeat bit for bit.
+#include <algorithm>
+
 #include "kernels.h"
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -17,8 +24,11 @@ namespace gonn {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int THREADS = 256;
-constexpr int WARPS = THREADS / 32;
+constexpr int BLOCK = 256;
+constexpr int WARPS = BLOCK / 32;
+constexpr uint32_t QUADS = 8;                       // 16-byte loads a thread has in flight
+constexpr uint32_t WARP_ROW = 1024;                 // longest row that one warp holds
+constexpr uint32_t MAX_SHARE = 8;                   // blocks of a cluster
 
 __device__ __forceinline__ void report_index(GemmStatus* st, uint32_t kind, uint64_t row, int index) {
   volatile GemmStatus* v = st;  // mapped host memory: plain stores, the first report wins
@@ -30,77 +40,110 @@ __device__ __forceinline__ void report_index(GemmStatus* st, uint32_t kind, uint
   }
 }
 
-// Running statistics of part of a row.  `c` is log2(e) / T of the tempered sum.
+// 2^x for sums: results below 2^-126 become 0.
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---- statistics of (part of) a row ------------------------------------------------------
+// What is summed beside S: nothing; U for the entropy; or the tempered sum e^((x-m)/T), with
+// `c` = log2(e) / T.
+enum class Sum : int { Plain = 0, Entropy = 1, Tempered = 2 };
+
 struct RowStats {
-  float m = -INFINITY;  // maximum
-  float s = 0.f;        // sum e^(x-m)
-  float u = 0.f;        // ENTROPY: sum e^(x-m) (x-m); else the tempered sum e^((x-m)/T)
+  float m = -INFINITY;
+  float s = 0.f;
+  float u = 0.f;
 };
 
 // The maximum that differences are taken from: a part that has seen nothing but -inf takes
 // them from 0, so that its elements still give e^-inf = 0 and not NaN.
 __device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
 
-template <bool ENTROPY>
+// Plain: `c` = log2(e) / T gives S itself a temperature.
+template <Sum SUM>
 __device__ __forceinline__ void rescale(RowStats& r, float m_new, float c) {
   if (m_new == r.m) return;
   if (r.m != -INFINITY) {
     const float d = r.m - m_new;
-    const float f = exp2f(d * kLog2e);
+    const float f = exp2f(d * (SUM == Sum::Plain ? c : kLog2e));
     // where f is 0 the limit keeps d S finite (the difference itself may be -inf)
-    r.u = ENTROPY ? f * (r.u + fmaxf(d, -1e4f) * r.s) : r.u * exp2f(d * c);
+    if (SUM == Sum::Entropy) r.u = f * (r.u + fmaxf(d, -1e4f) * r.s);
+    if (SUM == Sum::Tempered) r.u *= exp2f(d * c);
     r.s *= f;
   }
   r.m = m_new;
 }
 
-template <bool ENTROPY>
+template <Sum SUM>
 __device__ __forceinline__ void add(RowStats& r, float x, float ref, float c) {
   const float d = x - ref;
-  const float e = exp2f(d * kLog2e);
+  const float e = exp2_ftz(d * (SUM == Sum::Plain ? c : kLog2e));
   r.s += e;
   // a masked element (-inf) adds e = 0 times a finite number
-  if (ENTROPY) r.u += e * fmaxf(d, -1e30f);
-  else r.u += exp2f(d * c);
+  if (SUM == Sum::Entropy) r.u = fmaf(e, fmaxf(d, -1e30f), r.u);
+  if (SUM == Sum::Tempered) r.u += exp2_ftz(d * c);
 }
 
-template <bool ENTROPY>
+template <Sum SUM>
 __device__ __forceinline__ void merge(RowStats& a, RowStats b, float c) {
   const float m = fmaxf(a.m, b.m);
-  rescale<ENTROPY>(a, m, c);
-  rescale<ENTROPY>(b, m, c);
+  rescale<SUM>(a, m, c);
+  rescale<SUM>(b, m, c);
   a.s += b.s;
   a.u += b.u;
 }
 
-// The statistics of the whole row in every thread.  The order of the merges is fixed.
-template <bool ENTROPY>
-__device__ RowStats block_merge(RowStats r, float c, RowStats* smem) {
+template <Sum SUM>
+__device__ __forceinline__ RowStats warp_merge(RowStats r, float c) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     RowStats other;
     other.m = __shfl_xor_sync(0xffffffffu, r.m, o);
     other.s = __shfl_xor_sync(0xffffffffu, r.s, o);
     other.u = __shfl_xor_sync(0xffffffffu, r.u, o);
-    merge<ENTROPY>(r, other, c);
+    // both sides add the lower lane's part first: every lane ends with the same bits
+    if (threadIdx.x & o) {
+      merge<SUM>(other, r, c);
+      r = other;
+    } else {
+      merge<SUM>(r, other, c);
+    }
   }
+  return r;
+}
+
+template <Sum SUM>
+__device__ RowStats block_merge(RowStats r, float c, RowStats* smem) {
+  r = warp_merge<SUM>(r, c);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = r;
   __syncthreads();
   r = smem[0];
-  for (int w = 1; w < WARPS; ++w) merge<ENTROPY>(r, smem[w], c);
+  for (int w = 1; w < WARPS; ++w) merge<SUM>(r, smem[w], c);
   return r;
 }
 
-template <bool ENTROPY>
-__device__ RowStats row_stats(const float* x, uint64_t n, float c, RowStats* smem) {
-  RowStats r;
-  for (uint64_t i = threadIdx.x; i < n; i += THREADS) {
-    const float v = x[i];
-    rescale<ENTROPY>(r, fmaxf(r.m, v), c);
-    add<ENTROPY>(r, v, reference(r.m), c);
+// The statistics of all blocks of the cluster, in the order of their ranks; `slot` is this block's.
+// Everything the blocks did before is visible to all of them afterwards.
+template <Sum SUM>
+__device__ RowStats cluster_merge(RowStats r, float c, RowStats* slot, uint32_t shares) {
+  if (threadIdx.x == 0) *slot = r;
+  __syncthreads();
+  ptx::cluster_sync_all();
+  const uint32_t at = ptx::smem_u32(slot);
+  for (uint32_t k = 0; k < shares; ++k) {
+    const uint32_t there = ptx::mapa_shared(at, k);
+    RowStats other;
+    other.m = ptx::ld_shared_cluster(there);
+    other.s = ptx::ld_shared_cluster(there + 4);
+    other.u = ptx::ld_shared_cluster(there + 8);
+    if (k == 0) r = other;
+    else merge<SUM>(r, other, c);
   }
-  return block_merge<ENTROPY>(r, c, smem);
+  return r;
 }
 
 // log p of a logit: NaN for a row that holds a NaN or +inf, -inf for a masked token and for
@@ -110,59 +153,385 @@ __device__ __forceinline__ float log_prob(const RowStats& r, float x) {
   return (x - r.m) - logf(r.s);
 }
 
-// Orders like (value, lowest index first): larger keys come first among the alternatives.
-// -0 counts as 0.
-__device__ __forceinline__ uint64_t order_key(float x, uint32_t index) {
-  uint32_t b = __float_as_uint(x + 0.f);
-  b = (b & 0x80000000u) ? ~b : b | 0x80000000u;
-  return (uint64_t(b) << 32) | (0xffffffffu - index);
+// ---- a block's part of a long row --------------------------------------------------------
+// Whole 16-byte pieces of the row's memory, split evenly over the blocks of the cluster; the up to
+// three logits before the first piece belong to the first block and those behind the last one to
+// the last block, a thread each ("extra").
+struct Part {
+  const float4* quads;  // first piece of the row
+  uint32_t lead;        // logits before it
+  uint32_t q0, q1;      // this block's pieces
+  int extra;            // this thread's logit outside the pieces, or -1
+  uint32_t first, end;  // this block's logits
+};
+
+__device__ __forceinline__ Part part_of(const float* x, uint32_t vocab, uint32_t rank, uint32_t shares) {
+  Part p;
+  p.lead = min(uint32_t((16u - (reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / 4u, vocab);
+  const uint32_t all = (vocab - p.lead) / 4u, tail = vocab - p.lead - all * 4u;
+  p.quads = reinterpret_cast<const float4*>(x + p.lead);
+  p.q0 = uint32_t(uint64_t(all) * rank / shares);
+  p.q1 = uint32_t(uint64_t(all) * (rank + 1) / shares);
+  const bool head = rank == 0, last = rank + 1 == shares;
+  const uint32_t t = threadIdx.x;
+  p.extra = t < 4 ? (head && t < p.lead ? int(t) : -1) : (last && t - 4u < tail ? int(p.lead + all * 4u + t - 4u) : -1);
+  p.first = head ? 0u : p.lead + p.q0 * 4u;
+  p.end = last ? vocab : p.lead + p.q1 * 4u;
+  return p;
 }
 
-__global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobArgs a) {
+__device__ __forceinline__ float4 masked_quad() { return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
+
+__device__ __forceinline__ void load_quads(const Part& p, uint32_t q, float4 (&v)[QUADS]) {
+#pragma unroll
+  for (uint32_t j = 0; j < QUADS; ++j) {
+    const uint32_t at = q + j * BLOCK + threadIdx.x;
+    v[j] = at < p.q1 ? p.quads[at] : masked_quad();
+  }
+}
+
+__device__ __forceinline__ float max4(const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+
+// Adds a thread's 32 logits; returns their maximum.
+template <Sum SUM>
+__device__ __forceinline__ float add_quads(RowStats& r, const float4 (&v)[QUADS], float c) {
+  float most = max4(v[0]);
+#pragma unroll
+  for (uint32_t j = 1; j < QUADS; ++j) most = fmaxf(most, max4(v[j]));
+  if (most > r.m) rescale<SUM>(r, most, c);
+  const float ref = reference(r.m);
+#pragma unroll
+  for (uint32_t j = 0; j < QUADS; ++j) {
+    add<SUM>(r, v[j].x, ref, c);
+    add<SUM>(r, v[j].y, ref, c);
+    add<SUM>(r, v[j].z, ref, c);
+    add<SUM>(r, v[j].w, ref, c);
+  }
+  return most;
+}
+
+template <Sum SUM>
+__device__ __forceinline__ void add_one(RowStats& r, float x, float c) {
+  if (x > r.m) rescale<SUM>(r, x, c);
+  add<SUM>(r, x, reference(r.m), c);
+}
+
+// ---- alternatives -------------------------------------------------------------------------
+// Orders like (value, lowest index first): larger keys come first among the alternatives.
+// -0 counts as 0.
+__device__ __forceinline__ uint32_t order_bits(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t order_key(float x, uint32_t index) {
+  return (uint64_t(order_bits(x)) << 32) | (0xffffffffu - index);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu - uint32_t(key); }
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t b = uint32_t(key >> 32);
+  return __uint_as_float((b & 0x80000000u) ? b & 0x7fffffffu : ~b);
+}
+constexpr uint32_t kMaskedBits = 0x007fffffu;  // order_bits(-inf); below it only NaN
+
+// The largest `want` keys a block has met.  A key is kept when it lies above a floor that is known
+// to have `want` keys above it.  The first floor comes from the threads' maxima of their first 32
+// logits (as many of those as wanted lie above it, so as many logits do), which leaves about
+// want * n / 8192 keys of n; when the buffer runs over the limit, the keys below the exact
+// want-th one are thrown out and it becomes the floor.
+struct Selection {
+  static constexpr uint32_t CAP = 2048, LIMIT = 1024;
+  uint64_t key[CAP];
+  uint64_t sorted[kMaxTop];
+  uint64_t floor;
+  uint32_t count;
+  uint32_t part[2][WARPS];
+};
+
+// Sum over the block of a count; `turn` alternates so that one barrier a call is enough.
+__device__ __forceinline__ uint32_t block_count(Selection& s, uint32_t n, uint32_t& turn) {
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) s.part[turn][threadIdx.x >> 5] = n;
+  __syncthreads();
+  uint32_t all = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) all += s.part[turn][w];
+  turn ^= 1u;
+  return all;
+}
+
+// Throws out all but the `want` largest of the n > want keys (all different): bit by bit, the
+// largest floor that still has `want` keys at or above it.  Ends with a barrier.
+__device__ void keep_largest(Selection& s, uint32_t n, uint32_t want) {
+  constexpr uint32_t PER = Selection::CAP / BLOCK;
+  uint64_t mine[PER];
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i) {
+    const uint32_t at = i * BLOCK + threadIdx.x;
+    mine[i] = at < n ? s.key[at] : 0ull;
+  }
+  uint64_t floor = 0;
+  uint32_t turn = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t trial = floor | (1ull << bit);
+    uint32_t above = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) above += mine[i] >= trial;
+    above = block_count(s, above, turn);
+    if (above >= want) floor = trial;
+    if (above == want) break;
+  }
+  if (threadIdx.x == 0) {
+    s.count = 0;
+    s.floor = floor;
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < PER; ++i)
+    if (mine[i] >= floor && mine[i] != 0) s.key[atomicAdd(&s.count, 1u)] = mine[i];
+  __syncthreads();
+}
+
+// The first floor from the threads' maxima: 20 bits of it.
+__device__ void first_floor(Selection& s, float most, uint32_t want) {
+  const uint32_t bits = order_bits(most);
+  uint32_t floor = 0;
+  for (int bit = 31; bit >= 12; --bit) {
+    const uint32_t trial = floor | (1u << bit);
+    const uint32_t above = uint32_t(__syncthreads_count(bits >= trial));
+    if (above >= want) floor = trial;
+    if (above == want) break;
+  }
+  if (threadIdx.x == 0) {
+    s.floor = uint64_t(floor) << 32;
+    s.count = 0;
+  }
+  __syncthreads();
+}
+
+// Offers a thread's logits (8 quads of the row from `q`, of which `most` is the maximum, and the
+// logit outside the quads) to the selection.  All threads of the block call it.
+__device__ __forceinline__ void offer(Selection& s, const float* x, const Part& p, uint32_t q,
+                                      const float4 (&v)[QUADS], float most, float extra, uint32_t want) {
+  uint64_t floor = s.floor;
+  // a floor below the order of -inf lets everything pass
+  float low = uint32_t(floor >> 32) <= kMaskedBits ? -INFINITY : key_value(floor);
+  uint32_t hits = 0;       // logits that may lie above the floor, a bit each
+  bool outside = p.extra >= 0 && extra >= low;
+  if (most >= low) {
+#pragma unroll
+    for (uint32_t j = 0; j < QUADS; ++j) {
+      const uint32_t four = uint32_t(v[j].x >= low) | uint32_t(v[j].y >= low) << 1 | uint32_t(v[j].z >= low) << 2 |
+                            uint32_t(v[j].w >= low) << 3;
+      if (q + j * BLOCK + threadIdx.x < p.q1) hits |= four << (4 * j);
+    }
+  }
+  while (true) {
+    bool over = false;
+    uint32_t left = hits;
+    while (left | uint32_t(outside)) {
+      // few logits get here; their values are read again (from L1) rather than picked out of the
+      // registers
+      uint32_t index = uint32_t(p.extra), bit = 0;
+      if (left) {
+        bit = left & (0u - left);
+        const uint32_t i = 31u - uint32_t(__clz(int(bit)));
+        index = p.lead + (q + (i >> 2) * BLOCK + threadIdx.x) * 4u + (i & 3u);
+        left ^= bit;
+      } else {
+        outside = false;
+      }
+      const uint64_t key = order_key(x[index], index);
+      bool stored = true;
+      if (key >= floor) {
+        const uint32_t at = atomicAdd(&s.count, 1u);
+        over = over || at >= Selection::LIMIT;
+        stored = at < Selection::CAP;
+        if (stored) s.key[at] = key;
+      }
+      if (stored) {
+        hits &= ~bit;
+      } else if (bit == 0) {
+        outside = true;
+        break;  // the buffer is full: nothing after this one fits either
+      }
+    }
+    if (!__syncthreads_or(over)) return;
+    keep_largest(s, min(s.count, Selection::CAP), want);
+    floor = s.floor;
+    if (!__syncthreads_or(hits != 0 || outside)) return;
+  }
+}
+
+// Sorts the selection's keys: s.sorted[0 .. min(n, want)) in descending order.  Returns how many.
+__device__ uint32_t sort_selection(Selection& s, uint32_t want) {
+  __syncthreads();
+  uint32_t n = s.count;
+  if (n > 512 && n > want) {
+    keep_largest(s, n, want);
+    n = want;
+  }
+  // a key's place is the number of keys above it
+  for (uint32_t i = threadIdx.x; i < n; i += BLOCK) {
+    const uint64_t mine = s.key[i];
+    uint32_t place = 0;
+#pragma unroll 8
+    for (uint32_t j = 0; j < n; ++j) place += s.key[j] > mine;
+    if (place < want) s.sorted[place] = mine;
+  }
+  __syncthreads();
+  return min(n, want);
+}
+
+// ---- log probabilities ----------------------------------------------------------------------
+__device__ __forceinline__ float token_logprob(const LogprobArgs& a, const RowStats& r, uint64_t row, const float* x,
+                                               uint32_t t) {
+  const int token = a.tokens[row * a.n_tokens + t];
+  if (token < 0) return 0.f;  // none
+  if (uint64_t(token) >= a.vocab) {
+    report_index(a.status, INDEX_TOKEN, row, token);
+    return NAN;
+  }
+  return log_prob(r, x[token]);
+}
+__device__ __forceinline__ float row_entropy(const RowStats& r) {
+  return r.s == 0.f ? 0.f : logf(r.s) - r.u / r.s;
+}
+
+template <bool TOP>
+__global__ void __launch_bounds__(BLOCK, 4) logprobs_block_kernel(const LogprobArgs a, uint32_t shares) {
   ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
   ptx::grid_dependency_wait();
-  __shared__ RowStats smem[WARPS];
-  __shared__ uint64_t best_of[WARPS];
-  for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const float* x = a.x + row * a.ld;
-    const RowStats r = row_stats<true>(x, a.vocab, 0.f, smem);
+  __shared__ RowStats merged[WARPS], slot;
+  __shared__ Selection sel;
+  const uint32_t rank = blockIdx.x % shares;
+  const uint64_t row = blockIdx.x / shares;
+  const float* x = a.x + row * a.ld;
+  const Part p = part_of(x, uint32_t(a.vocab), rank, shares);
+  RowStats r;
+  const float extra = p.extra >= 0 ? x[p.extra] : -INFINITY;
+  add_one<Sum::Entropy>(r, extra, 0.f);
+  for (uint32_t q = p.q0; q < p.q1 || q == p.q0; q += QUADS * BLOCK) {
+    float4 v[QUADS];
+    load_quads(p, q, v);
+    const float most = add_quads<Sum::Entropy>(r, v, 0.f);
+    if (TOP) {
+      const bool first = q == p.q0;
+      if (first) first_floor(sel, fmaxf(most, extra), a.top_n);
+      Part mine = p;
+      if (!first) mine.extra = -1;
+      offer(sel, x, mine, q, v, most, extra, a.top_n);
+    }
+  }
+  r = block_merge<Sum::Entropy>(r, 0.f, merged);
+  uint32_t found = 0;
+  if (TOP) found = sort_selection(sel, a.top_n);
+  if (shares > 1) {
+    if (TOP && threadIdx.x == 0) sel.count = found;
+    r = cluster_merge<Sum::Entropy>(r, 0.f, &slot, shares);
+    if (TOP && rank == 0) {
+      // the blocks' own alternatives, at most 8 x 128, behind one another
+      uint32_t n = found;
+      __syncthreads();
+      if (threadIdx.x < found) sel.key[threadIdx.x] = sel.sorted[threadIdx.x];
+      for (uint32_t k = 1; k < shares; ++k) {
+        const uint32_t theirs = ptx::ld_shared_cluster_u32(ptx::mapa_shared(ptx::smem_u32(&sel.count), k));
+        if (threadIdx.x < theirs)
+          sel.key[n + threadIdx.x] =
+              ptx::ld_shared_cluster_u64(ptx::mapa_shared(ptx::smem_u32(&sel.sorted[threadIdx.x]), k));
+        n += theirs;
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) sel.count = n;
+      found = sort_selection(sel, a.top_n);
+    }
+    ptx::cluster_sync_all();  // no block leaves while another still reads its shared memory
+    if (rank != 0) return;
+  }
+  for (uint32_t t = threadIdx.x; t < a.n_tokens; t += BLOCK)
+    a.logprobs[row * a.n_tokens + t] = token_logprob(a, r, row, x, t);
+  if (a.entropy && threadIdx.x == 0) a.entropy[row] = row_entropy(r);
+  if (TOP && threadIdx.x < a.top_n) {
     const bool nan = !(r.s == r.s);
-    for (uint32_t t = threadIdx.x; t < a.n_tokens; t += THREADS) {
-      const int token = a.tokens[row * a.n_tokens + t];
-      float lp = 0.f;  // no token
-      if (token >= 0 && uint64_t(token) >= a.vocab) {
-        report_index(a.status, INDEX_TOKEN, row, token);
-        lp = NAN;
-      } else if (token >= 0) {
-        lp = log_prob(r, x[token]);
+    const uint32_t index = key_index(sel.sorted[threadIdx.x]);
+    a.top_tokens[row * a.top_n + threadIdx.x] = nan ? -1 : int(index);
+    a.top_logprobs[row * a.top_n + threadIdx.x] = nan ? NAN : log_prob(r, x[index]);
+  }
+}
+
+// One warp a row, PER logits a lane in registers.
+template <int PER>
+__device__ __forceinline__ void load_row(const float* x, uint32_t vocab, uint32_t lane, float (&v)[PER]) {
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const uint32_t i = uint32_t(j) * 32u + lane;
+    v[j] = i < vocab ? x[i] : -INFINITY;
+  }
+}
+template <Sum SUM, int PER>
+__device__ __forceinline__ RowStats stats_of(const float (&v)[PER], float c) {
+  RowStats r;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) r.m = fmaxf(r.m, v[j]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) r.m = fmaxf(r.m, __shfl_xor_sync(0xffffffffu, r.m, o));
+  const float ref = reference(r.m);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) add<SUM>(r, v[j], ref, c);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+    r.u += __shfl_xor_sync(0xffffffffu, r.u, o);
+  }
+  return r;
+}
+
+template <int PER>
+__global__ void __launch_bounds__(BLOCK) logprobs_warp_kernel(const LogprobArgs a) {
+  ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
+  ptx::grid_dependency_wait();
+  const uint32_t lane = threadIdx.x & 31, vocab = uint32_t(a.vocab);
+  const uint64_t row = uint64_t(blockIdx.x) * WARPS + (threadIdx.x >> 5);
+  if (row >= a.rows) return;
+  const float* x = a.x + row * a.ld;
+  float v[PER];
+  load_row<PER>(x, vocab, lane, v);
+  const RowStats r = stats_of<Sum::Entropy, PER>(v, 0.f);
+  for (uint32_t t = lane; t < a.n_tokens; t += 32) a.logprobs[row * a.n_tokens + t] = token_logprob(a, r, row, x, t);
+  if (a.entropy && lane == 0) a.entropy[row] = row_entropy(r);
+  if (a.top_n == 0) return;
+  const bool nan = !(r.s == r.s);
+  // every round takes the largest logit that is left, the lowest index among equal ones; `taken`
+  // marks the lane's logits that are gone
+  uint32_t taken = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (uint32_t(j) * 32u + lane >= vocab) taken |= 1u << j;
+  uint32_t best = 0, best_j = 0;  // the lane's largest order bits (0: none left) and which logit has them
+  auto look = [&] {
+    best = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint32_t b = order_bits(v[j]);
+      if (!(taken >> j & 1u) && b > best) {  // ascending j: equal logits keep the lowest index
+        best = b;
+        best_j = uint32_t(j);
       }
-      a.logprobs[row * a.n_tokens + t] = lp;
     }
-    if (a.entropy && threadIdx.x == 0) a.entropy[row] = r.s == 0.f ? 0.f : logf(r.s) - r.u / r.s;
-    uint64_t last = ~0ull;
-    for (uint32_t k = 0; k < a.top_n; ++k) {
-      uint64_t best = 0;
-      for (uint64_t i = threadIdx.x; i < a.vocab; i += THREADS) {
-        const uint64_t key = order_key(x[i], uint32_t(i));
-        if (key < last && key > best) best = key;
-      }
-      for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
-        if (other > best) best = other;
-      }
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) best_of[threadIdx.x >> 5] = best;
-      __syncthreads();
-      for (int w = 0; w < WARPS; ++w)
-        if (best_of[w] > best) best = best_of[w];
-      last = best;
-      if (threadIdx.x == 0) {
-        const uint32_t index = 0xffffffffu - uint32_t(best);
-        a.top_tokens[row * a.top_n + k] = nan ? -1 : int(index);
-        a.top_logprobs[row * a.top_n + k] = nan ? NAN : log_prob(r, x[index]);
-      }
+  };
+  look();
+  for (uint32_t k = 0; k < a.top_n; ++k) {
+    const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+    const uint32_t index = __reduce_min_sync(0xffffffffu, best == most ? best_j * 32u + lane : 0xffffffffu);
+    if (lane == (k & 31u)) {
+      const float value = key_value(uint64_t(most) << 32);
+      a.top_tokens[row * a.top_n + k] = nan ? -1 : int(index);
+      a.top_logprobs[row * a.top_n + k] = nan ? NAN : log_prob(r, value);
     }
-    __syncthreads();
+    if ((index & 31u) == lane) {
+      taken |= 1u << (index >> 5);
+      look();
+    }
+    __syncwarp();
   }
 }
 
@@ -171,166 +540,427 @@ __global__ void __launch_bounds__(THREADS) token_logprobs_kernel(const LogprobAr
 // vocabulary, logit above -inf), p_T = softmax(x / T), p = softmax(x):
 //   loss = w T^2 sum_k q_k (log q_k - log p_T[idx_k]) + (1-w) (-log p[label])
 //   dx_j = g (w T (p_T[j] - sum_{k: idx_k = j} q_k) + (1-w) (p[j] - [j = label]))
-// What a row's teacher and label take away from the gradient at single places, and the row's
-// loss, come from this per-row state in shared memory.
+// The statistics keep S_1 = sum e^(x-m) in `s` and S_T = sum e^((x-m)/T) in `u`; where only one of
+// them is wanted, or T is 1, only that one is summed.
 struct Targets {
-  int index[kMaxTop + 1];    // teacher tokens, then the label; -1: not there
-  float take[kMaxTop + 1];   // q_k, then 1 for the label
-  float soft, hard;          // 1 where the row has a teacher / a label
-  float loss;
+  int index[kMaxTop + 1];   // teacher tokens, then the label; -1: not there
+  float take[kMaxTop + 1];  // q_k, then 1 for the label
 };
 
-__device__ float block_reduce(float v, bool is_max, float* smem) {
-  for (int o = 16; o > 0; o >>= 1) {
-    const float w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = is_max ? fmaxf(v, w) : v + w;
-  }
+// What a team (a warp or a block) knows about a row's teacher and label; a thread of a warp holds
+// four of the teacher's entries, one of a block one.
+template <int TEAM>
+struct RowTargets {
+  static constexpr int PER = TEAM >= kMaxTop ? 1 : kMaxTop / TEAM;
+  float x_at[PER];     // the student's logit at the entry's token
+  float log_q[PER], q[PER];
+  int index[PER];
+  float x_label;
+  int label;
+  float soft;          // 1: there is a teacher, 0: there is none, NaN: it is spoiled
+};
+
+template <int TEAM>
+__device__ float team_sum(float v, float* smem) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (TEAM == 32) return v;
   __syncthreads();
   if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
   __syncthreads();
   float r = smem[0];
-  for (int w = 1; w < WARPS; ++w) r = is_max ? fmaxf(r, smem[w]) : r + smem[w];
+  for (int w = 1; w < WARPS; ++w) r += smem[w];
   return r;
 }
-
-// Fills `t` for the row; with `want_loss` its loss too (`r` holds the row's statistics).
-__device__ void row_targets(const DistillArgs& a, uint64_t row, const float* x, const RowStats& r,
-                            bool want_loss, Targets& t, float* smem) {
-  const float inv_t = 1.f / a.temperature;
-  const bool here = threadIdx.x < a.top_n;
-  int index = -1;
-  float z = -INFINITY;
-  if (here && a.soft_weight > 0.f) {
-    index = a.teacher_tokens[row * a.top_n + threadIdx.x];
-    if (index >= 0 && uint64_t(index) >= a.vocab) {
-      report_index(a.status, INDEX_TEACHER, row, index);
-      index = -1;
-    }
-    if (index >= 0) z = a.teacher_logits[row * a.top_n + threadIdx.x] * inv_t;
-    if (z == -INFINITY) index = -1;
-  }
-  const float zm = block_reduce(index >= 0 ? z : -INFINITY, true, smem);
-  const float ze = index >= 0 ? exp2f((z - zm) * kLog2e) : 0.f;
-  const float total = block_reduce(ze, false, smem);
-  const bool soft = !(total == 0.f);  // NaN counts: it has to reach the outputs
-  const float q = soft ? ze / total : 0.f;
-  int label = -1;
-  if (a.soft_weight < 1.f) {
-    label = a.labels[row];
-    if (label >= 0 && uint64_t(label) >= a.vocab) {
-      if (threadIdx.x == 0) report_index(a.status, INDEX_LABEL, row, label);
-      label = -1;
-    }
-  }
-  if (here) {
-    t.index[threadIdx.x] = index;
-    t.take[threadIdx.x] = q;
-  }
-  if (threadIdx.x == 0) {
-    t.index[a.top_n] = label;
-    t.take[a.top_n] = 1.f;
-    // a NaN among the teacher's logits spoils the whole row, not only the tokens it names
-    t.soft = soft && a.soft_weight > 0.f ? (total == total ? 1.f : NAN) : 0.f;
-    t.hard = label >= 0 ? 1.f : 0.f;
-  }
-  if (want_loss) {
-    float kl = 0.f;
-    // q_k = 0 (an underflow) contributes 0 whatever the student says
-    if (index >= 0 && q != 0.f)
-      kl = q * (((z - zm) - logf(total)) - ((x[index] - r.m) * inv_t - logf(r.u)));
-    kl = block_reduce(kl, false, smem);
-    if (threadIdx.x == 0) {
-      const float w = a.soft_weight;
-      float loss = 0.f;
-      if (soft && w > 0.f) loss += w * a.temperature * a.temperature * kl;
-      if (label >= 0) loss += (1.f - w) * (logf(r.s) - (x[label] - r.m));
-      t.loss = r.s == 0.f ? 0.f : loss;  // a row that is masked as a whole has no distribution
-    }
-  }
+template <int TEAM>
+__device__ float team_max(float v, float* smem) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if (TEAM == 32) return v;
   __syncthreads();
+  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float r = smem[0];
+  for (int w = 1; w < WARPS; ++w) r = fmaxf(r, smem[w]);
+  return r;
+}
+template <int TEAM>
+__device__ __forceinline__ void team_sync() {
+  if (TEAM == 32) __syncwarp();
+  else __syncthreads();
 }
 
-// The gradient of one row; `x` and `grad` may be the same memory.
-__device__ void row_gradient(const DistillArgs& a, uint64_t row, const float* x, const RowStats& r,
-                             const Targets& t) {
-  float* g = a.grad + row * a.ld_grad;
-  if (r.s == 0.f) {
-    for (uint64_t i = threadIdx.x; i < a.vocab; i += THREADS) g[i] = 0.f;
-    return;
+// Reads the row's targets, the student's logits at them included: before anyone may overwrite the
+// row with its gradient.  `report`: one team of a row reports bad indices.
+template <int TEAM>
+__device__ RowTargets<TEAM> read_targets(const DistillArgs& a, uint64_t row, const float* x, bool report,
+                                         Targets& shared, float* smem) {
+  using R = RowTargets<TEAM>;
+  R t;
+  const uint32_t id = threadIdx.x % TEAM;
+  const float inv_t = 1.f / a.temperature;
+  float z[R::PER], zm = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < R::PER; ++i) {
+    const uint32_t k = uint32_t(i) * TEAM + id;
+    t.index[i] = -1;
+    t.x_at[i] = 0.f;
+    z[i] = -INFINITY;
+    if (k < a.top_n) {
+      const int index = a.teacher_tokens[row * a.top_n + k];
+      if (index >= 0 && uint64_t(index) >= a.vocab) {
+        if (report) report_index(a.status, INDEX_TEACHER, row, index);
+      } else if (index >= 0) {
+        z[i] = a.teacher_logits[row * a.top_n + k] * inv_t;
+        if (z[i] != -INFINITY) {
+          t.index[i] = index;
+          t.x_at[i] = x[index];
+        }
+      }
+    }
+    zm = fmaxf(zm, z[i]);
   }
+  zm = team_max<TEAM>(zm, smem);
+  float total = 0.f;
+#pragma unroll
+  for (int i = 0; i < R::PER; ++i) {
+    t.q[i] = t.index[i] >= 0 ? exp2f((z[i] - zm) * kLog2e) : 0.f;
+    total += t.q[i];
+  }
+  total = team_sum<TEAM>(total, smem);
+  // a NaN among the teacher's logits spoils the whole row, not only the tokens it names
+  t.soft = total == 0.f ? 0.f : total == total ? 1.f : NAN;
+  const float inv_total = total == 0.f ? 0.f : 1.f / total, log_total = logf(total);
+  t.label = -1;
+  t.x_label = 0.f;
+  if (a.labels) {
+    const int label = a.labels[row];
+    if (label >= 0 && uint64_t(label) >= a.vocab) {
+      if (report && id == 0) report_index(a.status, INDEX_LABEL, row, label);
+    } else if (label >= 0) {
+      t.label = label;
+      t.x_label = x[label];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R::PER; ++i) {
+    const uint32_t k = uint32_t(i) * TEAM + id;
+    t.q[i] *= inv_total;
+    t.log_q[i] = (z[i] - zm) - log_total;
+    if (k < a.top_n) {
+      shared.index[k] = t.index[i];
+      shared.take[k] = t.q[i];
+    }
+  }
+  if (id == 0) {
+    shared.index[a.top_n] = t.label;
+    shared.take[a.top_n] = 1.f;
+  }
+  team_sync<TEAM>();
+  return t;
+}
+
+// The row's loss, in every thread of the team.
+template <int TEAM>
+__device__ float row_loss(const DistillArgs& a, const RowStats& r, const RowTargets<TEAM>& t, float* smem) {
+  const float inv_t = 1.f / a.temperature, w = a.soft_weight;
+  float far = 0.f;
+  if (a.top_n) {
+    const float log_u = logf(r.u);
+#pragma unroll
+    for (int i = 0; i < RowTargets<TEAM>::PER; ++i)
+      // q_k = 0 (an underflow) contributes 0 whatever the student says
+      if (t.index[i] >= 0 && t.q[i] != 0.f) far += t.q[i] * (t.log_q[i] - ((t.x_at[i] - r.m) * inv_t - log_u));
+    far = team_sum<TEAM>(far, smem);
+  }
+  if (r.m == -INFINITY && r.s == 0.f && r.u == 0.f) return 0.f;  // masked as a whole: no distribution
+  float loss = 0.f;
+  if (!(t.soft == 0.f)) loss += w * a.temperature * a.temperature * far;
+  if (t.label >= 0) loss += (1.f - w) * (logf(r.s) - (t.x_label - r.m));
+  return loss;
+}
+
+// Factors of a row's gradient: dx = e^((x-m)/T) ks + e^(x-m) kh, minus soft q_k and hard at the
+// named places.
+struct GradFactors {
+  float m, ks, kh, soft, hard;
+  bool empty;
+};
+__device__ __forceinline__ GradFactors grad_factors(const DistillArgs& a, uint64_t row, const RowStats& r, float soft,
+                                                    int label) {
+  GradFactors f;
   const float scale = a.grad_loss ? a.grad_scale * a.grad_loss[row] : a.grad_scale;
-  const float soft = t.soft * scale * (a.soft_weight * a.temperature);
-  const float hard = t.hard * scale * (1.f - a.soft_weight);
-  const float ks = t.soft != 0.f ? soft / r.u : 0.f, kh = t.hard != 0.f ? hard / r.s : 0.f;
-  const float c = kLog2e / a.temperature;
-  for (uint64_t i = threadIdx.x; i < a.vocab; i += THREADS) {
-    const float d = x[i] - r.m;
-    g[i] = exp2f(d * c) * ks + exp2f(d * kLog2e) * kh;
-  }
-  __syncthreads();
-  // the places that the teacher and the label name: the first entry that names a place takes
-  // away what all of them do there, in their order
+  f.empty = r.m == -INFINITY && r.s == 0.f && r.u == 0.f;
+  f.m = r.m;
+  f.soft = soft * scale * (a.soft_weight * a.temperature);
+  f.hard = label >= 0 ? scale * (1.f - a.soft_weight) : 0.f;
+  f.ks = soft == 0.f || a.soft_weight == 0.f ? 0.f : f.soft / r.u;
+  f.kh = label < 0 ? 0.f : f.hard / r.s;
+  return f;
+}
+// How many exponentials an element of the gradient takes: with T = 1 both parts share one, and a
+// loss with one part has one.
+template <Sum SUM>
+__device__ __forceinline__ float grad_at(const GradFactors& f, float x, float c) {
+  const float d = x - f.m;
+  if (SUM == Sum::Tempered) return exp2f(d * c) * f.ks + exp2f(d * kLog2e) * f.kh;
+  return exp2f(d * c) * (f.ks + f.kh);
+}
+
+// The places that the teacher and the label name, among [first, end): the first entry that names
+// a place takes away what all of them do there, in their order.
+template <int TEAM>
+__device__ void take_targets(const DistillArgs& a, float* g, const Targets& t, const GradFactors& f, uint32_t first,
+                             uint32_t end) {
+  if (f.empty) return;
   const uint32_t n = a.top_n + 1;
-  for (uint32_t k = threadIdx.x; k < n; k += THREADS) {
+  for (uint32_t k = threadIdx.x % TEAM; k < n; k += TEAM) {
     const int index = t.index[k];
-    bool first = index >= 0;
-    for (uint32_t j = 0; j < k && first; ++j) first = t.index[j] != index;
-    if (!first) continue;
+    bool lead = index >= int(first) && uint32_t(index) < end;
+#pragma unroll 8
+    for (uint32_t j = 0; j < k; ++j) lead = lead && t.index[j] != index;
+    if (!lead) continue;
     float v = g[index];
-    for (uint32_t j = k; j < n; ++j)
-      if (t.index[j] == index) v -= t.take[j] * (j == a.top_n ? hard : soft);
+#pragma unroll 8
+    for (uint32_t j = k; j < n; ++j) v -= t.index[j] == index ? t.take[j] * (j == a.top_n ? f.hard : f.soft) : 0.f;
     g[index] = v;
   }
 }
 
-template <DistillPass PASS>
-__global__ void __launch_bounds__(THREADS) distill_kernel(const DistillArgs a) {
+__device__ __forceinline__ RowStats saved_stats(const DistillArgs& a, uint64_t row) {
+  RowStats r;
+  r.m = a.stats_in[row * 3];
+  r.u = a.stats_in[row * 3 + 1];
+  r.s = a.stats_in[row * 3 + 2];
+  return r;
+}
+// Plain sums one of the two; with T = 1 it is both.
+template <Sum SUM>
+__device__ __forceinline__ void complete(RowStats& r) {
+  if (SUM == Sum::Plain) r.u = r.s;
+}
+__device__ __forceinline__ void save_stats(const DistillArgs& a, uint64_t row, const RowStats& r) {
+  a.stats[row * 3] = r.m;
+  a.stats[row * 3 + 1] = r.u;
+  a.stats[row * 3 + 2] = r.s;
+}
+
+// Long rows.  The step keeps its part of the row in shared memory between the sums and the
+// gradient (`cached`; every thread reads back what it wrote itself); rows that do not fit are read
+// again, from L2 as far as they are still there.
+template <DistillPass PASS, Sum SUM>
+__global__ void __launch_bounds__(BLOCK, 3) distill_block_kernel(const DistillArgs a, uint32_t shares, bool cached) {
   ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
   ptx::grid_dependency_wait();
-  __shared__ RowStats smem[WARPS];
+  extern __shared__ float4 cache[];
+  __shared__ RowStats merged[WARPS], slot;
   __shared__ float red[WARPS];
   __shared__ Targets targets;
   const float c = kLog2e / a.temperature;
-  for (uint64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const float* x = a.x + row * a.ld;
-    RowStats r;
-    if (PASS == DistillPass::Backward) {
-      r.m = a.stats_in[row * 3];
-      r.u = a.stats_in[row * 3 + 1];
-      r.s = a.stats_in[row * 3 + 2];
-    } else {
-      r = row_stats<false>(x, a.vocab, c, smem);
+  const uint32_t rank = blockIdx.x % shares;
+  const uint64_t row = blockIdx.x / shares;
+  const float* x = a.x + row * a.ld;
+  const Part p = part_of(x, uint32_t(a.vocab), rank, shares);
+  const float extra = p.extra >= 0 ? x[p.extra] : -INFINITY;
+  RowStats r;
+  if (PASS == DistillPass::Backward) {
+    r = saved_stats(a, row);
+  } else {
+    add_one<SUM>(r, extra, c);
+    for (uint32_t q = p.q0; q < p.q1; q += QUADS * BLOCK) {
+      float4 v[QUADS];
+      load_quads(p, q, v);
+      add_quads<SUM>(r, v, c);
+      if (PASS == DistillPass::Step && cached) {
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; ++j) {
+          const uint32_t at = q + j * BLOCK + threadIdx.x;
+          if (at < p.q1) cache[at - p.q0] = v[j];
+        }
+      }
     }
-    row_targets(a, row, x, r, PASS != DistillPass::Backward, targets, red);
-    if (PASS != DistillPass::Backward && threadIdx.x == 0) a.loss[row] = targets.loss;
-    if (PASS == DistillPass::Forward && a.stats && threadIdx.x == 0) {
-      a.stats[row * 3] = r.m;
-      a.stats[row * 3 + 1] = r.u;
-      a.stats[row * 3 + 2] = r.s;
+    r = block_merge<SUM>(r, c, merged);
+  }
+  // the targets' logits are read before any block of the row writes its gradient
+  const bool first_block = rank == 0;
+  const RowTargets<BLOCK> t = read_targets<BLOCK>(a, row, x, first_block, targets, red);
+  if (PASS != DistillPass::Backward) {
+    if (shares > 1) r = cluster_merge<SUM>(r, c, &slot, shares);
+    complete<SUM>(r);
+    if (first_block) {
+      const float loss = row_loss<BLOCK>(a, r, t, red);
+      if (threadIdx.x == 0) {
+        a.loss[row] = loss;
+        if (PASS == DistillPass::Forward && a.stats) save_stats(a, row, r);
+      }
     }
-    if (PASS != DistillPass::Forward) row_gradient(a, row, x, r, targets);
+  }
+  if (PASS != DistillPass::Forward) {
+    const GradFactors f = grad_factors(a, row, r, t.soft, t.label);
+    float* g = a.grad + row * a.ld_grad;
+    if (p.extra >= 0) g[p.extra] = f.empty ? 0.f : grad_at<SUM>(f, extra, c);
+    // the same distance to a 16-byte boundary in both rows: 16-byte stores
+    const bool vec = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
+    float4* gq = reinterpret_cast<float4*>(g + p.lead);
+    for (uint32_t q = p.q0; q < p.q1; q += QUADS * BLOCK) {
+      float4 v[QUADS];
+      if (PASS == DistillPass::Step && cached) {
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; ++j) {
+          const uint32_t at = q + j * BLOCK + threadIdx.x;
+          if (at < p.q1) v[j] = cache[at - p.q0];
+        }
+      } else {
+        // plain loads: in place, the row is being written
+#pragma unroll
+        for (uint32_t j = 0; j < QUADS; ++j) {
+          const uint32_t at = q + j * BLOCK + threadIdx.x;
+          if (at < p.q1) v[j] = p.quads[at];
+        }
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < QUADS; ++j) {
+        const uint32_t at = q + j * BLOCK + threadIdx.x;
+        if (at >= p.q1) continue;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!f.empty)
+          o = make_float4(grad_at<SUM>(f, v[j].x, c), grad_at<SUM>(f, v[j].y, c), grad_at<SUM>(f, v[j].z, c),
+                          grad_at<SUM>(f, v[j].w, c));
+        if (vec) {
+          gq[at] = o;
+        } else {
+          float* out = g + p.lead + uint64_t(at) * 4;
+          out[0] = o.x;
+          out[1] = o.y;
+          out[2] = o.z;
+          out[3] = o.w;
+        }
+      }
+    }
     __syncthreads();
+    take_targets<BLOCK>(a, g, targets, f, p.first, p.end);
+  }
+  // no block leaves while another may still read its shared memory
+  if (PASS != DistillPass::Backward && shares > 1) ptx::cluster_sync_all();
+}
+
+// Short rows, one warp each.
+template <DistillPass PASS, Sum SUM, int PER>
+__global__ void __launch_bounds__(BLOCK) distill_warp_kernel(const DistillArgs a) {
+  ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
+  ptx::grid_dependency_wait();
+  __shared__ Targets targets[WARPS];
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, vocab = uint32_t(a.vocab);
+  const uint64_t row = uint64_t(blockIdx.x) * WARPS + warp;
+  if (row >= a.rows) return;
+  const float* x = a.x + row * a.ld;
+  const float c = kLog2e / a.temperature;
+  float v[PER];
+  load_row<PER>(x, vocab, lane, v);
+  RowStats r;
+  if (PASS == DistillPass::Backward) {
+    r = saved_stats(a, row);
+  } else {
+    r = stats_of<SUM, PER>(v, c);
+    complete<SUM>(r);
+  }
+  const RowTargets<32> t = read_targets<32>(a, row, x, true, targets[warp], nullptr);
+  if (PASS != DistillPass::Backward) {
+    const float loss = row_loss<32>(a, r, t, nullptr);
+    if (lane == 0) {
+      a.loss[row] = loss;
+      if (PASS == DistillPass::Forward && a.stats) save_stats(a, row, r);
+    }
+  }
+  if (PASS != DistillPass::Forward) {
+    const GradFactors f = grad_factors(a, row, r, t.soft, t.label);
+    float* g = a.grad + row * a.ld_grad;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const uint32_t i = uint32_t(j) * 32u + lane;
+      if (i < vocab) g[i] = f.empty ? 0.f : grad_at<SUM>(f, v[j], c);
+    }
+    __syncwarp();
+    take_targets<32>(a, g, targets[warp], f, 0, vocab);
   }
 }
 
-uint32_t row_grid(uint64_t rows, int sm_count) {
-  const uint64_t most = uint64_t(sm_count) * 8;
-  return uint32_t(rows < most ? rows : most);
+// ---- host side -----------------------------------------------------------------------------
+// Blocks per row: enough that few rows still fill the GPU twice over, each with at least 4096
+// logits.
+uint32_t shares_for(uint64_t rows, uint64_t vocab, int sm_count) {
+  uint32_t n = 1;
+  while (n < MAX_SHARE && rows * n * 2 <= uint64_t(sm_count) * 2 && vocab / (n * 2) >= 4096) n *= 2;
+  return n;
+}
+
+template <DistillPass PASS, Sum SUM>
+cudaError_t launch_distill_sum(const DistillArgs& a, int sm_count, cudaStream_t stream) {
+  if (a.vocab <= WARP_ROW) {
+    auto kern = a.vocab <= 32    ? distill_warp_kernel<PASS, SUM, 1>
+                : a.vocab <= 128 ? distill_warp_kernel<PASS, SUM, 4>
+                : a.vocab <= 512 ? distill_warp_kernel<PASS, SUM, 16>
+                                 : distill_warp_kernel<PASS, SUM, 32>;
+    return launch_kernel(kern, dim3(uint32_t((a.rows + WARPS - 1) / WARPS)), dim3(BLOCK), 0, stream, a);
+  }
+  uint32_t shares = shares_for(a.rows, a.vocab, sm_count);
+  size_t smem = 0;
+  constexpr auto kern = distill_block_kernel<PASS, SUM>;
+  if (PASS == DistillPass::Step) {
+    // parts of at most 64 KB (three blocks an SM) where 8 blocks allow that, of 220 KB where not
+    constexpr size_t GOOD = 64 << 10, MOST = 220 << 10;
+    auto bytes = [&](uint32_t n) { return (a.vocab / 4 / n + 1) * 16; };
+    while (shares < MAX_SHARE && bytes(shares) > GOOD) shares *= 2;
+    smem = bytes(shares) <= MOST ? bytes(shares) : 0;
+    static bool done[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (smem && !done[dev & 63]) {
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(MOST));
+      if (e != cudaSuccess) return e;
+      done[dev & 63] = true;
+    }
+  }
+  if (a.rows * shares > 0x7fffffffull) return cudaErrorInvalidValue;
+  return launch_kernel_cluster(kern, shares, dim3(uint32_t(a.rows * shares)), dim3(BLOCK), smem, stream, a, shares,
+                               smem != 0);
+}
+
+template <DistillPass PASS>
+cudaError_t launch_distill_pass(const DistillArgs& given, int sm_count, cudaStream_t stream) {
+  DistillArgs a = given;
+  const bool soft = a.soft_weight > 0.f, hard = a.soft_weight < 1.f;
+  // the saved statistics hold both sums
+  const bool both = (soft && hard) || (PASS == DistillPass::Forward && a.stats);
+  if (both && a.temperature != 1.f) return launch_distill_sum<PASS, Sum::Tempered>(a, sm_count, stream);
+  if (!soft && !both) a.temperature = 1.f;  // a loss of the labels alone has no temperature
+  return launch_distill_sum<PASS, Sum::Plain>(a, sm_count, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_token_logprobs(const LogprobArgs& a, int sm_count, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;
-  return launch_kernel(token_logprobs_kernel, dim3(row_grid(a.rows, sm_count)), dim3(THREADS), 0, stream, a);
+  if (a.vocab <= WARP_ROW) {
+    auto kern = a.vocab <= 32    ? logprobs_warp_kernel<1>
+                : a.vocab <= 128 ? logprobs_warp_kernel<4>
+                : a.vocab <= 512 ? logprobs_warp_kernel<16>
+                                 : logprobs_warp_kernel<32>;
+    return launch_kernel(kern, dim3(uint32_t((a.rows + WARPS - 1) / WARPS)), dim3(BLOCK), 0, stream, a);
+  }
+  const uint32_t shares = shares_for(a.rows, a.vocab, sm_count);
+  return launch_kernel_cluster(a.top_n ? logprobs_block_kernel<true> : logprobs_block_kernel<false>, shares,
+                               dim3(uint32_t(a.rows * shares)), dim3(BLOCK), 0, stream, a, shares);
 }
 
 cudaError_t launch_distill(DistillPass pass, const DistillArgs& a, int sm_count, cudaStream_t stream) {
   if (a.rows == 0) return cudaSuccess;
-  auto kern = pass == DistillPass::Forward    ? distill_kernel<DistillPass::Forward>
-              : pass == DistillPass::Backward ? distill_kernel<DistillPass::Backward>
-                                              : distill_kernel<DistillPass::Step>;
-  return launch_kernel(kern, dim3(row_grid(a.rows, sm_count)), dim3(THREADS), 0, stream, a);
+  switch (pass) {
+    case DistillPass::Forward: return launch_distill_pass<DistillPass::Forward>(a, sm_count, stream);
+    case DistillPass::Backward: return launch_distill_pass<DistillPass::Backward>(a, sm_count, stream);
+    default: return launch_distill_pass<DistillPass::Step>(a, sm_count, stream);
+  }
 }
 
 }  // namespace gonn

@@ -96,6 +96,7 @@ __device__ __forceinline__ void wait_out(volatile uint32_t* abort_flag) {
 // sums in its shared memory, and then adds up every `splits`-th column over all of them, in the
 // order of the shares.
 constexpr uint32_t SINGLE_THREADS = 192;
+constexpr uint32_t MAX_SPLITS = 8;  // the portable size of a cluster
 
 template <int BN, int STAGES>
 struct SingleShape {
@@ -260,16 +261,39 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
     __syncthreads();
     ptx::cluster_sync_all();  // the sums of every share are in place
     if (warp >= 2) {
-      const uint32_t r = (warp & 3u) * 32u + lane;
+      // A warp takes whole columns, four rows a lane.  All shares of a column are asked for
+      // before the first is added (a read of another CTA's shared memory takes a good 200 ns:
+      // one at a time, the 64 columns of a CTA cost 15 us), two columns in flight.
+      const uint32_t r = lane * 4;
       const uint64_t n = uint64_t(tn) * ROWS + r;
       const uint32_t m0 = tm * BN, cols = min(uint32_t(BN), p.M - m0);
-      const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
-#pragma unroll 1
-      for (uint32_t c = split; c < cols; c += p.splits) {
-        const uint32_t at = base + (c * ROWS + r) * 4;
-        float sum = 0.f;
-        for (uint32_t s = 0; s < p.splits; ++s) sum += ptx::ld_shared_cluster(ptx::mapa_shared(at, s));
-        if (n < p.N) p.c[(uint64_t(m0) + c) * p.N + n] = finish<CLASS>(p, sum, bias);
+      float bias[4] = {0.f, 0.f, 0.f, 0.f};
+      if (p.bias) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+          if (n + i < p.N) bias[i] = p.bias[n + i];
+      }
+      const uint32_t step = 4 * p.splits;
+#pragma unroll 2
+      for (uint32_t c = (warp & 3u) * p.splits + split; c < cols; c += step) {
+        float4 part[MAX_SPLITS];
+#pragma unroll
+        for (uint32_t s = 0; s < MAX_SPLITS; ++s)
+          if (s < p.splits) part[s] = ptx::ld_shared_cluster_16(ptx::mapa_shared(base + (c * ROWS + r) * 4, s));
+        float4 sum = part[0];
+#pragma unroll
+        for (uint32_t s = 1; s < MAX_SPLITS; ++s)
+          if (s < p.splits) {
+            sum.x += part[s].x;
+            sum.y += part[s].y;
+            sum.z += part[s].z;
+            sum.w += part[s].w;
+          }
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        float* out = p.c + (uint64_t(m0) + c) * p.N + n;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+          if (n + i < p.N) out[i] = finish<CLASS>(p, v[i], bias[i]);
       }
     }
     ptx::cluster_sync_all();  // no CTA leaves while another still reads its sums
@@ -579,7 +603,7 @@ const char* launch_class(const Mxfp4Product& q, GemmStatus* status, int sm_count
   p.tiles_m = uint32_t((q.M + bn - 1) / bn);
   p.num_tiles = p.tiles_n * p.tiles_m;
   // few tiles: share each one's K among the CTAs of a cluster
-  const uint32_t splits = std::min({std::max(1u, uint32_t(sm_count) / p.num_tiles), p.kblocks, 8u});
+  const uint32_t splits = std::min({std::max(1u, uint32_t(sm_count) / p.num_tiles), p.kblocks, MAX_SPLITS});
   p.kb_per_split = (p.kblocks + splits - 1) / splits;
   p.splits = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;
   return bn == 32   ? launch_single<32, 6, CLASS>(q, la, lb, p, stream)

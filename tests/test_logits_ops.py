@@ -235,7 +235,8 @@ def test_float64_gradient_is_the_derivative_of_the_loss():
 
 # ---------------------------------------------------------------------- GPU: log probabilities
 SIZES = [(1, 1), (1, 2), (3, 10), (5, 31), (4, 33), (7, 100), (2, 255), (2, 257), (300, 10), (3, 1000), (2, 1023),
-         (3, 4097), (2, 12345), (1, 50001), (5, 32768), (1, 150001), (160, 2049), (700, 515)]
+         (3, 4097), (2, 12345), (1, 50001), (5, 32768), (1, 150001), (160, 2049), (700, 515),
+         (40, 33000), (1, 600001)]
 
 
 @pytest.mark.gpu
@@ -367,7 +368,8 @@ def test_sizes_and_overlaps_are_refused(gpu):
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (3, 10, 4), (5, 31, 31), (4, 100, 7), (300, 10, 3), (3, 1000, 64),
                                             (2, 4097, 128), (2, 12345, 20), (1, 50001, 64), (3, 32768, 33),
-                                            (1, 150001, 16), (170, 515, 5)])
+                                            (1, 150001, 16), (170, 515, 5),
+                                            (40, 33000, 9), (1, 500003, 128)])
 @pytest.mark.parametrize("t,w", [(1.0, 1.0), (2.0, 0.5), (1.0, 0.25), (4.0, 0.0)])
 @pytest.mark.parametrize("kind", ["forward", "backward", "step"])
 def test_distillation(gpu, rows, vocab, top, t, w, kind):
