@@ -10,8 +10,9 @@
 // log p(t) = (x_t - m) - log S, and the entropy is log S - U / S.
 //
 // Short rows (up to 1024 logits) are held in the registers of one warp.  Longer ones are streamed
-// by a block of 256 threads, 32 logits a thread in flight; few long rows are shared by the up to 8
-// blocks of a cluster, which merge what they found through distributed shared memory.  All merges
+// by a block of 256 threads that loads the next 16 logits of a thread while it adds the last 16
+// (loading 32, then adding 32, reached half of the copy rate: the additions take as long as half
+// the loads); few long rows are shared by the up to 8 blocks of a cluster, which merge what they found through distributed shared memory.  All merges
 // have a fixed order: results repeat bit for bit.
 #include <algorithm>
 
@@ -26,7 +27,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int BLOCK = 256;
 constexpr int WARPS = BLOCK / 32;
-constexpr uint32_t QUADS = 8;                       // 16-byte loads a thread has in flight
+constexpr uint32_t QUADS = 4;                       // 16-byte loads of a thread in one half step
+constexpr uint32_t HALF = QUADS * BLOCK;            // pieces that a block takes in a half step
 constexpr uint32_t WARP_ROW = 1024;                 // longest row that one warp holds
 constexpr uint32_t MAX_SHARE = 8;                   // blocks of a cluster
 
@@ -96,33 +98,43 @@ __device__ __forceinline__ void merge(RowStats& a, RowStats b, float c) {
   a.u += b.u;
 }
 
-template <Sum SUM>
-__device__ __forceinline__ RowStats warp_merge(RowStats r, float c) {
+__device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    RowStats other;
-    other.m = __shfl_xor_sync(0xffffffffu, r.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, r.s, o);
-    other.u = __shfl_xor_sync(0xffffffffu, r.u, o);
-    // both sides add the lower lane's part first: every lane ends with the same bits
-    if (threadIdx.x & o) {
-      merge<SUM>(other, r, c);
-      r = other;
-    } else {
-      merge<SUM>(r, other, c);
-    }
-  }
-  return r;
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
 
+// The statistics of the block in every thread: the maximum first, then the sums relative to it, in
+// a fixed order.
 template <Sum SUM>
-__device__ RowStats block_merge(RowStats r, float c, RowStats* smem) {
-  r = warp_merge<SUM>(r, c);
+__device__ RowStats block_merge(RowStats r, float c, float (*smem)[WARPS]) {
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float mine = warp_max(r.m);
+  if (lane == 0) smem[0][warp] = mine;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = r;
+  float m = smem[0][0];
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) m = fmaxf(m, smem[0][w]);
+  rescale<SUM>(r, m, c);
+  const float s = warp_sum(r.s), u = SUM == Sum::Plain ? 0.f : warp_sum(r.u);
+  if (lane == 0) {
+    smem[1][warp] = s;
+    smem[2][warp] = u;
+  }
   __syncthreads();
-  r = smem[0];
-  for (int w = 1; w < WARPS; ++w) merge<SUM>(r, smem[w], c);
+  r.m = m;
+  r.s = smem[1][0];
+  r.u = smem[2][0];
+#pragma unroll
+  for (int w = 1; w < WARPS; ++w) {
+    r.s += smem[1][w];
+    r.u += smem[2][w];
+  }
   return r;
 }
 
@@ -182,39 +194,121 @@ __device__ __forceinline__ Part part_of(const float* x, uint32_t vocab, uint32_t
 
 __device__ __forceinline__ float4 masked_quad() { return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
 
+// A thread's 16 logits of the half step at piece `q`; -inf past the part's end.
 __device__ __forceinline__ void load_quads(const Part& p, uint32_t q, float4 (&v)[QUADS]) {
+  const float4* at = p.quads + q + threadIdx.x;
+  if (q + HALF <= p.q1) {
 #pragma unroll
-  for (uint32_t j = 0; j < QUADS; ++j) {
-    const uint32_t at = q + j * BLOCK + threadIdx.x;
-    v[j] = at < p.q1 ? p.quads[at] : masked_quad();
+    for (uint32_t j = 0; j < QUADS; ++j) v[j] = at[j * BLOCK];
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < QUADS; ++j)
+      v[j] = q + j * BLOCK + threadIdx.x < p.q1 ? at[j * BLOCK] : masked_quad();
   }
 }
 
 __device__ __forceinline__ float max4(const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
-
-// Adds a thread's 32 logits; returns their maximum.
-template <Sum SUM>
-__device__ __forceinline__ float add_quads(RowStats& r, const float4 (&v)[QUADS], float c) {
-  float most = max4(v[0]);
-#pragma unroll
-  for (uint32_t j = 1; j < QUADS; ++j) most = fmaxf(most, max4(v[j]));
-  if (most > r.m) rescale<SUM>(r, most, c);
-  const float ref = reference(r.m);
-#pragma unroll
-  for (uint32_t j = 0; j < QUADS; ++j) {
-    add<SUM>(r, v[j].x, ref, c);
-    add<SUM>(r, v[j].y, ref, c);
-    add<SUM>(r, v[j].z, ref, c);
-    add<SUM>(r, v[j].w, ref, c);
-  }
-  return most;
-}
 
 template <Sum SUM>
 __device__ __forceinline__ void add_one(RowStats& r, float x, float c) {
   if (x > r.m) rescale<SUM>(r, x, c);
   add<SUM>(r, x, reference(r.m), c);
 }
+
+// A thread's running statistics while it streams a row, two elements an instruction.  An exponent
+// is one fused multiply-add, x c - b with b = m c rounded (the same b for all elements, so its
+// rounding is a common factor, which result() takes out again); logits beyond 1e37, where the
+// products could overflow, take the difference first (`far`).
+template <Sum SUM>
+struct Stream {
+  float m = -INFINITY, b = 0.f, bt = 0.f;
+  float2 s = make_float2(0.f, 0.f), u = make_float2(0.f, 0.f);
+  bool far = false;
+
+  // scale of S itself; Plain: log2(e) / T
+  static __device__ __forceinline__ float scale(float c) { return SUM == Sum::Plain ? c : kLog2e; }
+
+  __device__ __forceinline__ void raise(float most, float c) {
+    const float k = scale(c), ref = reference(most);
+    const bool far_new = !(fabsf(ref) < 1e37f);
+    const float b_new = far_new ? 0.f : ref * k, bt_new = far_new ? 0.f : ref * c;
+    if (m != -INFINITY) {
+      const bool apart = far || far_new;
+      const float d = apart ? (m - most) * k : b - b_new, dt = apart ? (m - most) * c : bt - bt_new;
+      const float f = exp2f(d);
+      if (SUM == Sum::Entropy) {
+        const float by = fmaxf(d, -1e4f);  // where f is 0 the limit keeps the product finite
+        u.x = f * (u.x + by * s.x);
+        u.y = f * (u.y + by * s.y);
+      }
+      if (SUM == Sum::Tempered) {
+        const float ft = exp2f(dt);
+        u.x *= ft;
+        u.y *= ft;
+      }
+      s.x *= f;
+      s.y *= f;
+    }
+    m = most;
+    b = b_new;
+    bt = bt_new;
+    far = far_new;
+  }
+
+  __device__ __forceinline__ void add_pair(float x, float y, float c) {
+    const float k = scale(c);
+    float2 t;
+    if (far) t = make_float2((x - m) * k, (y - m) * k);
+    else t = ptx::fma2(make_float2(x, y), make_float2(k, k), make_float2(-b, -b));
+    const float2 e = make_float2(exp2_ftz(t.x), exp2_ftz(t.y));
+    s = ptx::add2(s, e);
+    // a masked element (-inf) adds e = 0 times a finite number
+    if (SUM == Sum::Entropy) u = ptx::fma2(e, make_float2(fmaxf(t.x, -1e30f), fmaxf(t.y, -1e30f)), u);
+    if (SUM == Sum::Tempered) {
+      float2 w;
+      if (far) w = make_float2((x - m) * c, (y - m) * c);
+      else w = ptx::fma2(make_float2(x, y), make_float2(c, c), make_float2(-bt, -bt));
+      u = ptx::add2(u, make_float2(exp2_ftz(w.x), exp2_ftz(w.y)));
+    }
+  }
+
+  // Adds 16 logits; returns their maximum.
+  __device__ __forceinline__ float add(const float4 (&v)[QUADS], float c) {
+    float most = max4(v[0]);
+#pragma unroll
+    for (uint32_t j = 1; j < QUADS; ++j) most = fmaxf(most, max4(v[j]));
+    if (most > m) raise(most, c);
+    if (!far) {
+#pragma unroll
+      for (uint32_t j = 0; j < QUADS; ++j) {
+        add_pair(v[j].x, v[j].y, c);
+        add_pair(v[j].z, v[j].w, c);
+      }
+    } else {
+#pragma unroll 1
+      for (uint32_t j = 0; j < QUADS; ++j) {
+        const float4 f = j == 0 ? v[0] : j == 1 ? v[1] : j == 2 ? v[2] : v[3];
+        add_pair(f.x, f.y, c);
+        add_pair(f.z, f.w, c);
+      }
+    }
+    return most;
+  }
+
+  __device__ __forceinline__ RowStats result(float c) const {
+    RowStats r;
+    r.m = m;
+    const float ref = reference(m);
+    // m c - b, exactly
+    const float off = far ? 0.f : fmaf(ref, scale(c), -b), off_t = far ? 0.f : fmaf(ref, c, -bt);
+    const float f = exp2f(-off);
+    r.s = (s.x + s.y) * f;
+    if (SUM == Sum::Entropy) r.u = ((u.x + u.y) - off * (s.x + s.y)) * f * 0.6931471805599453f;
+    if (SUM == Sum::Tempered) r.u = (u.x + u.y) * exp2f(-off_t);
+    return r;
+  }
+};
+static_assert(QUADS == 4, "Stream::add picks one of four");
 
 // ---- alternatives -------------------------------------------------------------------------
 // Orders like (value, lowest index first): larger keys come first among the alternatives.
@@ -235,11 +329,11 @@ constexpr uint32_t kMaskedBits = 0x007fffffu;  // order_bits(-inf); below it onl
 
 // The largest `want` keys a block has met.  A key is kept when it lies above a floor that is known
 // to have `want` keys above it.  The first floor comes from the threads' maxima of their first 32
-// logits (as many of those as wanted lie above it, so as many logits do), which leaves about
-// want * n / 8192 keys of n; when the buffer runs over the limit, the keys below the exact
-// want-th one are thrown out and it becomes the floor.
+// logits (as many of those as wanted lie above it, so as many logits do); when more than about
+// twice the wanted keys are kept, the surplus is thrown out and the floor rises to the exact
+// want-th key, which in ordinary rows happens each time the logits seen have doubled.
 struct Selection {
-  static constexpr uint32_t CAP = 2048, LIMIT = 1024;
+  static constexpr uint32_t CAP = 2048;
   uint64_t key[CAP];
   uint64_t sorted[kMaxTop];
   uint64_t floor;
@@ -274,9 +368,13 @@ __device__ void keep_largest(Selection& s, uint32_t n, uint32_t want) {
   for (int bit = 63; bit >= 0; --bit) {
     const uint64_t trial = floor | (1ull << bit);
     uint32_t above = 0;
+    if (n <= BLOCK) {
+      above = uint32_t(__syncthreads_count(mine[0] >= trial));
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < PER; ++i) above += mine[i] >= trial;
-    above = block_count(s, above, turn);
+      for (uint32_t i = 0; i < PER; ++i) above += mine[i] >= trial;
+      above = block_count(s, above, turn);
+    }
     if (above >= want) floor = trial;
     if (above == want) break;
   }
@@ -308,23 +406,28 @@ __device__ void first_floor(Selection& s, float most, uint32_t want) {
   __syncthreads();
 }
 
-// Offers a thread's logits (8 quads of the row from `q`, of which `most` is the maximum, and the
-// logit outside the quads) to the selection.  All threads of the block call it.
-__device__ __forceinline__ void offer(Selection& s, const float* x, const Part& p, uint32_t q,
-                                      const float4 (&v)[QUADS], float most, float extra, uint32_t want) {
-  uint64_t floor = s.floor;
-  // a floor below the order of -inf lets everything pass
-  float low = uint32_t(floor >> 32) <= kMaskedBits ? -INFINITY : key_value(floor);
-  uint32_t hits = 0;       // logits that may lie above the floor, a bit each
-  bool outside = p.extra >= 0 && extra >= low;
-  if (most >= low) {
+// The floor's value as a bound on logits; one below the order of -inf lets everything pass.
+__device__ __forceinline__ float floor_value(uint64_t floor) {
+  return uint32_t(floor >> 32) <= kMaskedBits ? -INFINITY : key_value(floor);
+}
+// Which of a thread's 16 logits from piece `q` may lie above the floor, a bit each.
+__device__ __forceinline__ uint32_t above_floor(const Part& p, uint32_t q, const float4 (&v)[QUADS], float low) {
+  uint32_t hits = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < QUADS; ++j) {
-      const uint32_t four = uint32_t(v[j].x >= low) | uint32_t(v[j].y >= low) << 1 | uint32_t(v[j].z >= low) << 2 |
-                            uint32_t(v[j].w >= low) << 3;
-      if (q + j * BLOCK + threadIdx.x < p.q1) hits |= four << (4 * j);
-    }
+  for (uint32_t j = 0; j < QUADS; ++j) {
+    const uint32_t four = uint32_t(v[j].x >= low) | uint32_t(v[j].y >= low) << 1 | uint32_t(v[j].z >= low) << 2 |
+                          uint32_t(v[j].w >= low) << 3;
+    if (q + j * BLOCK + threadIdx.x < p.q1) hits |= four << (4 * j);
   }
+  return hits;
+}
+
+// Offers a thread's logits of a whole step (two halves from piece `q`, the marked ones) and, with
+// `outside`, its logit outside the pieces to the selection.  All threads of the block call it.
+__device__ __forceinline__ void offer(Selection& s, const float* x, const Part& p, uint32_t q, uint32_t hits,
+                                      bool outside, uint32_t want) {
+  uint64_t floor = s.floor;
+  const uint32_t limit = 2 * want + 64;
   while (true) {
     bool over = false;
     uint32_t left = hits;
@@ -344,7 +447,7 @@ __device__ __forceinline__ void offer(Selection& s, const float* x, const Part& 
       bool stored = true;
       if (key >= floor) {
         const uint32_t at = atomicAdd(&s.count, 1u);
-        over = over || at >= Selection::LIMIT;
+        over = over || at >= limit;
         stored = at < Selection::CAP;
         if (stored) s.key[at] = key;
       }
@@ -366,7 +469,7 @@ __device__ __forceinline__ void offer(Selection& s, const float* x, const Part& 
 __device__ uint32_t sort_selection(Selection& s, uint32_t want) {
   __syncthreads();
   uint32_t n = s.count;
-  if (n > 512 && n > want) {
+  if (n > 2 * kMaxTop + 64) {  // the alternatives of several blocks
     keep_largest(s, n, want);
     n = want;
   }
@@ -401,27 +504,45 @@ template <bool TOP>
 __global__ void __launch_bounds__(BLOCK, 4) logprobs_block_kernel(const LogprobArgs a, uint32_t shares) {
   ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
   ptx::grid_dependency_wait();
-  __shared__ RowStats merged[WARPS], slot;
+  __shared__ float merged[3][WARPS];
+  __shared__ RowStats slot;
   __shared__ Selection sel;
   const uint32_t rank = blockIdx.x % shares;
   const uint64_t row = blockIdx.x / shares;
   const float* x = a.x + row * a.ld;
   const Part p = part_of(x, uint32_t(a.vocab), rank, shares);
-  RowStats r;
   const float extra = p.extra >= 0 ? x[p.extra] : -INFINITY;
-  add_one<Sum::Entropy>(r, extra, 0.f);
-  for (uint32_t q = p.q0; q < p.q1 || q == p.q0; q += QUADS * BLOCK) {
-    float4 v[QUADS];
-    load_quads(p, q, v);
-    const float most = add_quads<Sum::Entropy>(r, v, 0.f);
+  Stream<Sum::Entropy> stream;
+  float4 v[QUADS], next[QUADS];
+  load_quads(p, p.q0, v);
+  for (uint32_t q = p.q0; q < p.q1 || q == p.q0; q += 2 * HALF) {
+    const bool first = q == p.q0;
+    const float low = TOP && !first ? floor_value(sel.floor) : INFINITY;
+    uint32_t hits = 0;
+    load_quads(p, q + HALF, next);
+    const float most = stream.add(v, kLog2e);
+    if (TOP && most >= low) hits = above_floor(p, q, v, low);
+    load_quads(p, q + 2 * HALF, v);
+    const float most2 = stream.add(next, kLog2e);
+    if (TOP && most2 >= low) hits |= above_floor(p, q + HALF, next, low) << 16;
     if (TOP) {
-      const bool first = q == p.q0;
-      if (first) first_floor(sel, fmaxf(most, extra), a.top_n);
-      Part mine = p;
-      if (!first) mine.extra = -1;
-      offer(sel, x, mine, q, v, most, extra, a.top_n);
+      bool outside = false;
+      if (first) {
+        const float all = fmaxf(fmaxf(most, most2), extra);
+        first_floor(sel, all, a.top_n);
+        const float start = floor_value(sel.floor);
+        if (all >= start) {  // the first half comes from L1 once more
+          outside = p.extra >= 0 && extra >= start;
+          hits = above_floor(p, q + HALF, next, start) << 16;
+          load_quads(p, q, next);
+          hits |= above_floor(p, q, next, start);
+        }
+      }
+      offer(sel, x, p, q, hits, outside, a.top_n);
     }
   }
+  RowStats r = stream.result(kLog2e);
+  add_one<Sum::Entropy>(r, extra, 0.f);
   r = block_merge<Sum::Entropy>(r, 0.f, merged);
   uint32_t found = 0;
   if (TOP) found = sort_selection(sel, a.top_n);
@@ -542,169 +663,148 @@ __global__ void __launch_bounds__(BLOCK) logprobs_warp_kernel(const LogprobArgs 
 //   dx_j = g (w T (p_T[j] - sum_{k: idx_k = j} q_k) + (1-w) (p[j] - [j = label]))
 // The statistics keep S_1 = sum e^(x-m) in `s` and S_T = sum e^((x-m)/T) in `u`; where only one of
 // them is wanted, or T is 1, only that one is summed.
+// One warp takes care of a row's teacher and label, before the row is streamed: what it finds waits
+// in shared memory.
 struct Targets {
   int index[kMaxTop + 1];   // teacher tokens, then the label; -1: not there
   float take[kMaxTop + 1];  // q_k, then 1 for the label
+  float x_at[kMaxTop + 1];  // the student's logit there
+  float log_q[kMaxTop];
+  float soft;               // 1: there is a teacher, 0: there is none, NaN: it is spoiled
 };
-
-// What a team (a warp or a block) knows about a row's teacher and label; a thread of a warp holds
-// four of the teacher's entries, one of a block one.
-template <int TEAM>
-struct RowTargets {
-  static constexpr int PER = TEAM >= kMaxTop ? 1 : kMaxTop / TEAM;
-  float x_at[PER];     // the student's logit at the entry's token
-  float log_q[PER], q[PER];
-  int index[PER];
-  float x_label;
-  int label;
-  float soft;          // 1: there is a teacher, 0: there is none, NaN: it is spoiled
-};
-
-template <int TEAM>
-__device__ float team_sum(float v, float* smem) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (TEAM == 32) return v;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float r = smem[0];
-  for (int w = 1; w < WARPS; ++w) r += smem[w];
-  return r;
-}
-template <int TEAM>
-__device__ float team_max(float v, float* smem) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if (TEAM == 32) return v;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) smem[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float r = smem[0];
-  for (int w = 1; w < WARPS; ++w) r = fmaxf(r, smem[w]);
-  return r;
-}
-template <int TEAM>
-__device__ __forceinline__ void team_sync() {
-  if (TEAM == 32) __syncwarp();
-  else __syncthreads();
-}
 
 // Reads the row's targets, the student's logits at them included: before anyone may overwrite the
-// row with its gradient.  `report`: one team of a row reports bad indices.
-template <int TEAM>
-__device__ RowTargets<TEAM> read_targets(const DistillArgs& a, uint64_t row, const float* x, bool report,
-                                         Targets& shared, float* smem) {
-  using R = RowTargets<TEAM>;
-  R t;
-  const uint32_t id = threadIdx.x % TEAM;
+// row with its gradient.  Called by one warp; `report`: one warp of a row reports bad indices.
+__device__ void read_targets(const DistillArgs& a, uint64_t row, const float* x, bool report, Targets& t) {
+  constexpr int PER = kMaxTop / 32;
+  const uint32_t lane = threadIdx.x & 31;
   const float inv_t = 1.f / a.temperature;
-  float z[R::PER], zm = -INFINITY;
+  int index[PER];
+  float z[PER], x_at[PER], zm = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < R::PER; ++i) {
-    const uint32_t k = uint32_t(i) * TEAM + id;
-    t.index[i] = -1;
-    t.x_at[i] = 0.f;
+  for (int i = 0; i < PER; ++i) {
+    const uint32_t k = uint32_t(i) * 32u + lane;
+    index[i] = -1;
+    x_at[i] = 0.f;
     z[i] = -INFINITY;
     if (k < a.top_n) {
-      const int index = a.teacher_tokens[row * a.top_n + k];
-      if (index >= 0 && uint64_t(index) >= a.vocab) {
-        if (report) report_index(a.status, INDEX_TEACHER, row, index);
-      } else if (index >= 0) {
-        z[i] = a.teacher_logits[row * a.top_n + k] * inv_t;
-        if (z[i] != -INFINITY) {
-          t.index[i] = index;
-          t.x_at[i] = x[index];
-        }
-      }
+      index[i] = a.teacher_tokens[row * a.top_n + k];
+      z[i] = a.teacher_logits[row * a.top_n + k] * inv_t;
     }
+  }
+  int label = lane == 0 && a.labels ? a.labels[row] : -1;
+  if (label >= 0 && uint64_t(label) >= a.vocab) {
+    if (report) report_index(a.status, INDEX_LABEL, row, label);
+    label = -1;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (index[i] >= 0 && uint64_t(index[i]) >= a.vocab) {
+      if (report) report_index(a.status, INDEX_TEACHER, row, index[i]);
+      index[i] = -1;
+    }
+    if (z[i] == -INFINITY) index[i] = -1;
+    if (index[i] >= 0) x_at[i] = x[index[i]];
+    else z[i] = -INFINITY;
     zm = fmaxf(zm, z[i]);
   }
-  zm = team_max<TEAM>(zm, smem);
-  float total = 0.f;
+  const float x_label = label >= 0 ? x[label] : 0.f;
+  zm = warp_max(zm);
+  float q[PER], total = 0.f;
 #pragma unroll
-  for (int i = 0; i < R::PER; ++i) {
-    t.q[i] = t.index[i] >= 0 ? exp2f((z[i] - zm) * kLog2e) : 0.f;
-    total += t.q[i];
+  for (int i = 0; i < PER; ++i) {
+    q[i] = index[i] >= 0 ? exp2f((z[i] - zm) * kLog2e) : 0.f;
+    total += q[i];
   }
-  total = team_sum<TEAM>(total, smem);
-  // a NaN among the teacher's logits spoils the whole row, not only the tokens it names
-  t.soft = total == 0.f ? 0.f : total == total ? 1.f : NAN;
+  total = warp_sum(total);
   const float inv_total = total == 0.f ? 0.f : 1.f / total, log_total = logf(total);
-  t.label = -1;
-  t.x_label = 0.f;
-  if (a.labels) {
-    const int label = a.labels[row];
-    if (label >= 0 && uint64_t(label) >= a.vocab) {
-      if (report && id == 0) report_index(a.status, INDEX_LABEL, row, label);
-    } else if (label >= 0) {
-      t.label = label;
-      t.x_label = x[label];
-    }
-  }
 #pragma unroll
-  for (int i = 0; i < R::PER; ++i) {
-    const uint32_t k = uint32_t(i) * TEAM + id;
-    t.q[i] *= inv_total;
-    t.log_q[i] = (z[i] - zm) - log_total;
+  for (int i = 0; i < PER; ++i) {
+    const uint32_t k = uint32_t(i) * 32u + lane;
     if (k < a.top_n) {
-      shared.index[k] = t.index[i];
-      shared.take[k] = t.q[i];
+      t.index[k] = index[i];
+      t.take[k] = q[i] * inv_total;
+      t.x_at[k] = x_at[i];
+      t.log_q[k] = (z[i] - zm) - log_total;
     }
   }
-  if (id == 0) {
-    shared.index[a.top_n] = t.label;
-    shared.take[a.top_n] = 1.f;
+  if (lane == 0) {
+    t.index[a.top_n] = label;
+    t.take[a.top_n] = 1.f;
+    t.x_at[a.top_n] = x_label;
+    // a NaN among the teacher's logits spoils the whole row, not only the tokens it names
+    t.soft = total == 0.f ? 0.f : total == total ? 1.f : NAN;
   }
-  team_sync<TEAM>();
-  return t;
+  __syncwarp();
 }
 
-// The row's loss, in every thread of the team.
-template <int TEAM>
-__device__ float row_loss(const DistillArgs& a, const RowStats& r, const RowTargets<TEAM>& t, float* smem) {
+// The row's loss, in every lane of the warp that read the targets.
+__device__ float row_loss(const DistillArgs& a, const RowStats& r, const Targets& t) {
   const float inv_t = 1.f / a.temperature, w = a.soft_weight;
   float far = 0.f;
   if (a.top_n) {
     const float log_u = logf(r.u);
-#pragma unroll
-    for (int i = 0; i < RowTargets<TEAM>::PER; ++i)
+    for (uint32_t k = threadIdx.x & 31; k < a.top_n; k += 32)
       // q_k = 0 (an underflow) contributes 0 whatever the student says
-      if (t.index[i] >= 0 && t.q[i] != 0.f) far += t.q[i] * (t.log_q[i] - ((t.x_at[i] - r.m) * inv_t - log_u));
-    far = team_sum<TEAM>(far, smem);
+      if (t.index[k] >= 0 && t.take[k] != 0.f)
+        far += t.take[k] * (t.log_q[k] - ((t.x_at[k] - r.m) * inv_t - log_u));
+    far = warp_sum(far);
   }
   if (r.m == -INFINITY && r.s == 0.f && r.u == 0.f) return 0.f;  // masked as a whole: no distribution
   float loss = 0.f;
   if (!(t.soft == 0.f)) loss += w * a.temperature * a.temperature * far;
-  if (t.label >= 0) loss += (1.f - w) * (logf(r.s) - (t.x_label - r.m));
+  if (t.index[a.top_n] >= 0) loss += (1.f - w) * (logf(r.s) - (t.x_at[a.top_n] - r.m));
   return loss;
 }
 
 // Factors of a row's gradient: dx = e^((x-m)/T) ks + e^(x-m) kh, minus soft q_k and hard at the
-// named places.
+// named places.  Exponents as in Stream; what the rounding of b adds is taken out of ks and kh.
+// With T = 1 both parts share an exponential, and a loss with one part has one (Plain).
 struct GradFactors {
-  float m, ks, kh, soft, hard;
-  bool empty;
+  float m, b, bt, ks, kh, soft, hard;
+  bool empty, far;
 };
+template <Sum SUM>
 __device__ __forceinline__ GradFactors grad_factors(const DistillArgs& a, uint64_t row, const RowStats& r, float soft,
-                                                    int label) {
+                                                    int label, float c) {
   GradFactors f;
   const float scale = a.grad_loss ? a.grad_scale * a.grad_loss[row] : a.grad_scale;
   f.empty = r.m == -INFINITY && r.s == 0.f && r.u == 0.f;
-  f.m = r.m;
+  f.m = reference(r.m);
+  f.far = !(fabsf(f.m) < 1e37f);
+  f.b = f.far ? 0.f : f.m * kLog2e;
+  f.bt = f.far ? 0.f : f.m * c;
+  const float off = f.far ? 0.f : fmaf(f.m, kLog2e, -f.b), off_t = f.far ? 0.f : fmaf(f.m, c, -f.bt);
   f.soft = soft * scale * (a.soft_weight * a.temperature);
   f.hard = label >= 0 ? scale * (1.f - a.soft_weight) : 0.f;
-  f.ks = soft == 0.f || a.soft_weight == 0.f ? 0.f : f.soft / r.u;
-  f.kh = label < 0 ? 0.f : f.hard / r.s;
+  f.ks = soft == 0.f || a.soft_weight == 0.f ? 0.f : f.soft / r.u * exp2f(-off_t);
+  f.kh = label < 0 ? 0.f : f.hard / r.s * exp2f(-(SUM == Sum::Tempered ? off : off_t));
+  if (SUM == Sum::Plain) f.ks += f.kh;
   return f;
 }
-// How many exponentials an element of the gradient takes: with T = 1 both parts share one, and a
-// loss with one part has one.
+// A probability below 2^-126 gives 0.
+template <Sum SUM>
+__device__ __forceinline__ float2 grad_pair(const GradFactors& f, float x, float y, float c) {
+  float2 t;
+  if (f.far) t = make_float2((x - f.m) * c, (y - f.m) * c);
+  else t = ptx::fma2(make_float2(x, y), make_float2(c, c), make_float2(-f.bt, -f.bt));
+  float2 g = make_float2(exp2_ftz(t.x) * f.ks, exp2_ftz(t.y) * f.ks);
+  if (SUM == Sum::Tempered) {
+    if (f.far) t = make_float2((x - f.m) * kLog2e, (y - f.m) * kLog2e);
+    else t = ptx::fma2(make_float2(x, y), make_float2(kLog2e, kLog2e), make_float2(-f.b, -f.b));
+    g = ptx::fma2(make_float2(exp2_ftz(t.x), exp2_ftz(t.y)), make_float2(f.kh, f.kh), g);
+  }
+  return g;
+}
 template <Sum SUM>
 __device__ __forceinline__ float grad_at(const GradFactors& f, float x, float c) {
-  const float d = x - f.m;
-  if (SUM == Sum::Tempered) return exp2f(d * c) * f.ks + exp2f(d * kLog2e) * f.kh;
-  return exp2f(d * c) * (f.ks + f.kh);
+  return f.empty ? 0.f : grad_pair<SUM>(f, x, x, c).x;
+}
+template <Sum SUM>
+__device__ __forceinline__ float4 grad_quad(const GradFactors& f, const float4& v, float c) {
+  if (f.empty) return make_float4(0.f, 0.f, 0.f, 0.f);
+  const float2 a = grad_pair<SUM>(f, v.x, v.y, c), b = grad_pair<SUM>(f, v.z, v.w, c);
+  return make_float4(a.x, a.y, b.x, b.y);
 }
 
 // The places that the teacher and the label name, among [first, end): the first entry that names
@@ -749,46 +849,53 @@ __device__ __forceinline__ void save_stats(const DistillArgs& a, uint64_t row, c
 // gradient (`cached`; every thread reads back what it wrote itself); rows that do not fit are read
 // again, from L2 as far as they are still there.
 template <DistillPass PASS, Sum SUM>
-__global__ void __launch_bounds__(BLOCK, 3) distill_block_kernel(const DistillArgs a, uint32_t shares, bool cached) {
+__global__ void __launch_bounds__(BLOCK, 4) distill_block_kernel(const DistillArgs a, uint32_t shares, bool cached) {
   ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
   ptx::grid_dependency_wait();
   extern __shared__ float4 cache[];
-  __shared__ RowStats merged[WARPS], slot;
-  __shared__ float red[WARPS];
+  __shared__ float merged[3][WARPS];
+  __shared__ RowStats slot;
   __shared__ Targets targets;
   const float c = kLog2e / a.temperature;
   const uint32_t rank = blockIdx.x % shares;
   const uint64_t row = blockIdx.x / shares;
   const float* x = a.x + row * a.ld;
   const Part p = part_of(x, uint32_t(a.vocab), rank, shares);
+  // the targets' logits are read before any block of the row writes its gradient
+  if (threadIdx.x < 32 && (PASS != DistillPass::Forward || rank == 0)) read_targets(a, row, x, rank == 0, targets);
   const float extra = p.extra >= 0 ? x[p.extra] : -INFINITY;
   RowStats r;
   if (PASS == DistillPass::Backward) {
     r = saved_stats(a, row);
   } else {
-    add_one<SUM>(r, extra, c);
-    for (uint32_t q = p.q0; q < p.q1; q += QUADS * BLOCK) {
-      float4 v[QUADS];
-      load_quads(p, q, v);
-      add_quads<SUM>(r, v, c);
-      if (PASS == DistillPass::Step && cached) {
+    Stream<SUM> stream;
+    float4 v[QUADS], next[QUADS];
+    auto keep = [&](uint32_t q, const float4 (&w)[QUADS]) {
+      if (PASS != DistillPass::Step || !cached) return;
 #pragma unroll
-        for (uint32_t j = 0; j < QUADS; ++j) {
-          const uint32_t at = q + j * BLOCK + threadIdx.x;
-          if (at < p.q1) cache[at - p.q0] = v[j];
-        }
+      for (uint32_t j = 0; j < QUADS; ++j) {
+        const uint32_t at = q + j * BLOCK + threadIdx.x;
+        if (at < p.q1) cache[at - p.q0] = w[j];
       }
+    };
+    load_quads(p, p.q0, v);
+    for (uint32_t q = p.q0; q < p.q1; q += 2 * HALF) {
+      load_quads(p, q + HALF, next);
+      stream.add(v, c);
+      keep(q, v);
+      load_quads(p, q + 2 * HALF, v);
+      stream.add(next, c);
+      keep(q + HALF, next);
     }
+    r = stream.result(c);
+    add_one<SUM>(r, extra, c);
     r = block_merge<SUM>(r, c, merged);
   }
-  // the targets' logits are read before any block of the row writes its gradient
-  const bool first_block = rank == 0;
-  const RowTargets<BLOCK> t = read_targets<BLOCK>(a, row, x, first_block, targets, red);
   if (PASS != DistillPass::Backward) {
     if (shares > 1) r = cluster_merge<SUM>(r, c, &slot, shares);
     complete<SUM>(r);
-    if (first_block) {
-      const float loss = row_loss<BLOCK>(a, r, t, red);
+    if (rank == 0 && threadIdx.x < 32) {
+      const float loss = row_loss(a, r, targets);
       if (threadIdx.x == 0) {
         a.loss[row] = loss;
         if (PASS == DistillPass::Forward && a.stats) save_stats(a, row, r);
@@ -796,14 +903,15 @@ __global__ void __launch_bounds__(BLOCK, 3) distill_block_kernel(const DistillAr
     }
   }
   if (PASS != DistillPass::Forward) {
-    const GradFactors f = grad_factors(a, row, r, t.soft, t.label);
+    // Backward: the targets have to be there; in the step the merge's barriers came after them
+    if (PASS == DistillPass::Backward) __syncthreads();
+    const GradFactors f = grad_factors<SUM>(a, row, r, targets.soft, targets.index[a.top_n], c);
     float* g = a.grad + row * a.ld_grad;
-    if (p.extra >= 0) g[p.extra] = f.empty ? 0.f : grad_at<SUM>(f, extra, c);
+    if (p.extra >= 0) g[p.extra] = grad_at<SUM>(f, extra, c);
     // the same distance to a 16-byte boundary in both rows: 16-byte stores
     const bool vec = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
     float4* gq = reinterpret_cast<float4*>(g + p.lead);
-    for (uint32_t q = p.q0; q < p.q1; q += QUADS * BLOCK) {
-      float4 v[QUADS];
+    auto read = [&](uint32_t q, float4 (&v)[QUADS]) {
       if (PASS == DistillPass::Step && cached) {
 #pragma unroll
         for (uint32_t j = 0; j < QUADS; ++j) {
@@ -811,21 +919,20 @@ __global__ void __launch_bounds__(BLOCK, 3) distill_block_kernel(const DistillAr
           if (at < p.q1) v[j] = cache[at - p.q0];
         }
       } else {
-        // plain loads: in place, the row is being written
+        load_quads(p, q, v);
+      }
+    };
+    auto write = [&](uint32_t q, const float4 (&v)[QUADS]) {
+      if (vec && q + HALF <= p.q1) {
 #pragma unroll
-        for (uint32_t j = 0; j < QUADS; ++j) {
-          const uint32_t at = q + j * BLOCK + threadIdx.x;
-          if (at < p.q1) v[j] = p.quads[at];
-        }
+        for (uint32_t j = 0; j < QUADS; ++j) __stcs(gq + q + threadIdx.x + j * BLOCK, grad_quad<SUM>(f, v[j], c));
+        return;
       }
 #pragma unroll
       for (uint32_t j = 0; j < QUADS; ++j) {
         const uint32_t at = q + j * BLOCK + threadIdx.x;
         if (at >= p.q1) continue;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (!f.empty)
-          o = make_float4(grad_at<SUM>(f, v[j].x, c), grad_at<SUM>(f, v[j].y, c), grad_at<SUM>(f, v[j].z, c),
-                          grad_at<SUM>(f, v[j].w, c));
+        const float4 o = grad_quad<SUM>(f, v[j], c);
         if (vec) {
           gq[at] = o;
         } else {
@@ -836,6 +943,14 @@ __global__ void __launch_bounds__(BLOCK, 3) distill_block_kernel(const DistillAr
           out[3] = o.w;
         }
       }
+    };
+    float4 v[QUADS], next[QUADS];
+    if (p.q0 < p.q1) read(p.q0, v);
+    for (uint32_t q = p.q0; q < p.q1; q += 2 * HALF) {
+      if (q + HALF < p.q1) read(q + HALF, next);
+      write(q, v);
+      if (q + 2 * HALF < p.q1) read(q + 2 * HALF, v);
+      if (q + HALF < p.q1) write(q + HALF, next);
     }
     __syncthreads();
     take_targets<BLOCK>(a, g, targets, f, p.first, p.end);
@@ -864,22 +979,22 @@ __global__ void __launch_bounds__(BLOCK) distill_warp_kernel(const DistillArgs a
     r = stats_of<SUM, PER>(v, c);
     complete<SUM>(r);
   }
-  const RowTargets<32> t = read_targets<32>(a, row, x, true, targets[warp], nullptr);
+  read_targets(a, row, x, true, targets[warp]);
   if (PASS != DistillPass::Backward) {
-    const float loss = row_loss<32>(a, r, t, nullptr);
+    const float loss = row_loss(a, r, targets[warp]);
     if (lane == 0) {
       a.loss[row] = loss;
       if (PASS == DistillPass::Forward && a.stats) save_stats(a, row, r);
     }
   }
   if (PASS != DistillPass::Forward) {
-    const GradFactors f = grad_factors(a, row, r, t.soft, t.label);
+    const GradFactors f = grad_factors<SUM>(a, row, r, targets[warp].soft, targets[warp].index[a.top_n], c);
     float* g = a.grad + row * a.ld_grad;
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const uint32_t i = uint32_t(j) * 32u + lane;
-      if (i < vocab) g[i] = f.empty ? 0.f : grad_at<SUM>(f, v[j], c);
+      if (i < vocab) g[i] = grad_at<SUM>(f, v[j], c);
     }
     __syncwarp();
     take_targets<32>(a, g, targets[warp], f, 0, vocab);

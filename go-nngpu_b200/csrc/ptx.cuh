@@ -424,6 +424,35 @@ __device__ __forceinline__ bool flag_wait(const uint32_t* word, uint32_t wanted,
   return false;
 }
 
+// ------------------------------------------------- pairs of floats
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t"
+      ".reg .b64 A, B, C, D;\n\t"
+      "mov.b64 A, {%2, %3};\n\t"
+      "mov.b64 B, {%4, %5};\n\t"
+      "mov.b64 C, {%6, %7};\n\t"
+      "fma.rn.f32x2 D, A, B, C;\n\t"
+      "mov.b64 {%0, %1}, D;\n\t"
+      "}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t"
+      ".reg .b64 A, B, D;\n\t"
+      "mov.b64 A, {%2, %3};\n\t"
+      "mov.b64 B, {%4, %5};\n\t"
+      "add.rn.f32x2 D, A, B;\n\t"
+      "mov.b64 {%0, %1}, D;\n\t"
+      "}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 // ------------------------------------------------- descriptors (host+device)
 // Shared-memory matrix descriptor for tcgen05.mma, 128-byte swizzle:
 //   [0,14) start address >> 4, [16,30) leading byte offset >> 4,
