@@ -14,7 +14,7 @@ SOURCES = ["gemm_sm100.cu", "hbm_kernels.cu", "elementwise.cu", "bridge.cu", "st
 HEADERS = ["ptx.cuh", "kernels.h", "launch.cuh", "activation.cuh", "mxfp4.cuh", "status.cuh", "tmap.h",
            os.path.join("..", "..", "include", "gonngpu.h")]
 NVCC_FLAGS = [
-    "-std=c++17", "-O3", "-lineinfo",
+    "-std=c++20", "-O3", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
     "-shared", "-cudart", "static",

@@ -9,26 +9,27 @@
 //   m' = max(m1, m2),  S' = sum_i S_i e^(m_i-m'),  U' = sum_i e^(m_i-m') (U_i + (m_i-m') S_i).
 // log p(t) = (x_t - m) - log S, and the entropy is log S - U / S.
 //
-// Short rows (up to 1024 logits) are held in the registers of one warp.  Longer ones are streamed
-// by a block of 256 threads that loads the next 16 logits of a thread while it adds the last 16
-// (loading 32, then adding 32, reached half of the copy rate: the additions take as long as half
-// the loads); few long rows are shared by the up to 8 blocks of a cluster, which merge what they found through distributed shared memory.  All merges
-// have a fixed order: results repeat bit for bit.
+// Short rows (up to 1024 logits) are held in the registers of one warp.  Longer ones go through a
+// ring of shared-memory stages of 4096 or 8192 logits: one warp of a block feeds it with bulk copies,
+// ahead of the eight or sixteen warps that add (T threads), and into the next row; another warp takes care of what is little
+// and slow, the tokens, targets and results of a row.  Few long rows are shared by the up to 8 blocks
+// of a cluster.  All merges have a fixed order: results repeat bit for bit.
 #include <algorithm>
 
 #include "kernels.h"
 #include "launch.cuh"
 #include "ptx.cuh"
+#include "status.cuh"
 
 namespace gonn {
 
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int BLOCK = 256;
-constexpr int WARPS = BLOCK / 32;
-constexpr uint32_t QUADS = 4;                       // 16-byte loads of a thread in one half step
-constexpr uint32_t HALF = QUADS * BLOCK;            // pieces that a block takes in a half step
+constexpr int BLOCK = 256;                          // adding threads of a ring kernel, and
+constexpr int WIDE = 512;                           // of the step, which has an SM to itself
+constexpr int ROWS_BLOCK = 256;                     // threads of a kernel with a warp per row
+constexpr uint32_t QUADS = 4;                       // 16-byte pieces of an adding thread in one stage
 constexpr uint32_t WARP_ROW = 1024;                 // longest row that one warp holds
 constexpr uint32_t MAX_SHARE = 8;                   // blocks of a cluster
 
@@ -47,6 +48,41 @@ __device__ __forceinline__ float exp2_ftz(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// ---- barriers of the T adding threads alone -------------------------------------------------
+template <int T>
+__device__ __forceinline__ void adders_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(T) : "memory");
+}
+template <int T>
+__device__ __forceinline__ bool adders_or(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P, Q;\n\t"
+      "setp.ne.u32 P, %1, 0;\n\t"
+      "bar.red.or.pred Q, 1, %2, P;\n\t"
+      "selp.u32 %0, 1, 0, Q;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"(uint32_t(v)), "n"(T)
+      : "memory");
+  return r != 0;
+}
+template <int T>
+__device__ __forceinline__ uint32_t adders_count(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred P;\n\t"
+      "setp.ne.u32 P, %1, 0;\n\t"
+      "bar.red.popc.u32 %0, 1, %2, P;\n\t"
+      "}\n"
+      : "=r"(r)
+      : "r"(uint32_t(v)), "n"(T)
+      : "memory");
+  return r;
 }
 
 // ---- statistics of (part of) a row ------------------------------------------------------
@@ -111,12 +147,13 @@ __device__ __forceinline__ float warp_max(float v) {
 
 // The statistics of the block in every thread: the maximum first, then the sums relative to it, in
 // a fixed order.
-template <Sum SUM>
-__device__ RowStats block_merge(RowStats r, float c, float (*smem)[WARPS]) {
+template <Sum SUM, int T>
+__device__ RowStats block_merge(RowStats r, float c, float (*smem)[T / 32]) {
+  constexpr int WARPS = T / 32;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float mine = warp_max(r.m);
   if (lane == 0) smem[0][warp] = mine;
-  __syncthreads();
+  adders_sync<T>();
   float m = smem[0][0];
 #pragma unroll
   for (int w = 1; w < WARPS; ++w) m = fmaxf(m, smem[0][w]);
@@ -126,7 +163,7 @@ __device__ RowStats block_merge(RowStats r, float c, float (*smem)[WARPS]) {
     smem[1][warp] = s;
     smem[2][warp] = u;
   }
-  __syncthreads();
+  adders_sync<T>();
   r.m = m;
   r.s = smem[1][0];
   r.u = smem[2][0];
@@ -134,26 +171,6 @@ __device__ RowStats block_merge(RowStats r, float c, float (*smem)[WARPS]) {
   for (int w = 1; w < WARPS; ++w) {
     r.s += smem[1][w];
     r.u += smem[2][w];
-  }
-  return r;
-}
-
-// The statistics of all blocks of the cluster, in the order of their ranks; `slot` is this block's.
-// Everything the blocks did before is visible to all of them afterwards.
-template <Sum SUM>
-__device__ RowStats cluster_merge(RowStats r, float c, RowStats* slot, uint32_t shares) {
-  if (threadIdx.x == 0) *slot = r;
-  __syncthreads();
-  ptx::cluster_sync_all();
-  const uint32_t at = ptx::smem_u32(slot);
-  for (uint32_t k = 0; k < shares; ++k) {
-    const uint32_t there = ptx::mapa_shared(at, k);
-    RowStats other;
-    other.m = ptx::ld_shared_cluster(there);
-    other.s = ptx::ld_shared_cluster(there + 4);
-    other.u = ptx::ld_shared_cluster(there + 8);
-    if (k == 0) r = other;
-    else merge<SUM>(r, other, c);
   }
   return r;
 }
@@ -168,43 +185,122 @@ __device__ __forceinline__ float log_prob(const RowStats& r, float x) {
 // ---- a block's part of a long row --------------------------------------------------------
 // Whole 16-byte pieces of the row's memory, split evenly over the blocks of the cluster; the up to
 // three logits before the first piece belong to the first block and those behind the last one to
-// the last block, a thread each ("extra").
+// the last block, a thread each.
 struct Part {
   const float4* quads;  // first piece of the row
   uint32_t lead;        // logits before it
   uint32_t q0, q1;      // this block's pieces
-  int extra;            // this thread's logit outside the pieces, or -1
   uint32_t first, end;  // this block's logits
+  uint32_t tail;        // first logit behind the row's pieces
 };
 
 __device__ __forceinline__ Part part_of(const float* x, uint32_t vocab, uint32_t rank, uint32_t shares) {
   Part p;
   p.lead = min(uint32_t((16u - (reinterpret_cast<uintptr_t>(x) & 15u)) & 15u) / 4u, vocab);
-  const uint32_t all = (vocab - p.lead) / 4u, tail = vocab - p.lead - all * 4u;
+  const uint32_t all = (vocab - p.lead) / 4u;
   p.quads = reinterpret_cast<const float4*>(x + p.lead);
   p.q0 = uint32_t(uint64_t(all) * rank / shares);
   p.q1 = uint32_t(uint64_t(all) * (rank + 1) / shares);
-  const bool head = rank == 0, last = rank + 1 == shares;
-  const uint32_t t = threadIdx.x;
-  p.extra = t < 4 ? (head && t < p.lead ? int(t) : -1) : (last && t - 4u < tail ? int(p.lead + all * 4u + t - 4u) : -1);
-  p.first = head ? 0u : p.lead + p.q0 * 4u;
-  p.end = last ? vocab : p.lead + p.q1 * 4u;
+  p.tail = p.lead + all * 4u;
+  p.first = rank == 0 ? 0u : p.lead + p.q0 * 4u;
+  p.end = rank + 1 == shares ? vocab : p.lead + p.q1 * 4u;
   return p;
+}
+// This thread's logit outside the pieces, or -1.
+__device__ __forceinline__ int extra_of(const Part& p) {
+  const uint32_t t = threadIdx.x;
+  if (t < 4) return p.first == 0 && t < p.lead ? int(t) : -1;
+  return p.tail >= p.first && p.tail + t - 4u < p.end && t < 8 ? int(p.tail + t - 4u) : -1;
 }
 
 __device__ __forceinline__ float4 masked_quad() { return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
 
-// A thread's 16 logits of the half step at piece `q`; -inf past the part's end.
-__device__ __forceinline__ void load_quads(const Part& p, uint32_t q, float4 (&v)[QUADS]) {
-  const float4* at = p.quads + q + threadIdx.x;
-  if (q + HALF <= p.q1) {
+// ---- the ring ------------------------------------------------------------------------------
+// full[s]: the feeder's arrival and the stage's bytes; empty[s]: the adding warps.
+template <int T>
+constexpr uint32_t kStage = QUADS * T;  // pieces of a stage: 16 or 32 KB
+template <int T>
+constexpr uint32_t kStages = T == WIDE ? 6 : 4;  // 192 KB and one block an SM, or 64 KB and three
+template <int T>
+struct RingBars {
+  uint64_t full[kStages<T>], empty[kStages<T>];
+  __device__ void init() {
+    for (uint32_t i = 0; i < kStages<T>; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&full[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&empty[i]), T / 32);
+    }
+  }
+};
+
+// What all roles of a ring kernel share.  A wait that runs out is reported and the roles carry on
+// without waiting (every index they use stays within the row): results are then undefined, the
+// call fails, and all barriers are still met.
+struct Waits {
+  GemmStatus* status;
+  volatile uint32_t* abort_flag;
+  __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, uint32_t where) const {
+    if (!ptx::mbar_wait(ptx::smem_u32(bar), parity, abort_flag)) gave_up(where);
+  }
+  __device__ __forceinline__ void wait_cluster(uint64_t* bar, uint32_t parity, uint32_t where) const {
+    if (!ptx::mbar_wait_cluster(ptx::smem_u32(bar), parity, abort_flag)) gave_up(where);
+  }
+  __device__ __noinline__ void gave_up(uint32_t where) const {
+    if (first_to_give_up(abort_flag)) report(status, 1, where, blockIdx.x, 0);
+  }
+};
+__device__ __forceinline__ void arrive(uint64_t* bar) { ptx::mbar_arrive(ptx::smem_u32(bar)); }
+
+// Place and phase of a ring's next stage.
+template <int T>
+struct RingAt {
+  uint32_t slot = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == kStages<T>) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
+// One lane feeds a part's stages; a part without pieces is one empty stage.
+template <int T>
+__device__ __forceinline__ void feed_part(const Part& p, float4* ring, RingBars<T>& bars, RingAt<T>& at,
+                                          const Waits& w) {
+  uint32_t q = p.q0;
+  do {
+    const uint32_t n = min(kStage<T>, p.q1 - q);
+    w.wait(&bars.empty[at.slot], at.phase ^ 1u, 0x10u | at.slot);
+    const uint32_t full = ptx::smem_u32(&bars.full[at.slot]);
+    if (n) {
+      ptx::mbar_arrive_expect_tx(full, n * 16);
+      ptx::bulk_load(ptx::smem_u32(ring + at.slot * kStage<T>), p.quads + q, n * 16, full);
+    } else {
+      ptx::mbar_arrive(full);
+    }
+    at.next();
+    q += kStage<T>;
+  } while (q < p.q1);
+}
+
+// A thread's logits of the stage that holds the pieces from `q`; -inf past the part's end.  WAIT:
+// the stage may not have arrived; LEAVE: it is not needed any more.
+template <int T, bool WAIT, bool LEAVE>
+__device__ __forceinline__ void take_stage(const Part& p, uint32_t q, const float4* ring, RingBars<T>& bars,
+                                           RingAt<T>& at, const Waits& w, float4 (&v)[QUADS]) {
+  if (WAIT) w.wait(&bars.full[at.slot], at.phase, at.slot);
+  const float4* from = ring + at.slot * kStage<T> + threadIdx.x;
+  if (q + kStage<T> <= p.q1) {
 #pragma unroll
-    for (uint32_t j = 0; j < QUADS; ++j) v[j] = at[j * BLOCK];
+    for (uint32_t j = 0; j < QUADS; ++j) v[j] = from[j * T];
   } else {
 #pragma unroll
-    for (uint32_t j = 0; j < QUADS; ++j)
-      v[j] = q + j * BLOCK + threadIdx.x < p.q1 ? at[j * BLOCK] : masked_quad();
+    for (uint32_t j = 0; j < QUADS; ++j) v[j] = q + j * T + threadIdx.x < p.q1 ? from[j * T] : masked_quad();
   }
+  if (LEAVE) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) arrive(&bars.empty[at.slot]);
+  }
+  at.next();
 }
 
 __device__ __forceinline__ float max4(const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
@@ -272,7 +368,7 @@ struct Stream {
     }
   }
 
-  // Adds 16 logits; returns their maximum.
+  // Adds a thread's logits of a stage; returns their maximum.
   __device__ __forceinline__ float add(const float4 (&v)[QUADS], float c) {
     float most = max4(v[0]);
 #pragma unroll
@@ -331,24 +427,23 @@ constexpr uint32_t kMaskedBits = 0x007fffffu;  // order_bits(-inf); below it onl
 // to have `want` keys above it.  The first floor comes from the threads' maxima of their first 32
 // logits (as many of those as wanted lie above it, so as many logits do); when more than about
 // twice the wanted keys are kept, the surplus is thrown out and the floor rises to the exact
-// want-th key, which in ordinary rows happens each time the logits seen have doubled.
+// want-th key, which in ordinary rows happens each time the logits seen have tripled.
 struct Selection {
-  static constexpr uint32_t CAP = 2048;
+  static constexpr uint32_t CAP = 1024;
   uint64_t key[CAP];
-  uint64_t sorted[kMaxTop];
   uint64_t floor;
   uint32_t count;
-  uint32_t part[2][WARPS];
+  uint32_t part[2][BLOCK / 32];
 };
 
 // Sum over the block of a count; `turn` alternates so that one barrier a call is enough.
 __device__ __forceinline__ uint32_t block_count(Selection& s, uint32_t n, uint32_t& turn) {
   n = __reduce_add_sync(0xffffffffu, n);
   if ((threadIdx.x & 31) == 0) s.part[turn][threadIdx.x >> 5] = n;
-  __syncthreads();
+  adders_sync<BLOCK>();
   uint32_t all = 0;
 #pragma unroll
-  for (int w = 0; w < WARPS; ++w) all += s.part[turn][w];
+  for (int w = 0; w < BLOCK / 32; ++w) all += s.part[turn][w];
   turn ^= 1u;
   return all;
 }
@@ -369,7 +464,7 @@ __device__ void keep_largest(Selection& s, uint32_t n, uint32_t want) {
     const uint64_t trial = floor | (1ull << bit);
     uint32_t above = 0;
     if (n <= BLOCK) {
-      above = uint32_t(__syncthreads_count(mine[0] >= trial));
+      above = adders_count<BLOCK>(mine[0] >= trial);
     } else {
 #pragma unroll
       for (uint32_t i = 0; i < PER; ++i) above += mine[i] >= trial;
@@ -382,11 +477,11 @@ __device__ void keep_largest(Selection& s, uint32_t n, uint32_t want) {
     s.count = 0;
     s.floor = floor;
   }
-  __syncthreads();
+  adders_sync<BLOCK>();
 #pragma unroll
   for (uint32_t i = 0; i < PER; ++i)
     if (mine[i] >= floor && mine[i] != 0) s.key[atomicAdd(&s.count, 1u)] = mine[i];
-  __syncthreads();
+  adders_sync<BLOCK>();
 }
 
 // The first floor from the threads' maxima: 20 bits of it.
@@ -395,7 +490,7 @@ __device__ void first_floor(Selection& s, float most, uint32_t want) {
   uint32_t floor = 0;
   for (int bit = 31; bit >= 12; --bit) {
     const uint32_t trial = floor | (1u << bit);
-    const uint32_t above = uint32_t(__syncthreads_count(bits >= trial));
+    const uint32_t above = adders_count<BLOCK>(bits >= trial);
     if (above >= want) floor = trial;
     if (above == want) break;
   }
@@ -403,13 +498,14 @@ __device__ void first_floor(Selection& s, float most, uint32_t want) {
     s.floor = uint64_t(floor) << 32;
     s.count = 0;
   }
-  __syncthreads();
+  adders_sync<BLOCK>();
 }
 
 // The floor's value as a bound on logits; one below the order of -inf lets everything pass.
 __device__ __forceinline__ float floor_value(uint64_t floor) {
   return uint32_t(floor >> 32) <= kMaskedBits ? -INFINITY : key_value(floor);
 }
+constexpr uint32_t STEP = 2;  // stages between two offers to the selection: 8192 logits
 // Which of a thread's 16 logits from piece `q` may lie above the floor, a bit each.
 __device__ __forceinline__ uint32_t above_floor(const Part& p, uint32_t q, const float4 (&v)[QUADS], float low) {
   uint32_t hits = 0;
@@ -422,10 +518,10 @@ __device__ __forceinline__ uint32_t above_floor(const Part& p, uint32_t q, const
   return hits;
 }
 
-// Offers a thread's logits of a whole step (two halves from piece `q`, the marked ones) and, with
-// `outside`, its logit outside the pieces to the selection.  All threads of the block call it.
+// Offers a thread's logits of a whole step (STEP stages from piece `q`, the marked ones) and, with
+// `outside`, its logit `extra` outside the pieces to the selection.  All adding threads call it.
 __device__ __forceinline__ void offer(Selection& s, const float* x, const Part& p, uint32_t q, uint32_t hits,
-                                      bool outside, uint32_t want) {
+                                      bool outside, int extra, uint32_t want) {
   uint64_t floor = s.floor;
   const uint32_t limit = 2 * want + 64;
   while (true) {
@@ -434,7 +530,7 @@ __device__ __forceinline__ void offer(Selection& s, const float* x, const Part& 
     while (left | uint32_t(outside)) {
       // few logits get here; their values are read again (from L1) rather than picked out of the
       // registers
-      uint32_t index = uint32_t(p.extra), bit = 0;
+      uint32_t index = uint32_t(extra), bit = 0;
       if (left) {
         bit = left & (0u - left);
         const uint32_t i = 31u - uint32_t(__clz(int(bit)));
@@ -458,16 +554,17 @@ __device__ __forceinline__ void offer(Selection& s, const float* x, const Part& 
         break;  // the buffer is full: nothing after this one fits either
       }
     }
-    if (!__syncthreads_or(over)) return;
+    if (!adders_or<BLOCK>(over)) return;
     keep_largest(s, min(s.count, Selection::CAP), want);
     floor = s.floor;
-    if (!__syncthreads_or(hits != 0 || outside)) return;
+    if (!adders_or<BLOCK>(hits != 0 || outside)) return;
   }
 }
 
-// Sorts the selection's keys: s.sorted[0 .. min(n, want)) in descending order.  Returns how many.
-__device__ uint32_t sort_selection(Selection& s, uint32_t want) {
-  __syncthreads();
+// Sorts the selection's keys: sorted[0 .. min(n, want)) in descending order.  Returns how many.
+// The caller sees to it that `sorted` is complete before it is read.
+__device__ uint32_t sort_selection(Selection& s, uint64_t* sorted, uint32_t want) {
+  adders_sync<BLOCK>();
   uint32_t n = s.count;
   if (n > 2 * kMaxTop + 64) {  // the alternatives of several blocks
     keep_largest(s, n, want);
@@ -479,9 +576,8 @@ __device__ uint32_t sort_selection(Selection& s, uint32_t want) {
     uint32_t place = 0;
 #pragma unroll 8
     for (uint32_t j = 0; j < n; ++j) place += s.key[j] > mine;
-    if (place < want) s.sorted[place] = mine;
+    if (place < want) sorted[place] = mine;
   }
-  __syncthreads();
   return min(n, want);
 }
 
@@ -500,83 +596,168 @@ __device__ __forceinline__ float row_entropy(const RowStats& r) {
   return r.s == 0.f ? 0.f : logf(r.s) - r.u / r.s;
 }
 
+// The results of one row, by one warp.
+__device__ __forceinline__ void write_logprobs(const LogprobArgs& a, const RowStats& r, uint64_t row, const float* x,
+                                               const uint64_t* sorted) {
+  const uint32_t lane = threadIdx.x & 31;
+  for (uint32_t t = lane; t < a.n_tokens; t += 32) a.logprobs[row * a.n_tokens + t] = token_logprob(a, r, row, x, t);
+  if (a.entropy && lane == 0) a.entropy[row] = row_entropy(r);
+  const bool nan = !(r.s == r.s);
+  for (uint32_t k = lane; k < a.top_n; k += 32) {
+    const uint64_t key = sorted[k];
+    a.top_tokens[row * a.top_n + k] = nan ? -1 : int(key_index(key));
+    a.top_logprobs[row * a.top_n + k] = nan ? NAN : log_prob(r, key_value(key));
+  }
+}
+
+// Long rows.  With shares > 1 a cluster has exactly one row.
 template <bool TOP>
-__global__ void __launch_bounds__(BLOCK, 4) logprobs_block_kernel(const LogprobArgs a, uint32_t shares) {
+__global__ void __launch_bounds__(BLOCK + 64, 3)
+logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
+  constexpr int T = BLOCK, WARPS = T / 32;
+  extern __shared__ float4 ring[];
+  __shared__ RingBars<T> bars;
+  __shared__ uint64_t ready[2], freed[2];  // a row's results: written by the adders, read by the server
+  __shared__ uint32_t abort_word;
+  __shared__ float merged[3][WARPS];
+  __shared__ RowStats result[2];
+  __shared__ uint64_t sorted[2][TOP ? kMaxTop : 1];
+  __shared__ Selection sel;
+  const uint32_t warp = threadIdx.x >> 5, rank = blockIdx.x % shares, vocab = uint32_t(a.vocab);
+  const uint64_t first_row = blockIdx.x / shares, step = gridDim.x / shares;
+  if (threadIdx.x == 0) {
+    bars.init();
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&ready[i]), WARPS);
+      ptx::mbar_init(ptx::smem_u32(&freed[i]), 1);
+    }
+    abort_word = 0;
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+  }
+  __syncthreads();
   ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
   ptx::grid_dependency_wait();
-  __shared__ float merged[3][WARPS];
-  __shared__ RowStats slot;
-  __shared__ Selection sel;
-  const uint32_t rank = blockIdx.x % shares;
-  const uint64_t row = blockIdx.x / shares;
-  const float* x = a.x + row * a.ld;
-  const Part p = part_of(x, uint32_t(a.vocab), rank, shares);
-  const float extra = p.extra >= 0 ? x[p.extra] : -INFINITY;
-  Stream<Sum::Entropy> stream;
-  float4 v[QUADS], next[QUADS];
-  load_quads(p, p.q0, v);
-  for (uint32_t q = p.q0; q < p.q1 || q == p.q0; q += 2 * HALF) {
-    const bool first = q == p.q0;
-    const float low = TOP && !first ? floor_value(sel.floor) : INFINITY;
-    uint32_t hits = 0;
-    load_quads(p, q + HALF, next);
-    const float most = stream.add(v, kLog2e);
-    if (TOP && most >= low) hits = above_floor(p, q, v, low);
-    load_quads(p, q + 2 * HALF, v);
-    const float most2 = stream.add(next, kLog2e);
-    if (TOP && most2 >= low) hits |= above_floor(p, q + HALF, next, low) << 16;
-    if (TOP) {
-      bool outside = false;
-      if (first) {
-        const float all = fmaxf(fmaxf(most, most2), extra);
-        first_floor(sel, all, a.top_n);
-        const float start = floor_value(sel.floor);
-        if (all >= start) {  // the first half comes from L1 once more
-          outside = p.extra >= 0 && extra >= start;
-          hits = above_floor(p, q + HALF, next, start) << 16;
-          load_quads(p, q, next);
-          hits |= above_floor(p, q, next, start);
+  const Waits w{a.status, &abort_word};
+
+  if (warp == WARPS) {  // feeder
+    if ((threadIdx.x & 31) == 0) {
+      RingAt<T> at;
+      for (uint64_t row = first_row; row < a.rows; row += step)
+        feed_part<T>(part_of(a.x + row * a.ld, vocab, rank, shares), ring, bars, at, w);
+    }
+    __syncwarp();
+  } else if (warp == WARPS + 1) {  // server
+    if (shares == 1) {
+      uint32_t i = 0;
+      for (uint64_t row = first_row; row < a.rows; row += step, ++i) {
+        w.wait(&ready[i & 1], (i >> 1) & 1u, 0x20u);
+        write_logprobs(a, result[i & 1], row, a.x + row * a.ld, sorted[i & 1]);
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) arrive(&freed[i & 1]);
+      }
+    }
+  } else {  // adders
+    RingAt<T> at;
+    uint32_t i = 0;
+    for (uint64_t row = first_row; row < a.rows; row += step, ++i) {
+      const float* x = a.x + row * a.ld;
+      const Part p = part_of(x, vocab, rank, shares);
+      const int extra_at = extra_of(p);
+      const float extra = extra_at >= 0 ? x[extra_at] : -INFINITY;
+      Stream<Sum::Entropy> stream;
+      uint32_t q = p.q0;
+      do {
+        const bool first = q == p.q0;
+        const float low = TOP && !first ? floor_value(sel.floor) : INFINITY;
+        uint32_t hits = 0;
+        float most = first ? extra : -INFINITY;
+        float4 v[QUADS];
+#pragma unroll 1
+        for (uint32_t k = 0; k < STEP && (k == 0 || q + k * kStage<T> < p.q1); ++k) {
+          take_stage<T, true, true>(p, q + k * kStage<T>, ring, bars, at, w, v);
+          const float here = stream.add(v, kLog2e);
+          if (TOP) {
+            if (here >= low) hits |= above_floor(p, q + k * kStage<T>, v, low) << (16 * k);
+            most = fmaxf(most, here);
+          }
+        }
+        if (TOP) {
+          bool outside = false;
+          if (first) {
+            first_floor(sel, most, a.top_n);
+            const float start = floor_value(sel.floor);
+            if (most >= start) {  // the first logits are read once more, from L2
+              outside = extra_at >= 0 && extra >= start;
+#pragma unroll 1
+              for (uint32_t k = 0; k < STEP; ++k) {
+#pragma unroll
+                for (uint32_t j = 0; j < QUADS; ++j) {
+                  const uint32_t piece = q + k * kStage<T> + j * T + threadIdx.x;
+                  v[j] = piece < p.q1 ? p.quads[piece] : masked_quad();
+                }
+                hits |= above_floor(p, q + k * kStage<T>, v, start) << (16 * k);
+              }
+            }
+          }
+          offer(sel, x, p, q, hits, outside, extra_at, a.top_n);
+        }
+        q += STEP * kStage<T>;
+      } while (q < p.q1);
+      RowStats r = stream.result(kLog2e);
+      add_one<Sum::Entropy>(r, extra, 0.f);
+      r = block_merge<Sum::Entropy, T>(r, 0.f, merged);
+      w.wait(&freed[i & 1], ((i >> 1) & 1u) ^ 1u, 0x21u);
+      uint32_t found = 0;
+      if (TOP) found = sort_selection(sel, sorted[i & 1], a.top_n);
+      if (threadIdx.x == 0) result[i & 1] = r;
+      if (TOP && shares > 1) {  // for the first block of the cluster
+        adders_sync<T>();
+        if (threadIdx.x == 0) sel.count = found;
+      }
+      // (the next row's first floor comes behind barriers that all threads reach after this)
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) arrive(&ready[i & 1]);
+    }
+  }
+
+  if (shares > 1) {
+    __syncthreads();
+    ptx::cluster_sync_all();  // every block's results are in place
+    if (rank == 0 && warp < WARPS) {
+      RowStats r = result[0];
+      const uint32_t at = ptx::smem_u32(&result[0]);
+      uint32_t n = 0;
+      if (TOP) {  // the blocks' own alternatives, at most 8 x 128, behind one another
+        n = sel.count;
+        if (threadIdx.x < n) sel.key[threadIdx.x] = sorted[0][threadIdx.x];
+      }
+      for (uint32_t k = 1; k < shares; ++k) {
+        RowStats other;
+        other.m = ptx::ld_shared_cluster(ptx::mapa_shared(at, k));
+        other.s = ptx::ld_shared_cluster(ptx::mapa_shared(at + 4, k));
+        other.u = ptx::ld_shared_cluster(ptx::mapa_shared(at + 8, k));
+        merge<Sum::Entropy>(r, other, 0.f);
+        if (TOP) {
+          const uint32_t theirs = ptx::ld_shared_cluster_u32(ptx::mapa_shared(ptx::smem_u32(&sel.count), k));
+          if (threadIdx.x < theirs)
+            sel.key[n + threadIdx.x] =
+                ptx::ld_shared_cluster_u64(ptx::mapa_shared(ptx::smem_u32(&sorted[0][threadIdx.x]), k));
+          n += theirs;
         }
       }
-      offer(sel, x, p, q, hits, outside, a.top_n);
-    }
-  }
-  RowStats r = stream.result(kLog2e);
-  add_one<Sum::Entropy>(r, extra, 0.f);
-  r = block_merge<Sum::Entropy>(r, 0.f, merged);
-  uint32_t found = 0;
-  if (TOP) found = sort_selection(sel, a.top_n);
-  if (shares > 1) {
-    if (TOP && threadIdx.x == 0) sel.count = found;
-    r = cluster_merge<Sum::Entropy>(r, 0.f, &slot, shares);
-    if (TOP && rank == 0) {
-      // the blocks' own alternatives, at most 8 x 128, behind one another
-      uint32_t n = found;
-      __syncthreads();
-      if (threadIdx.x < found) sel.key[threadIdx.x] = sel.sorted[threadIdx.x];
-      for (uint32_t k = 1; k < shares; ++k) {
-        const uint32_t theirs = ptx::ld_shared_cluster_u32(ptx::mapa_shared(ptx::smem_u32(&sel.count), k));
-        if (threadIdx.x < theirs)
-          sel.key[n + threadIdx.x] =
-              ptx::ld_shared_cluster_u64(ptx::mapa_shared(ptx::smem_u32(&sel.sorted[threadIdx.x]), k));
-        n += theirs;
+      if (TOP) {
+        adders_sync<T>();
+        if (threadIdx.x == 0) sel.count = n;
+        sort_selection(sel, sorted[1], a.top_n);
+        adders_sync<T>();
       }
-      __syncthreads();
-      if (threadIdx.x == 0) sel.count = n;
-      found = sort_selection(sel, a.top_n);
+      if (warp == 0) write_logprobs(a, r, first_row, a.x + first_row * a.ld, sorted[1]);
     }
     ptx::cluster_sync_all();  // no block leaves while another still reads its shared memory
-    if (rank != 0) return;
   }
-  for (uint32_t t = threadIdx.x; t < a.n_tokens; t += BLOCK)
-    a.logprobs[row * a.n_tokens + t] = token_logprob(a, r, row, x, t);
-  if (a.entropy && threadIdx.x == 0) a.entropy[row] = row_entropy(r);
-  if (TOP && threadIdx.x < a.top_n) {
-    const bool nan = !(r.s == r.s);
-    const uint32_t index = key_index(sel.sorted[threadIdx.x]);
-    a.top_tokens[row * a.top_n + threadIdx.x] = nan ? -1 : int(index);
-    a.top_logprobs[row * a.top_n + threadIdx.x] = nan ? NAN : log_prob(r, x[index]);
-  }
+  __syncthreads();
+  wait_out(&abort_word);
 }
 
 // One warp a row, PER logits a lane in registers.
@@ -607,11 +788,11 @@ __device__ __forceinline__ RowStats stats_of(const float (&v)[PER], float c) {
 }
 
 template <int PER>
-__global__ void __launch_bounds__(BLOCK) logprobs_warp_kernel(const LogprobArgs a) {
+__global__ void __launch_bounds__(ROWS_BLOCK) logprobs_warp_kernel(const LogprobArgs a) {
   ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
   ptx::grid_dependency_wait();
   const uint32_t lane = threadIdx.x & 31, vocab = uint32_t(a.vocab);
-  const uint64_t row = uint64_t(blockIdx.x) * WARPS + (threadIdx.x >> 5);
+  const uint64_t row = uint64_t(blockIdx.x) * (ROWS_BLOCK / 32) + (threadIdx.x >> 5);
   if (row >= a.rows) return;
   const float* x = a.x + row * a.ld;
   float v[PER];
@@ -674,8 +855,10 @@ struct Targets {
 };
 
 // Reads the row's targets, the student's logits at them included: before anyone may overwrite the
-// row with its gradient.  Called by one warp; `report`: one warp of a row reports bad indices.
-__device__ void read_targets(const DistillArgs& a, uint64_t row, const float* x, bool report, Targets& t) {
+// row with its gradient.  Called by one warp; `tell`: one warp of a row reports bad indices; LOSS:
+// the student's logits are wanted.
+template <bool LOSS>
+__device__ void read_targets(const DistillArgs& a, uint64_t row, const float* x, bool tell, Targets& t) {
   constexpr int PER = kMaxTop / 32;
   const uint32_t lane = threadIdx.x & 31;
   const float inv_t = 1.f / a.temperature;
@@ -694,21 +877,21 @@ __device__ void read_targets(const DistillArgs& a, uint64_t row, const float* x,
   }
   int label = lane == 0 && a.labels ? a.labels[row] : -1;
   if (label >= 0 && uint64_t(label) >= a.vocab) {
-    if (report) report_index(a.status, INDEX_LABEL, row, label);
+    if (tell) report_index(a.status, INDEX_LABEL, row, label);
     label = -1;
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     if (index[i] >= 0 && uint64_t(index[i]) >= a.vocab) {
-      if (report) report_index(a.status, INDEX_TEACHER, row, index[i]);
+      if (tell) report_index(a.status, INDEX_TEACHER, row, index[i]);
       index[i] = -1;
     }
     if (z[i] == -INFINITY) index[i] = -1;
-    if (index[i] >= 0) x_at[i] = x[index[i]];
-    else z[i] = -INFINITY;
+    if (index[i] < 0) z[i] = -INFINITY;
+    else if (LOSS) x_at[i] = x[index[i]];
     zm = fmaxf(zm, z[i]);
   }
-  const float x_label = label >= 0 ? x[label] : 0.f;
+  const float x_label = LOSS && label >= 0 ? x[label] : 0.f;
   zm = warp_max(zm);
   float q[PER], total = 0.f;
 #pragma unroll
@@ -808,13 +991,12 @@ __device__ __forceinline__ float4 grad_quad(const GradFactors& f, const float4& 
 }
 
 // The places that the teacher and the label name, among [first, end): the first entry that names
-// a place takes away what all of them do there, in their order.
-template <int TEAM>
+// a place takes away what all of them do there, in their order.  Called by one warp.
 __device__ void take_targets(const DistillArgs& a, float* g, const Targets& t, const GradFactors& f, uint32_t first,
                              uint32_t end) {
   if (f.empty) return;
   const uint32_t n = a.top_n + 1;
-  for (uint32_t k = threadIdx.x % TEAM; k < n; k += TEAM) {
+  for (uint32_t k = threadIdx.x & 31; k < n; k += 32) {
     const int index = t.index[k];
     bool lead = index >= int(first) && uint32_t(index) < end;
 #pragma unroll 8
@@ -845,128 +1027,197 @@ __device__ __forceinline__ void save_stats(const DistillArgs& a, uint64_t row, c
   a.stats[row * 3 + 2] = r.s;
 }
 
-// Long rows.  The step keeps its part of the row in shared memory between the sums and the
-// gradient (`cached`; every thread reads back what it wrote itself); rows that do not fit are read
-// again, from L2 as far as they are still there.
+// Long rows.  In the step a block keeps its part of a row in the ring until the gradient has been
+// written from there (`keep`); what is left of the ring holds the first stages of the next row
+// meanwhile.  (Reading the row twice, with the rows in flight small enough for L2, took 1.6 times
+// as long: the clusters that takes spent their time waiting for one another.)  Only rows too long
+// for 8 blocks' rings are read twice.
+//
+// The serving warp reads a row's targets while the row before it is being added (tfull, tempty),
+// writes its loss (done) and corrects the gradient at the targets (written).  The blocks of a
+// cluster exchange their statistics by writing them into each other's shared memory (peers).
+template <DistillPass PASS>
+constexpr int kAdders = PASS == DistillPass::Step ? WIDE : BLOCK;
 template <DistillPass PASS, Sum SUM>
-__global__ void __launch_bounds__(BLOCK, 4) distill_block_kernel(const DistillArgs a, uint32_t shares, bool cached) {
+__global__ void __launch_bounds__(kAdders<PASS> + 64, PASS == DistillPass::Step ? 1 : 3)
+distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
+  constexpr int T = kAdders<PASS>, WARPS = T / 32;
+  extern __shared__ float4 ring[];
+  __shared__ RingBars<T> bars;
+  __shared__ uint64_t tfull[2], tempty[2], done[2], written[2], peers[2];
+  __shared__ uint32_t abort_word;
+  __shared__ float merged[3][WARPS];
+  __shared__ RowStats result[2], parts[2][MAX_SHARE];
+  __shared__ Targets targets[2];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % shares;
+  const uint32_t vocab = uint32_t(a.vocab);
+  const uint64_t first_row = blockIdx.x / shares, step = gridDim.x / shares;
+  const float c = kLog2e / a.temperature;
+  if (threadIdx.x == 0) {
+    bars.init();
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(ptx::smem_u32(&tfull[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&tempty[i]), WARPS);
+      ptx::mbar_init(ptx::smem_u32(&done[i]), 1);
+      ptx::mbar_init(ptx::smem_u32(&written[i]), WARPS);
+      ptx::mbar_init(ptx::smem_u32(&peers[i]), shares);
+    }
+    abort_word = 0;
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+  }
+  __syncthreads();
+  if (shares > 1) ptx::cluster_sync_all();  // the peers' barriers exist
   ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
   ptx::grid_dependency_wait();
-  extern __shared__ float4 cache[];
-  __shared__ float merged[3][WARPS];
-  __shared__ RowStats slot;
-  __shared__ Targets targets;
-  const float c = kLog2e / a.temperature;
-  const uint32_t rank = blockIdx.x % shares;
-  const uint64_t row = blockIdx.x / shares;
-  const float* x = a.x + row * a.ld;
-  const Part p = part_of(x, uint32_t(a.vocab), rank, shares);
-  // the targets' logits are read before any block of the row writes its gradient
-  if (threadIdx.x < 32 && (PASS != DistillPass::Forward || rank == 0)) read_targets(a, row, x, rank == 0, targets);
-  const float extra = p.extra >= 0 ? x[p.extra] : -INFINITY;
-  RowStats r;
-  if (PASS == DistillPass::Backward) {
-    r = saved_stats(a, row);
-  } else {
-    Stream<SUM> stream;
-    float4 v[QUADS], next[QUADS];
-    auto keep = [&](uint32_t q, const float4 (&w)[QUADS]) {
-      if (PASS != DistillPass::Step || !cached) return;
-#pragma unroll
-      for (uint32_t j = 0; j < QUADS; ++j) {
-        const uint32_t at = q + j * BLOCK + threadIdx.x;
-        if (at < p.q1) cache[at - p.q0] = w[j];
+  const Waits w{a.status, &abort_word};
+
+  if (warp == WARPS) {  // feeder
+    if (lane == 0) {
+      RingAt<T> at;
+      for (uint64_t row = first_row; row < a.rows; row += step) {
+        const Part p = part_of(a.x + row * a.ld, vocab, rank, shares);
+        feed_part<T>(p, ring, bars, at, w);
+        if (PASS == DistillPass::Step && !keep) feed_part<T>(p, ring, bars, at, w);
       }
+    }
+    __syncwarp();
+  } else if (warp == WARPS + 1) {  // server
+    uint32_t i = 0;
+    auto publish = [&](uint32_t k, uint64_t row) {
+      w.wait(&tempty[k & 1], ((k >> 1) & 1u) ^ 1u, 0x30u);
+      if (PASS != DistillPass::Forward || rank == 0)
+        read_targets<PASS != DistillPass::Backward>(a, row, a.x + row * a.ld, rank == 0, targets[k & 1]);
+      __syncwarp();
+      if (lane == 0) arrive(&tfull[k & 1]);
     };
-    load_quads(p, p.q0, v);
-    for (uint32_t q = p.q0; q < p.q1; q += 2 * HALF) {
-      load_quads(p, q + HALF, next);
-      stream.add(v, c);
-      keep(q, v);
-      load_quads(p, q + 2 * HALF, v);
-      stream.add(next, c);
-      keep(q + HALF, next);
-    }
-    r = stream.result(c);
-    add_one<SUM>(r, extra, c);
-    r = block_merge<SUM>(r, c, merged);
-  }
-  if (PASS != DistillPass::Backward) {
-    if (shares > 1) r = cluster_merge<SUM>(r, c, &slot, shares);
-    complete<SUM>(r);
-    if (rank == 0 && threadIdx.x < 32) {
-      const float loss = row_loss(a, r, targets);
-      if (threadIdx.x == 0) {
-        a.loss[row] = loss;
-        if (PASS == DistillPass::Forward && a.stats) save_stats(a, row, r);
-      }
-    }
-  }
-  if (PASS != DistillPass::Forward) {
-    // Backward: the targets have to be there; in the step the merge's barriers came after them
-    if (PASS == DistillPass::Backward) __syncthreads();
-    const GradFactors f = grad_factors<SUM>(a, row, r, targets.soft, targets.index[a.top_n], c);
-    float* g = a.grad + row * a.ld_grad;
-    if (p.extra >= 0) g[p.extra] = grad_at<SUM>(f, extra, c);
-    // the same distance to a 16-byte boundary in both rows: 16-byte stores
-    const bool vec = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
-    float4* gq = reinterpret_cast<float4*>(g + p.lead);
-    auto read = [&](uint32_t q, float4 (&v)[QUADS]) {
-      if (PASS == DistillPass::Step && cached) {
-#pragma unroll
-        for (uint32_t j = 0; j < QUADS; ++j) {
-          const uint32_t at = q + j * BLOCK + threadIdx.x;
-          if (at < p.q1) v[j] = cache[at - p.q0];
+    if (first_row < a.rows) publish(0, first_row);
+    for (uint64_t row = first_row; row < a.rows; row += step, ++i) {
+      if (row + step < a.rows) publish(i + 1, row + step);
+      const uint32_t turn = i & 1, phase = (i >> 1) & 1u;
+      w.wait(&done[turn], phase, 0x31u);
+      const RowStats r = result[turn];
+      if (PASS != DistillPass::Backward && rank == 0) {
+        const float loss = row_loss(a, r, targets[turn]);
+        if (lane == 0) {
+          a.loss[row] = loss;
+          if (PASS == DistillPass::Forward && a.stats) save_stats(a, row, r);
         }
+      }
+      if (PASS != DistillPass::Forward) {
+        const GradFactors f = grad_factors<SUM>(a, row, r, targets[turn].soft, targets[turn].index[a.top_n], c);
+        const Part p = part_of(a.x + row * a.ld, vocab, rank, shares);
+        w.wait(&written[turn], phase, 0x34u);
+        take_targets(a, a.grad + row * a.ld_grad, targets[turn], f, p.first, p.end);
+      }
+      __syncwarp();
+    }
+  } else {  // adders
+    RingAt<T> at;
+    uint32_t i = 0;
+    for (uint64_t row = first_row; row < a.rows; row += step, ++i) {
+      RingAt<T> start = at;
+      const uint32_t turn = i & 1, phase = (i >> 1) & 1u;
+      const float* x = a.x + row * a.ld;
+      const Part p = part_of(x, vocab, rank, shares);
+      const int extra_at = extra_of(p);
+      const float extra = extra_at >= 0 ? x[extra_at] : -INFINITY;
+      RowStats r;
+      if (PASS == DistillPass::Backward) {
+        r = saved_stats(a, row);
       } else {
-        load_quads(p, q, v);
+        Stream<SUM> stream;
+        uint32_t q = p.q0;
+        do {
+          float4 v[QUADS];
+          if (PASS == DistillPass::Step && keep) take_stage<T, true, false>(p, q, ring, bars, at, w, v);
+          else take_stage<T, true, true>(p, q, ring, bars, at, w, v);
+          stream.add(v, c);
+          q += kStage<T>;
+        } while (q < p.q1);
+        r = stream.result(c);
+        add_one<SUM>(r, extra, c);
+        r = block_merge<SUM, T>(r, c, merged);
       }
-    };
-    auto write = [&](uint32_t q, const float4 (&v)[QUADS]) {
-      if (vec && q + HALF <= p.q1) {
-#pragma unroll
-        for (uint32_t j = 0; j < QUADS; ++j) __stcs(gq + q + threadIdx.x + j * BLOCK, grad_quad<SUM>(f, v[j], c));
-        return;
-      }
-#pragma unroll
-      for (uint32_t j = 0; j < QUADS; ++j) {
-        const uint32_t at = q + j * BLOCK + threadIdx.x;
-        if (at >= p.q1) continue;
-        const float4 o = grad_quad<SUM>(f, v[j], c);
-        if (vec) {
-          gq[at] = o;
-        } else {
-          float* out = g + p.lead + uint64_t(at) * 4;
-          out[0] = o.x;
-          out[1] = o.y;
-          out[2] = o.z;
-          out[3] = o.w;
+      // From here on the targets have been read, in every block of the cluster once its
+      // statistics have arrived: the row may be overwritten.  The wait also says that the server
+      // is done with the result of two rows ago.
+      w.wait(&tfull[turn], phase, 0x32u);
+      if (PASS != DistillPass::Backward) {
+        if (shares > 1) {
+          if (threadIdx.x < shares) {
+            const uint32_t to = ptx::mapa_shared(ptx::smem_u32(&parts[turn][rank]), threadIdx.x);
+            ptx::st_shared_cluster(to, r.m);
+            ptx::st_shared_cluster(to + 4, r.s);
+            ptx::st_shared_cluster(to + 8, r.u);
+            ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_u32(&peers[turn]), threadIdx.x));
+          }
+          w.wait_cluster(&peers[turn], phase, 0x33u);
+          r = parts[turn][0];
+          for (uint32_t k = 1; k < shares; ++k) merge<SUM>(r, parts[turn][k], c);
         }
+        complete<SUM>(r);
       }
-    };
-    float4 v[QUADS], next[QUADS];
-    if (p.q0 < p.q1) read(p.q0, v);
-    for (uint32_t q = p.q0; q < p.q1; q += 2 * HALF) {
-      if (q + HALF < p.q1) read(q + HALF, next);
-      write(q, v);
-      if (q + 2 * HALF < p.q1) read(q + 2 * HALF, v);
-      if (q + HALF < p.q1) write(q + HALF, next);
+      if (threadIdx.x == 0) {
+        result[turn] = r;
+        arrive(&done[turn]);
+      }
+      if (PASS != DistillPass::Forward) {
+        const GradFactors f = grad_factors<SUM>(a, row, r, targets[turn].soft, targets[turn].index[a.top_n], c);
+        float* g = a.grad + row * a.ld_grad;
+        if (extra_at >= 0) g[extra_at] = grad_at<SUM>(f, extra, c);
+        // the same distance to a 16-byte boundary in both rows: 16-byte stores
+        const bool vec = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(x)) & 15u) == 0;
+        float4* gq = reinterpret_cast<float4*>(g + p.lead);
+        uint32_t q = p.q0;
+        do {
+          float4 v[QUADS];
+          if (PASS == DistillPass::Step && keep) take_stage<T, false, true>(p, q, ring, bars, start, w, v);
+          else take_stage<T, true, true>(p, q, ring, bars, at, w, v);
+          if (vec && q + kStage<T> <= p.q1) {
+#pragma unroll
+            for (uint32_t j = 0; j < QUADS; ++j) __stcs(gq + q + threadIdx.x + j * T, grad_quad<SUM>(f, v[j], c));
+          } else {
+#pragma unroll
+            for (uint32_t j = 0; j < QUADS; ++j) {
+              const uint32_t piece = q + j * T + threadIdx.x;
+              if (piece < p.q1) {
+                const float4 o = grad_quad<SUM>(f, v[j], c);
+                if (vec) {
+                  __stcs(gq + piece, o);
+                } else {
+                  float* out = g + p.lead + uint64_t(piece) * 4;
+                  out[0] = o.x;
+                  out[1] = o.y;
+                  out[2] = o.z;
+                  out[3] = o.w;
+                }
+              }
+            }
+          }
+          q += kStage<T>;
+        } while (q < p.q1);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        if (PASS != DistillPass::Forward) arrive(&written[turn]);
+        arrive(&tempty[turn]);
+      }
     }
-    __syncthreads();
-    take_targets<BLOCK>(a, g, targets, f, p.first, p.end);
   }
-  // no block leaves while another may still read its shared memory
-  if (PASS != DistillPass::Backward && shares > 1) ptx::cluster_sync_all();
+  __syncthreads();
+  wait_out(&abort_word);
+  // (a peer's last message has been waited for: nobody writes here any more)
 }
 
 // Short rows, one warp each.
 template <DistillPass PASS, Sum SUM, int PER>
-__global__ void __launch_bounds__(BLOCK) distill_warp_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(ROWS_BLOCK) distill_warp_kernel(const DistillArgs a) {
   ptx::grid_dependency_release();  // programmatic dependent launch: see launch.cuh
   ptx::grid_dependency_wait();
-  __shared__ Targets targets[WARPS];
+  __shared__ Targets targets[ROWS_BLOCK / 32];
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, vocab = uint32_t(a.vocab);
-  const uint64_t row = uint64_t(blockIdx.x) * WARPS + warp;
+  const uint64_t row = uint64_t(blockIdx.x) * (ROWS_BLOCK / 32) + warp;
   if (row >= a.rows) return;
   const float* x = a.x + row * a.ld;
   const float c = kLog2e / a.temperature;
@@ -979,7 +1230,7 @@ __global__ void __launch_bounds__(BLOCK) distill_warp_kernel(const DistillArgs a
     r = stats_of<SUM, PER>(v, c);
     complete<SUM>(r);
   }
-  read_targets(a, row, x, true, targets[warp]);
+  read_targets<PASS != DistillPass::Backward>(a, row, x, true, targets[warp]);
   if (PASS != DistillPass::Backward) {
     const float loss = row_loss(a, r, targets[warp]);
     if (lane == 0) {
@@ -997,17 +1248,50 @@ __global__ void __launch_bounds__(BLOCK) distill_warp_kernel(const DistillArgs a
       if (i < vocab) g[i] = grad_at<SUM>(f, v[j], c);
     }
     __syncwarp();
-    take_targets<32>(a, g, targets[warp], f, 0, vocab);
+    take_targets(a, g, targets[warp], f, 0, vocab);
   }
 }
 
 // ---- host side -----------------------------------------------------------------------------
-// Blocks per row: enough that few rows still fill the GPU twice over, each with at least 4096
-// logits.
+// Blocks per row: few rows are shared so that the GPU is full, each block with at least 4096 logits.
 uint32_t shares_for(uint64_t rows, uint64_t vocab, int sm_count) {
   uint32_t n = 1;
   while (n < MAX_SHARE && rows * n * 2 <= uint64_t(sm_count) * 2 && vocab / (n * 2) >= 4096) n *= 2;
   return n;
+}
+uint32_t rows_grid(uint64_t rows) { return uint32_t((rows + ROWS_BLOCK / 32 - 1) / (ROWS_BLOCK / 32)); }
+
+// A ring kernel's clusters of `shares` blocks each take every so-many-th row.  As many as run at
+// once (a cluster lies within one GPC, so that is fewer than the SMs would hold: 33 clusters of 4
+// instead of 37 at one block an SM, and a 34th would start when the first are done), and no more
+// than it takes for all of them to get the same number of rows.
+template <auto KERN, int T>
+cudaError_t launch_ring(uint64_t rows, uint32_t shares, cudaStream_t stream, auto... args) {
+  constexpr size_t smem = size_t(kStages<T>) * kStage<T> * 16;
+  static int fit[64][MAX_SHARE + 1] = {};  // per kernel and device: clusters that run at once
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int& at_once = fit[dev & 63][shares];
+  if (!at_once) {
+    cudaError_t e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(shares);
+    cfg.blockDim = dim3(T + 64);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = shares;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, KERN, &cfg);
+    if (e != cudaSuccess) return e;
+    if (n < 1) return cudaErrorInvalidConfiguration;
+    at_once = n;
+  }
+  const uint64_t rounds = (rows + at_once - 1) / at_once, clusters = (rows + rounds - 1) / rounds;
+  return launch_kernel_cluster(KERN, shares, dim3(uint32_t(clusters) * shares), dim3(T + 64), smem, stream, args...);
 }
 
 template <DistillPass PASS, Sum SUM>
@@ -1017,29 +1301,18 @@ cudaError_t launch_distill_sum(const DistillArgs& a, int sm_count, cudaStream_t 
                 : a.vocab <= 128 ? distill_warp_kernel<PASS, SUM, 4>
                 : a.vocab <= 512 ? distill_warp_kernel<PASS, SUM, 16>
                                  : distill_warp_kernel<PASS, SUM, 32>;
-    return launch_kernel(kern, dim3(uint32_t((a.rows + WARPS - 1) / WARPS)), dim3(BLOCK), 0, stream, a);
+    return launch_kernel(kern, dim3(rows_grid(a.rows)), dim3(ROWS_BLOCK), 0, stream, a);
   }
   uint32_t shares = shares_for(a.rows, a.vocab, sm_count);
-  size_t smem = 0;
-  constexpr auto kern = distill_block_kernel<PASS, SUM>;
-  if (PASS == DistillPass::Step) {
-    // parts of at most 64 KB (three blocks an SM) where 8 blocks allow that, of 220 KB where not
-    constexpr size_t GOOD = 64 << 10, MOST = 220 << 10;
-    auto bytes = [&](uint32_t n) { return (a.vocab / 4 / n + 1) * 16; };
-    while (shares < MAX_SHARE && bytes(shares) > GOOD) shares *= 2;
-    smem = bytes(shares) <= MOST ? bytes(shares) : 0;
-    static bool done[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (smem && !done[dev & 63]) {
-      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(MOST));
-      if (e != cudaSuccess) return e;
-      done[dev & 63] = true;
-    }
-  }
-  if (a.rows * shares > 0x7fffffffull) return cudaErrorInvalidValue;
-  return launch_kernel_cluster(kern, shares, dim3(uint32_t(a.rows * shares)), dim3(BLOCK), smem, stream, a, shares,
-                               smem != 0);
+  constexpr int T = kAdders<PASS>;
+  if (PASS != DistillPass::Step)
+    return launch_ring<distill_ring_kernel<PASS, SUM>, T>(a.rows, shares, stream, a, shares, false);
+  // a part takes at most 4 of the 6 stages, so that loads run while it is kept, or all of them where
+  // 8 blocks are not enough for that
+  auto part_stages = [&](uint32_t n) { return (a.vocab / 4 / n + 1 + kStage<T> - 1) / kStage<T>; };
+  while (shares < MAX_SHARE && part_stages(shares) > 4) shares *= 2;
+  const bool keep = part_stages(shares) <= kStages<T>;
+  return launch_ring<distill_ring_kernel<PASS, SUM>, T>(a.rows, shares, stream, a, shares, keep);
 }
 
 template <DistillPass PASS>
@@ -1062,11 +1335,11 @@ cudaError_t launch_token_logprobs(const LogprobArgs& a, int sm_count, cudaStream
                 : a.vocab <= 128 ? logprobs_warp_kernel<4>
                 : a.vocab <= 512 ? logprobs_warp_kernel<16>
                                  : logprobs_warp_kernel<32>;
-    return launch_kernel(kern, dim3(uint32_t((a.rows + WARPS - 1) / WARPS)), dim3(BLOCK), 0, stream, a);
+    return launch_kernel(kern, dim3(rows_grid(a.rows)), dim3(ROWS_BLOCK), 0, stream, a);
   }
   const uint32_t shares = shares_for(a.rows, a.vocab, sm_count);
-  return launch_kernel_cluster(a.top_n ? logprobs_block_kernel<true> : logprobs_block_kernel<false>, shares,
-                               dim3(uint32_t(a.rows * shares)), dim3(BLOCK), 0, stream, a, shares);
+  return a.top_n ? launch_ring<logprobs_ring_kernel<true>, BLOCK>(a.rows, shares, stream, a, shares)
+                 : launch_ring<logprobs_ring_kernel<false>, BLOCK>(a.rows, shares, stream, a, shares);
 }
 
 cudaError_t launch_distill(DistillPass pass, const DistillArgs& a, int sm_count, cudaStream_t stream) {

@@ -80,16 +80,6 @@ __device__ __forceinline__ uint64_t code_desc(uint32_t addr) {
   return ptx::smem_desc(2, 16, 1024) | uint64_t(addr >> 4);
 }
 
-__device__ __forceinline__ void wait_out(volatile uint32_t* abort_flag) {
-  if (!*abort_flag) return;
-  // a role gave up: give copies and MMAs in flight time to land
-  const uint64_t t0 = ptx::globaltimer_ns();
-  for (uint32_t i = 0; i < (1u << 16); ++i) {
-    if (ptx::globaltimer_ns() - t0 > 2000000ull) break;
-    __nanosleep(1000);
-  }
-}
-
 // ---- one CTA per tile of 128 outputs x BN batch rows, or a cluster that shares its K ------
 // Warp 0 loads, warp 1 issues the MMAs, warps 2-5 read the accumulators out.  A product with few
 // tiles gives each tile to a cluster of up to 8 CTAs: each multiplies its share of K, leaves its

@@ -1,6 +1,7 @@
 // How a kernel that gave up a bounded wait says so.
 #pragma once
 #include "kernels.h"
+#include "ptx.cuh"
 
 namespace gonn {
 namespace {
@@ -23,6 +24,17 @@ __device__ __forceinline__ void report(GemmStatus* st, uint32_t code, uint32_t w
     v->tile = tile;
     v->kblock = kb;
     v->code = code;
+  }
+}
+
+// Before a block whose waits may have run out leaves.
+__device__ __forceinline__ void wait_out(volatile uint32_t* abort_flag) {
+  if (!*abort_flag) return;
+  // a role gave up: give copies and MMAs in flight time to land
+  const uint64_t t0 = ptx::globaltimer_ns();
+  for (uint32_t i = 0; i < (1u << 16); ++i) {
+    if (ptx::globaltimer_ns() - t0 > 2000000ull) break;
+    __nanosleep(1000);
   }
 }
 
