@@ -87,8 +87,10 @@ __device__ __forceinline__ uint32_t adders_count(bool v) {
 
 // ---- statistics of (part of) a row ------------------------------------------------------
 // What is summed beside S: nothing; U for the entropy; or the tempered sum e^((x-m)/T), with
-// `c` = log2(e) / T.
-enum class Sum : int { Plain = 0, Entropy = 1, Tempered = 2 };
+// `c` = log2(e) / T.  With T = 2 or 4, e^(x-m) is the tempered exponential squared once or twice: one
+// exponential an element instead of two, of which an SM does 16 a clock.
+enum class Sum : int { Plain = 0, Entropy = 1, Tempered = 2, Tempered2 = 3, Tempered4 = 4 };
+__host__ __device__ constexpr bool tempered(Sum s) { return s == Sum::Tempered || s == Sum::Tempered2 || s == Sum::Tempered4; }
 
 struct RowStats {
   float m = -INFINITY;
@@ -109,7 +111,7 @@ __device__ __forceinline__ void rescale(RowStats& r, float m_new, float c) {
     const float f = exp2f(d * (SUM == Sum::Plain ? c : kLog2e));
     // where f is 0 the limit keeps d S finite (the difference itself may be -inf)
     if (SUM == Sum::Entropy) r.u = f * (r.u + fmaxf(d, -1e4f) * r.s);
-    if (SUM == Sum::Tempered) r.u *= exp2f(d * c);
+    if (tempered(SUM)) r.u *= exp2f(d * c);
     r.s *= f;
   }
   r.m = m_new;
@@ -122,7 +124,7 @@ __device__ __forceinline__ void add(RowStats& r, float x, float ref, float c) {
   r.s += e;
   // a masked element (-inf) adds e = 0 times a finite number
   if (SUM == Sum::Entropy) r.u = fmaf(e, fmaxf(d, -1e30f), r.u);
-  if (SUM == Sum::Tempered) r.u += exp2_ftz(d * c);
+  if (tempered(SUM)) r.u += exp2_ftz(d * c);
 }
 
 template <Sum SUM>
@@ -145,32 +147,33 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// The statistics of the block in every thread: the maximum first, then the sums relative to it, in
-// a fixed order.
+// Orders like the values (NaN aside); -0 counts as 0.
+__device__ __forceinline__ uint32_t order_bits(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float order_value(uint32_t b) {
+  return __uint_as_float((b & 0x80000000u) ? b & 0x7fffffffu : ~b);
+}
+
+// The statistics of the adding threads in every one of them, with one barrier: each warp's, then
+// all warps' in every warp.  `smem`: another one for every other row, so that the next row's may be
+// written while this one's are read.
 template <Sum SUM, int T>
-__device__ RowStats block_merge(RowStats r, float c, float (*smem)[T / 32]) {
-  constexpr int WARPS = T / 32;
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float mine = warp_max(r.m);
-  if (lane == 0) smem[0][warp] = mine;
+__device__ RowStats block_merge(RowStats r, float c, RowStats (&smem)[T / 32]) {
+  constexpr uint32_t WARPS = T / 32;
+  const uint32_t lane = threadIdx.x & 31;
+  rescale<SUM>(r, order_value(__reduce_max_sync(0xffffffffu, order_bits(r.m))), c);
+  r.s = warp_sum(r.s);
+  if (SUM != Sum::Plain) r.u = warp_sum(r.u);
+  if (lane == 0) smem[threadIdx.x >> 5] = r;
   adders_sync<T>();
-  float m = smem[0][0];
+  r = smem[lane % WARPS];
+  rescale<SUM>(r, order_value(__reduce_max_sync(0xffffffffu, order_bits(r.m))), c);
 #pragma unroll
-  for (int w = 1; w < WARPS; ++w) m = fmaxf(m, smem[0][w]);
-  rescale<SUM>(r, m, c);
-  const float s = warp_sum(r.s), u = SUM == Sum::Plain ? 0.f : warp_sum(r.u);
-  if (lane == 0) {
-    smem[1][warp] = s;
-    smem[2][warp] = u;
-  }
-  adders_sync<T>();
-  r.m = m;
-  r.s = smem[1][0];
-  r.u = smem[2][0];
-#pragma unroll
-  for (int w = 1; w < WARPS; ++w) {
-    r.s += smem[1][w];
-    r.u += smem[2][w];
+  for (uint32_t o = WARPS / 2; o > 0; o >>= 1) {
+    r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+    if (SUM != Sum::Plain) r.u += __shfl_xor_sync(0xffffffffu, r.u, o);
   }
   return r;
 }
@@ -282,13 +285,10 @@ __device__ __forceinline__ void feed_part(const Part& p, float4* ring, RingBars<
   } while (q < p.q1);
 }
 
-// A thread's logits of the stage that holds the pieces from `q`; -inf past the part's end.  WAIT:
-// the stage may not have arrived; LEAVE: it is not needed any more.
-template <int T, bool WAIT, bool LEAVE>
-__device__ __forceinline__ void take_stage(const Part& p, uint32_t q, const float4* ring, RingBars<T>& bars,
-                                           RingAt<T>& at, const Waits& w, float4 (&v)[QUADS]) {
-  if (WAIT) w.wait(&bars.full[at.slot], at.phase, at.slot);
-  const float4* from = ring + at.slot * kStage<T> + threadIdx.x;
+// A thread's logits of the stage that holds the pieces from `q`; -inf past the part's end.
+template <int T>
+__device__ __forceinline__ void read_stage(const Part& p, uint32_t q, const float4* stage, float4 (&v)[QUADS]) {
+  const float4* from = stage + threadIdx.x;
   if (q + kStage<T> <= p.q1) {
 #pragma unroll
     for (uint32_t j = 0; j < QUADS; ++j) v[j] = from[j * T];
@@ -296,11 +296,18 @@ __device__ __forceinline__ void take_stage(const Part& p, uint32_t q, const floa
 #pragma unroll
     for (uint32_t j = 0; j < QUADS; ++j) v[j] = q + j * T + threadIdx.x < p.q1 ? from[j * T] : masked_quad();
   }
-  if (LEAVE) {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) arrive(&bars.empty[at.slot]);
-  }
-  at.next();
+}
+template <int T>
+__device__ __forceinline__ void take_stage(const Part& p, uint32_t q, const float4* ring, RingBars<T>& bars,
+                                           const RingAt<T>& at, const Waits& w, float4 (&v)[QUADS]) {
+  w.wait(&bars.full[at.slot], at.phase, at.slot);
+  read_stage<T>(p, q, ring + at.slot * kStage<T>, v);
+}
+// The warp does not need the stage any more.
+template <int T>
+__device__ __forceinline__ void leave_stage(RingBars<T>& bars, const RingAt<T>& at) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) arrive(&bars.empty[at.slot]);
 }
 
 __device__ __forceinline__ float max4(const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
@@ -337,7 +344,7 @@ struct Stream {
         u.x = f * (u.x + by * s.x);
         u.y = f * (u.y + by * s.y);
       }
-      if (SUM == Sum::Tempered) {
+      if (tempered(SUM)) {
         const float ft = exp2f(dt);
         u.x *= ft;
         u.y *= ft;
@@ -351,42 +358,48 @@ struct Stream {
     far = far_new;
   }
 
-  __device__ __forceinline__ void add_pair(float x, float y, float c) {
-    const float k = scale(c);
-    float2 t;
-    if (far) t = make_float2((x - m) * k, (y - m) * k);
-    else t = ptx::fma2(make_float2(x, y), make_float2(k, k), make_float2(-b, -b));
+  // The exponent of scale `by` (whose b is `off`) of two elements.
+  __device__ __forceinline__ float2 exponent(float x, float y, float by, float off) const {
+    if (far) return make_float2((x - m) * by, (y - m) * by);
+    return ptx::fma2(make_float2(x, y), make_float2(by, by), make_float2(-off, -off));
+  }
+  // Adds two elements; returns their tempered exponentials (Plain, Entropy: those of S).
+  __device__ __forceinline__ float2 add_pair(float x, float y, float c) {
+    if (SUM == Sum::Tempered2 || SUM == Sum::Tempered4) {
+      const float2 t = exponent(x, y, c, bt);
+      const float2 e = make_float2(exp2_ftz(t.x), exp2_ftz(t.y));
+      u = ptx::add2(u, e);
+      if (SUM == Sum::Tempered2) {
+        s = ptx::fma2(e, e, s);
+      } else {
+        const float2 sq = make_float2(e.x * e.x, e.y * e.y);
+        s = ptx::fma2(sq, sq, s);
+      }
+      return e;
+    }
+    const float2 t = exponent(x, y, scale(c), b);
     const float2 e = make_float2(exp2_ftz(t.x), exp2_ftz(t.y));
     s = ptx::add2(s, e);
     // a masked element (-inf) adds e = 0 times a finite number
     if (SUM == Sum::Entropy) u = ptx::fma2(e, make_float2(fmaxf(t.x, -1e30f), fmaxf(t.y, -1e30f)), u);
     if (SUM == Sum::Tempered) {
-      float2 w;
-      if (far) w = make_float2((x - m) * c, (y - m) * c);
-      else w = ptx::fma2(make_float2(x, y), make_float2(c, c), make_float2(-bt, -bt));
+      const float2 w = exponent(x, y, c, bt);
       u = ptx::add2(u, make_float2(exp2_ftz(w.x), exp2_ftz(w.y)));
     }
+    return e;
   }
 
-  // Adds a thread's logits of a stage; returns their maximum.
-  __device__ __forceinline__ float add(const float4 (&v)[QUADS], float c) {
+  // Adds a thread's logits of a stage and leaves their exponentials, relative to the maximum m as
+  // it is then, in their place.  Returns their maximum.
+  __device__ __forceinline__ float add(float4 (&v)[QUADS], float c) {
     float most = max4(v[0]);
 #pragma unroll
     for (uint32_t j = 1; j < QUADS; ++j) most = fmaxf(most, max4(v[j]));
     if (most > m) raise(most, c);
-    if (!far) {
 #pragma unroll
-      for (uint32_t j = 0; j < QUADS; ++j) {
-        add_pair(v[j].x, v[j].y, c);
-        add_pair(v[j].z, v[j].w, c);
-      }
-    } else {
-#pragma unroll 1
-      for (uint32_t j = 0; j < QUADS; ++j) {
-        const float4 f = j == 0 ? v[0] : j == 1 ? v[1] : j == 2 ? v[2] : v[3];
-        add_pair(f.x, f.y, c);
-        add_pair(f.z, f.w, c);
-      }
+    for (uint32_t j = 0; j < QUADS; ++j) {
+      const float2 a = add_pair(v[j].x, v[j].y, c), z = add_pair(v[j].z, v[j].w, c);
+      v[j] = make_float4(a.x, a.y, z.x, z.y);
     }
     return most;
   }
@@ -400,27 +413,18 @@ struct Stream {
     const float f = exp2f(-off);
     r.s = (s.x + s.y) * f;
     if (SUM == Sum::Entropy) r.u = ((u.x + u.y) - off * (s.x + s.y)) * f * 0.6931471805599453f;
-    if (SUM == Sum::Tempered) r.u = (u.x + u.y) * exp2f(-off_t);
+    if (tempered(SUM)) r.u = (u.x + u.y) * exp2f(-off_t);
     return r;
   }
 };
-static_assert(QUADS == 4, "Stream::add picks one of four");
 
 // ---- alternatives -------------------------------------------------------------------------
 // Orders like (value, lowest index first): larger keys come first among the alternatives.
-// -0 counts as 0.
-__device__ __forceinline__ uint32_t order_bits(float x) {
-  const uint32_t b = __float_as_uint(x + 0.f);
-  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
-}
 __device__ __forceinline__ uint64_t order_key(float x, uint32_t index) {
   return (uint64_t(order_bits(x)) << 32) | (0xffffffffu - index);
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu - uint32_t(key); }
-__device__ __forceinline__ float key_value(uint64_t key) {
-  const uint32_t b = uint32_t(key >> 32);
-  return __uint_as_float((b & 0x80000000u) ? b & 0x7fffffffu : ~b);
-}
+__device__ __forceinline__ float key_value(uint64_t key) { return order_value(uint32_t(key >> 32)); }
 constexpr uint32_t kMaskedBits = 0x007fffffu;  // order_bits(-inf); below it only NaN
 
 // The largest `want` keys a block has met.  A key is kept when it lies above a floor that is known
@@ -484,11 +488,11 @@ __device__ void keep_largest(Selection& s, uint32_t n, uint32_t want) {
   adders_sync<BLOCK>();
 }
 
-// The first floor from the threads' maxima: 20 bits of it.
+// The first floor from the threads' maxima: 17 bits of it.
 __device__ void first_floor(Selection& s, float most, uint32_t want) {
   const uint32_t bits = order_bits(most);
   uint32_t floor = 0;
-  for (int bit = 31; bit >= 12; --bit) {
+  for (int bit = 31; bit >= 15; --bit) {
     const uint32_t trial = floor | (1u << bit);
     const uint32_t above = adders_count<BLOCK>(bits >= trial);
     if (above >= want) floor = trial;
@@ -505,7 +509,8 @@ __device__ void first_floor(Selection& s, float most, uint32_t want) {
 __device__ __forceinline__ float floor_value(uint64_t floor) {
   return uint32_t(floor >> 32) <= kMaskedBits ? -INFINITY : key_value(floor);
 }
-constexpr uint32_t STEP = 2;  // stages between two offers to the selection: 8192 logits
+constexpr uint32_t STEP = 4;   // stages between two looks at how many keys there are
+constexpr uint32_t FIRST = 2;  // stages that the first floor is taken from
 // Which of a thread's 16 logits from piece `q` may lie above the floor, a bit each.
 __device__ __forceinline__ uint32_t above_floor(const Part& p, uint32_t q, const float4 (&v)[QUADS], float low) {
   uint32_t hits = 0;
@@ -518,47 +523,59 @@ __device__ __forceinline__ uint32_t above_floor(const Part& p, uint32_t q, const
   return hits;
 }
 
-// Offers a thread's logits of a whole step (STEP stages from piece `q`, the marked ones) and, with
-// `outside`, its logit `extra` outside the pieces to the selection.  All adding threads call it.
-__device__ __forceinline__ void offer(Selection& s, const float* x, const Part& p, uint32_t q, uint32_t hits,
-                                      bool outside, int extra, uint32_t want) {
-  uint64_t floor = s.floor;
-  const uint32_t limit = 2 * want + 64;
-  while (true) {
-    bool over = false;
-    uint32_t left = hits;
-    while (left | uint32_t(outside)) {
-      // few logits get here; their values are read again (from L1) rather than picked out of the
-      // registers
-      uint32_t index = uint32_t(extra), bit = 0;
-      if (left) {
-        bit = left & (0u - left);
-        const uint32_t i = 31u - uint32_t(__clz(int(bit)));
-        index = p.lead + (q + (i >> 2) * BLOCK + threadIdx.x) * 4u + (i & 3u);
-        left ^= bit;
-      } else {
-        outside = false;
-      }
-      const uint64_t key = order_key(x[index], index);
-      bool stored = true;
-      if (key >= floor) {
-        const uint32_t at = atomicAdd(&s.count, 1u);
-        over = over || at >= limit;
-        stored = at < Selection::CAP;
-        if (stored) s.key[at] = key;
-      }
-      if (stored) {
-        hits &= ~bit;
-      } else if (bit == 0) {
-        outside = true;
-        break;  // the buffer is full: nothing after this one fits either
-      }
-    }
-    if (!adders_or<BLOCK>(over)) return;
-    keep_largest(s, min(s.count, Selection::CAP), want);
-    floor = s.floor;
-    if (!adders_or<BLOCK>(hits != 0 || outside)) return;
+// What a thread could not store since the last look (`waiting`: a bit for each logit of the step,
+// `outside`: the one outside the pieces), and whether it saw the buffer fill up.
+struct Offer {
+  uint64_t waiting = 0;
+  bool outside = false, over = false;
+};
+
+// Stores a logit's key unless it lies below the floor; false when there is no room.
+__device__ __forceinline__ bool store_key(Selection& s, uint64_t floor, float x, uint32_t index, uint32_t want,
+                                          Offer& o) {
+  const uint64_t key = order_key(x, index);
+  if (key < floor) return true;
+  const uint32_t at = atomicAdd(&s.count, 1u);
+  o.over = o.over || at >= 2 * want + 64;
+  if (at >= Selection::CAP) return false;
+  s.key[at] = key;
+  return true;
+}
+
+// Offers the marked ones of a thread's logits of the k-th stage of a step, which is still in shared
+// memory.
+__device__ __forceinline__ void offer_stage(Selection& s, const Part& p, uint32_t q, uint32_t k, const float4* stage,
+                                            uint32_t hits, uint64_t floor, uint32_t want, Offer& o) {
+  while (hits) {
+    const uint32_t bit = hits & (0u - hits), i = 31u - uint32_t(__clz(int(bit)));
+    const uint32_t piece = (i >> 2) * BLOCK + threadIdx.x;
+    const float x = reinterpret_cast<const float*>(stage + piece)[i & 3u];
+    if (!store_key(s, floor, x, p.lead + (q + piece) * 4u + (i & 3u), want, o)) o.waiting |= uint64_t(bit) << (16 * k);
+    hits ^= bit;
   }
+}
+
+// The look after a step that began at piece `q`: throws out the surplus when there is one, and
+// stores what had found no room (from the row itself: that is rare).  All adding threads call it.
+__device__ __forceinline__ void settle(Selection& s, const float* x, const Part& p, uint32_t q, int extra,
+                                       uint32_t want, Offer& o) {
+  while (adders_or<BLOCK>(o.over)) {
+    keep_largest(s, min(s.count, Selection::CAP), want);
+    if (!adders_or<BLOCK>(o.waiting != 0 || o.outside)) break;
+    o.over = false;
+    const uint64_t floor = s.floor;
+    uint64_t again = o.waiting;
+    o.waiting = 0;
+    if (o.outside) o.outside = !store_key(s, floor, x[extra], uint32_t(extra), want, o);
+    while (again) {
+      const uint64_t bit = again & (0ull - again);
+      const uint32_t i = 63u - uint32_t(__clzll(static_cast<long long>(bit)));
+      const uint32_t index = p.lead + (q + (i >> 2) * BLOCK + threadIdx.x) * 4u + (i & 3u);
+      if (!store_key(s, floor, x[index], index, want, o)) o.waiting |= bit;
+      again ^= bit;
+    }
+  }
+  o = Offer{};
 }
 
 // Sorts the selection's keys: sorted[0 .. min(n, want)) in descending order.  Returns how many.
@@ -619,8 +636,7 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
   __shared__ RingBars<T> bars;
   __shared__ uint64_t ready[2], freed[2];  // a row's results: written by the adders, read by the server
   __shared__ uint32_t abort_word;
-  __shared__ float merged[3][WARPS];
-  __shared__ RowStats result[2];
+  __shared__ RowStats result[2], merged[2][WARPS];
   __shared__ uint64_t sorted[2][TOP ? kMaxTop : 1];
   __shared__ Selection sel;
   const uint32_t warp = threadIdx.x >> 5, rank = blockIdx.x % shares, vocab = uint32_t(a.vocab);
@@ -666,47 +682,60 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
       const int extra_at = extra_of(p);
       const float extra = extra_at >= 0 ? x[extra_at] : -INFINITY;
       Stream<Sum::Entropy> stream;
+      Offer mine;
       uint32_t q = p.q0;
-      do {
-        const bool first = q == p.q0;
-        const float low = TOP && !first ? floor_value(sel.floor) : INFINITY;
-        uint32_t hits = 0;
-        float most = first ? extra : -INFINITY;
-        float4 v[QUADS];
+      if (TOP) {  // the first stages stay until there is a floor
+        RingAt<T> again = at;
+        float most = extra;
+#pragma unroll 1
+        for (uint32_t k = 0; k < FIRST && (k == 0 || q + k * kStage<T> < p.q1); ++k) {
+          float4 v[QUADS];
+          take_stage<T>(p, q + k * kStage<T>, ring, bars, at, w, v);
+          most = fmaxf(most, stream.add(v, kLog2e));
+          at.next();
+        }
+        first_floor(sel, most, a.top_n);
+        const uint64_t floor = sel.floor;
+        const float low = floor_value(floor);
+        if (extra_at >= 0 && extra >= low)
+          mine.outside = !store_key(sel, floor, extra, uint32_t(extra_at), a.top_n, mine);
+#pragma unroll 1
+        for (uint32_t k = 0; k < FIRST && (k == 0 || q + k * kStage<T> < p.q1); ++k) {
+          const float4* stage = ring + again.slot * kStage<T>;
+          if (most >= low) {
+            float4 v[QUADS];
+            read_stage<T>(p, q + k * kStage<T>, stage, v);
+            const uint32_t hits = above_floor(p, q + k * kStage<T>, v, low);
+            offer_stage(sel, p, q + k * kStage<T>, k, stage, hits, floor, a.top_n, mine);
+          }
+          leave_stage<T>(bars, again);
+          again.next();
+        }
+        settle(sel, x, p, q, extra_at, a.top_n, mine);
+        q += FIRST * kStage<T>;
+      }
+      while (q < p.q1 || (!TOP && q == p.q0)) {
+        const uint64_t floor = TOP ? sel.floor : 0;
+        const float low = TOP ? floor_value(floor) : INFINITY;
 #pragma unroll 1
         for (uint32_t k = 0; k < STEP && (k == 0 || q + k * kStage<T> < p.q1); ++k) {
-          take_stage<T, true, true>(p, q + k * kStage<T>, ring, bars, at, w, v);
-          const float here = stream.add(v, kLog2e);
-          if (TOP) {
-            if (here >= low) hits |= above_floor(p, q + k * kStage<T>, v, low) << (16 * k);
-            most = fmaxf(most, here);
+          float4 v[QUADS];
+          take_stage<T>(p, q + k * kStage<T>, ring, bars, at, w, v);
+          if (stream.add(v, kLog2e) >= low && TOP) {
+            const float4* stage = ring + at.slot * kStage<T>;
+            read_stage<T>(p, q + k * kStage<T>, stage, v);
+            const uint32_t hits = above_floor(p, q + k * kStage<T>, v, low);
+            offer_stage(sel, p, q + k * kStage<T>, k, stage, hits, floor, a.top_n, mine);
           }
+          leave_stage<T>(bars, at);
+          at.next();
         }
-        if (TOP) {
-          bool outside = false;
-          if (first) {
-            first_floor(sel, most, a.top_n);
-            const float start = floor_value(sel.floor);
-            if (most >= start) {  // the first logits are read once more, from L2
-              outside = extra_at >= 0 && extra >= start;
-#pragma unroll 1
-              for (uint32_t k = 0; k < STEP; ++k) {
-#pragma unroll
-                for (uint32_t j = 0; j < QUADS; ++j) {
-                  const uint32_t piece = q + k * kStage<T> + j * T + threadIdx.x;
-                  v[j] = piece < p.q1 ? p.quads[piece] : masked_quad();
-                }
-                hits |= above_floor(p, q + k * kStage<T>, v, start) << (16 * k);
-              }
-            }
-          }
-          offer(sel, x, p, q, hits, outside, extra_at, a.top_n);
-        }
+        if (TOP) settle(sel, x, p, q, -1, a.top_n, mine);
         q += STEP * kStage<T>;
-      } while (q < p.q1);
+      }
       RowStats r = stream.result(kLog2e);
       add_one<Sum::Entropy>(r, extra, 0.f);
-      r = block_merge<Sum::Entropy, T>(r, 0.f, merged);
+      r = block_merge<Sum::Entropy, T>(r, 0.f, merged[i & 1]);
       w.wait(&freed[i & 1], ((i >> 1) & 1u) ^ 1u, 0x21u);
       uint32_t found = 0;
       if (TOP) found = sort_selection(sel, sorted[i & 1], a.top_n);
@@ -961,33 +990,63 @@ __device__ __forceinline__ GradFactors grad_factors(const DistillArgs& a, uint64
   f.soft = soft * scale * (a.soft_weight * a.temperature);
   f.hard = label >= 0 ? scale * (1.f - a.soft_weight) : 0.f;
   f.ks = soft == 0.f || a.soft_weight == 0.f ? 0.f : f.soft / r.u * exp2f(-off_t);
-  f.kh = label < 0 ? 0.f : f.hard / r.s * exp2f(-(SUM == Sum::Tempered ? off : off_t));
+  f.kh = label < 0 ? 0.f : f.hard / r.s * exp2f(-(tempered(SUM) ? off : off_t));
   if (SUM == Sum::Plain) f.ks += f.kh;
+  if (f.empty) f.ks = f.kh = 0.f;
   return f;
+}
+// e: the tempered exponentials of two elements, e1: those of T = 1 (Tempered alone).
+template <Sum SUM>
+__device__ __forceinline__ float2 grad_of(float ks, float kh, float2 e, float2 e1) {
+  float2 g = make_float2(e.x * ks, e.y * ks);
+  if (SUM == Sum::Tempered) g = ptx::fma2(e1, make_float2(kh, kh), g);
+  if (SUM == Sum::Tempered2) g = ptx::fma2(make_float2(e.x * e.x, e.y * e.y), make_float2(kh, kh), g);
+  if (SUM == Sum::Tempered4) {
+    const float2 sq = make_float2(e.x * e.x, e.y * e.y);
+    g = ptx::fma2(make_float2(sq.x * sq.x, sq.y * sq.y), make_float2(kh, kh), g);
+  }
+  return g;
 }
 // A probability below 2^-126 gives 0.
 template <Sum SUM>
 __device__ __forceinline__ float2 grad_pair(const GradFactors& f, float x, float y, float c) {
-  float2 t;
-  if (f.far) t = make_float2((x - f.m) * c, (y - f.m) * c);
-  else t = ptx::fma2(make_float2(x, y), make_float2(c, c), make_float2(-f.bt, -f.bt));
-  float2 g = make_float2(exp2_ftz(t.x) * f.ks, exp2_ftz(t.y) * f.ks);
-  if (SUM == Sum::Tempered) {
-    if (f.far) t = make_float2((x - f.m) * kLog2e, (y - f.m) * kLog2e);
-    else t = ptx::fma2(make_float2(x, y), make_float2(kLog2e, kLog2e), make_float2(-f.b, -f.b));
-    g = ptx::fma2(make_float2(exp2_ftz(t.x), exp2_ftz(t.y)), make_float2(f.kh, f.kh), g);
-  }
-  return g;
+  auto exponential = [&](float by, float off) {
+    float2 t;
+    if (f.far) t = make_float2((x - f.m) * by, (y - f.m) * by);
+    else t = ptx::fma2(make_float2(x, y), make_float2(by, by), make_float2(-off, -off));
+    return make_float2(exp2_ftz(t.x), exp2_ftz(t.y));
+  };
+  const float2 e = exponential(c, f.bt);
+  return grad_of<SUM>(f.ks, f.kh, e, SUM == Sum::Tempered ? exponential(kLog2e, f.b) : e);
 }
 template <Sum SUM>
 __device__ __forceinline__ float grad_at(const GradFactors& f, float x, float c) {
   return f.empty ? 0.f : grad_pair<SUM>(f, x, x, c).x;
 }
+// A thread's logits of a stage -> their gradients.
 template <Sum SUM>
-__device__ __forceinline__ float4 grad_quad(const GradFactors& f, const float4& v, float c) {
-  if (f.empty) return make_float4(0.f, 0.f, 0.f, 0.f);
-  const float2 a = grad_pair<SUM>(f, v.x, v.y, c), b = grad_pair<SUM>(f, v.z, v.w, c);
-  return make_float4(a.x, a.y, b.x, b.y);
+__device__ __forceinline__ void grad_stage(const GradFactors& f, float4 (&v)[QUADS], float c) {
+#pragma unroll
+  for (uint32_t j = 0; j < QUADS; ++j) {
+    const float2 a = grad_pair<SUM>(f, v[j].x, v[j].y, c), b = grad_pair<SUM>(f, v[j].z, v[j].w, c);
+    v[j] = f.empty ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(a.x, a.y, b.x, b.y);
+  }
+}
+// The same from the exponentials that Stream::add left when its maximum was m (<= the row's).
+template <Sum SUM>
+__device__ __forceinline__ void scale_stage(const GradFactors& f, float4 (&v)[QUADS], float m, float c) {
+  const float ref = reference(m);
+  const bool apart = f.far || !(fabsf(ref) < 1e37f);
+  // nothing but masked logits: the exponentials are 0 whatever the reference is
+  const float by = m == -INFINITY ? 0.f : 1.f;
+  const float ks = by * f.ks * (by == 0.f ? 0.f : exp2f(apart ? (ref - f.m) * c : ref * c - f.bt));
+  const float kh = by * f.kh * (by == 0.f ? 0.f : exp2f(apart ? (ref - f.m) * kLog2e : ref * kLog2e - f.b));
+#pragma unroll
+  for (uint32_t j = 0; j < QUADS; ++j) {
+    const float2 p = make_float2(v[j].x, v[j].y), q = make_float2(v[j].z, v[j].w);
+    const float2 a = grad_of<SUM>(ks, kh, p, p), b = grad_of<SUM>(ks, kh, q, q);
+    v[j] = make_float4(a.x, a.y, b.x, b.y);
+  }
 }
 
 // The places that the teacher and the label name, among [first, end): the first entry that names
@@ -1046,8 +1105,8 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
   __shared__ RingBars<T> bars;
   __shared__ uint64_t tfull[2], tempty[2], done[2], written[2], peers[2];
   __shared__ uint32_t abort_word;
-  __shared__ float merged[3][WARPS];
-  __shared__ RowStats result[2], parts[2][MAX_SHARE];
+  __shared__ RowStats result[2], merged[2][WARPS], parts[2][MAX_SHARE];
+  __shared__ float kept_at[PASS == DistillPass::Step ? kStages<T> : 1][PASS == DistillPass::Step ? T : 1];
   __shared__ Targets targets[2];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % shares;
   const uint32_t vocab = uint32_t(a.vocab);
@@ -1130,14 +1189,25 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
         uint32_t q = p.q0;
         do {
           float4 v[QUADS];
-          if (PASS == DistillPass::Step && keep) take_stage<T, true, false>(p, q, ring, bars, at, w, v);
-          else take_stage<T, true, true>(p, q, ring, bars, at, w, v);
+          take_stage<T>(p, q, ring, bars, at, w, v);
           stream.add(v, c);
+          if (PASS == DistillPass::Step && keep) {
+            if (SUM != Sum::Tempered) {
+              // the exponentials take the logits' place: the gradient has only to scale them
+              float4* to = ring + at.slot * kStage<T> + threadIdx.x;
+#pragma unroll
+              for (uint32_t j = 0; j < QUADS; ++j) to[j * T] = v[j];
+              kept_at[at.slot][threadIdx.x] = stream.m;
+            }
+          } else {
+            leave_stage<T>(bars, at);
+          }
+          at.next();
           q += kStage<T>;
         } while (q < p.q1);
         r = stream.result(c);
         add_one<SUM>(r, extra, c);
-        r = block_merge<SUM, T>(r, c, merged);
+        r = block_merge<SUM, T>(r, c, merged[turn]);
       }
       // From here on the targets have been read, in every block of the cluster once its
       // statistics have arrived: the row may be overwritten.  The wait also says that the server
@@ -1172,17 +1242,29 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
         uint32_t q = p.q0;
         do {
           float4 v[QUADS];
-          if (PASS == DistillPass::Step && keep) take_stage<T, false, true>(p, q, ring, bars, start, w, v);
-          else take_stage<T, true, true>(p, q, ring, bars, at, w, v);
+          if (PASS == DistillPass::Step && keep) {
+            read_stage<T>(p, q, ring + start.slot * kStage<T>, v);
+            if (SUM == Sum::Tempered) grad_stage<SUM>(f, v, c);
+            else scale_stage<SUM>(f, v, kept_at[start.slot][threadIdx.x], c);
+            // the exponentials were written here: they come before the copy that fills the stage next
+            if (SUM != Sum::Tempered) ptx::fence_proxy_async_smem();
+            leave_stage<T>(bars, start);
+            start.next();
+          } else {
+            take_stage<T>(p, q, ring, bars, at, w, v);
+            leave_stage<T>(bars, at);
+            at.next();
+            grad_stage<SUM>(f, v, c);
+          }
           if (vec && q + kStage<T> <= p.q1) {
 #pragma unroll
-            for (uint32_t j = 0; j < QUADS; ++j) __stcs(gq + q + threadIdx.x + j * T, grad_quad<SUM>(f, v[j], c));
+            for (uint32_t j = 0; j < QUADS; ++j) __stcs(gq + q + threadIdx.x + j * T, v[j]);
           } else {
 #pragma unroll
             for (uint32_t j = 0; j < QUADS; ++j) {
               const uint32_t piece = q + j * T + threadIdx.x;
               if (piece < p.q1) {
-                const float4 o = grad_quad<SUM>(f, v[j], c);
+                const float4 o = v[j];
                 if (vec) {
                   __stcs(gq + piece, o);
                 } else {
@@ -1262,9 +1344,9 @@ uint32_t shares_for(uint64_t rows, uint64_t vocab, int sm_count) {
 uint32_t rows_grid(uint64_t rows) { return uint32_t((rows + ROWS_BLOCK / 32 - 1) / (ROWS_BLOCK / 32)); }
 
 // A ring kernel's clusters of `shares` blocks each take every so-many-th row.  As many as run at
-// once (a cluster lies within one GPC, so that is fewer than the SMs would hold: 33 clusters of 4
-// instead of 37 at one block an SM, and a 34th would start when the first are done), and no more
-// than it takes for all of them to get the same number of rows.
+// once: a cluster lies within one GPC, so that is fewer than the SMs would hold, and one more would
+// start when the first are done (the step over 1024 x 128000 took 479 us with 37 clusters of 4 on
+// 148 SMs, 263 us with those that fit).
 template <auto KERN, int T>
 cudaError_t launch_ring(uint64_t rows, uint32_t shares, cudaStream_t stream, auto... args) {
   constexpr size_t smem = size_t(kStages<T>) * kStage<T> * 16;
@@ -1290,7 +1372,7 @@ cudaError_t launch_ring(uint64_t rows, uint32_t shares, cudaStream_t stream, aut
     if (n < 1) return cudaErrorInvalidConfiguration;
     at_once = n;
   }
-  const uint64_t rounds = (rows + at_once - 1) / at_once, clusters = (rows + rounds - 1) / rounds;
+  const uint64_t clusters = std::min<uint64_t>(rows, at_once);
   return launch_kernel_cluster(KERN, shares, dim3(uint32_t(clusters) * shares), dim3(T + 64), smem, stream, args...);
 }
 
@@ -1321,6 +1403,8 @@ cudaError_t launch_distill_pass(const DistillArgs& given, int sm_count, cudaStre
   const bool soft = a.soft_weight > 0.f, hard = a.soft_weight < 1.f;
   // the saved statistics hold both sums
   const bool both = (soft && hard) || (PASS == DistillPass::Forward && a.stats);
+  if (both && a.temperature == 2.f) return launch_distill_sum<PASS, Sum::Tempered2>(a, sm_count, stream);
+  if (both && a.temperature == 4.f) return launch_distill_sum<PASS, Sum::Tempered4>(a, sm_count, stream);
   if (both && a.temperature != 1.f) return launch_distill_sum<PASS, Sum::Tempered>(a, sm_count, stream);
   if (!soft && !both) a.temperature = 1.f;  // a loss of the labels alone has no temperature
   return launch_distill_sum<PASS, Sum::Plain>(a, sm_count, stream);
