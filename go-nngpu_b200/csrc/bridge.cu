@@ -2232,7 +2232,10 @@ int mxfp4_product(const char* what, GPUPtr aPtr, bool a_float, long m, GPUPtr bP
   p.act = act;
   p.act_param = act_param;
   void* scratch = nullptr;
-  if (a_float) {
+  if (a_float && gonn::mxfp4_takes_float(uint64_t(m))) {
+    p.a = nullptr;
+    p.a_float = a->dptr;
+  } else if (a_float) {
     if (pool_alloc(c->device, &scratch, la.bytes) != cudaSuccess) {
       cudaGetLastError();
       set_error(err, "%s: could not allocate the packed operand.", what);

@@ -18,6 +18,7 @@
 #include "activation.cuh"
 #include "kernels.h"
 #include "launch.cuh"
+#include "mxfp4.cuh"
 #include "ptx.cuh"
 #include "status.cuh"
 #include "tmap.h"
@@ -48,6 +49,9 @@ struct Params {
   const float* bias;
   int act;
   float act_param;
+  const float* x;         // the float32 matrix that a fused kernel quantises itself: [M, K]
+  uint32_t K;
+  uint32_t x_vec;         // its rows start on 16 bytes
   GemmStatus* status;
 };
 
@@ -82,11 +86,16 @@ __device__ __forceinline__ uint64_t code_desc(uint32_t addr) {
 
 // ---- one CTA per tile of 128 outputs x BN batch rows, or a cluster that shares its K ------
 // Warp 0 loads, warp 1 issues the MMAs, warps 2-5 read the accumulators out.  A product with few
-// tiles gives each tile to a cluster of up to 8 CTAs: each multiplies its share of K, leaves its
+// tiles gives each tile to a cluster of up to 4 CTAs: each multiplies its share of K, leaves its
 // sums in its shared memory, and then adds up every `splits`-th column over all of them, in the
 // order of the shares.
+//
+// FLOAT_A: A is still float32 and has at most 8 rows.  Warps 2-5, idle while the weights stream
+// by, quantise it stage by stage into the place where the tensor core looks for its codes and
+// scales: one launch instead of two.  (Every CTA does all of it, which is why it stops at 8 rows.)
 constexpr uint32_t SINGLE_THREADS = 192;
-constexpr uint32_t MAX_SPLITS = 8;  // the portable size of a cluster
+constexpr uint32_t FLOAT_ROWS = 8;
+constexpr uint32_t MAX_SPLITS = 4;
 
 template <int BN, int STAGES>
 struct SingleShape {
@@ -98,7 +107,50 @@ struct SingleShape {
   static_assert(STAGES * STAGE >= BN * ROWS * 4, "the stages hold the sums of a share");
 };
 
-template <int BN, int STAGES, int CLASS>
+// This lane's 8 floats of every row for the stage kb.
+__device__ __forceinline__ void load_floats(const Params& p, uint32_t lane, uint32_t kb, float (&v)[FLOAT_ROWS][8]) {
+  const uint32_t k = kb * 256u + lane * 8u;
+#pragma unroll
+  for (uint32_t m = 0; m < FLOAT_ROWS; ++m) {
+    if (m >= p.M) break;
+    const float* x = p.x + uint64_t(m) * p.K + k;
+    if (p.x_vec && k + 8 <= p.K) {
+      const float4 a = reinterpret_cast<const float4*>(x)[0], b = reinterpret_cast<const float4*>(x)[1];
+      v[m][0] = a.x; v[m][1] = a.y; v[m][2] = a.z; v[m][3] = a.w;
+      v[m][4] = b.x; v[m][5] = b.y; v[m][6] = b.z; v[m][7] = b.w;
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) v[m][j] = k + j < p.K ? x[j] : 0.f;
+    }
+  }
+}
+// Quantises them into a stage: the same codes and scales as launch_mxfp4_quantize, the codes at
+// their place in the 128-byte swizzle (16-byte chunks XOR-ed with the row).
+__device__ __forceinline__ void quantize_stage(const Params& p, uint32_t lane, const float (&v)[FLOAT_ROWS][8],
+                                               uint8_t* codes, uint8_t* scales) {
+#pragma unroll
+  for (uint32_t m = 0; m < FLOAT_ROWS; ++m) {
+    if (m >= p.M) break;  // the same for the whole warp
+    uint32_t amax = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[m][j]) & 0x7fffffffu);
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t byte = mxfp4::scale_byte(amax);
+    const float f = mxfp4::inverse_scale(byte);
+    uint32_t word = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) word |= mxfp4::encode2(v[m][2 * j] * f, v[m][2 * j + 1] * f) << (8 * j);
+    if (byte == mxfp4::kScaleNan) word = 0;
+    *reinterpret_cast<uint32_t*>(codes + m * STAGE_K_BYTES + (((lane >> 2) ^ (m & 7u)) << 4) + (lane & 3u) * 4) = word;
+    uint32_t four = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) four |= __shfl_sync(0xffffffffu, byte, (lane & 16u) + j * 4) << (8 * j);
+    if ((lane & 15u) == 0) *reinterpret_cast<uint32_t*>(scales + (lane >> 4) * SCALE_TILE + m * 16) = four;
+  }
+}
+
+template <int BN, int STAGES, int CLASS, bool FLOAT_A>
 __global__ void __launch_bounds__(SINGLE_THREADS)
 mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_constant__ CUtensorMap tm_row_scales,
                     const __grid_constant__ CUtensorMap tm_cols, const __grid_constant__ CUtensorMap tm_col_scales,
@@ -123,7 +175,7 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < STAGES; ++s) {
-      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(full_bar(s), FLOAT_A ? 2 : 1);  // the loader, and the quantising warp
       ptx::mbar_init(empty_bar(s), 1);
     }
     ptx::mbar_init(tfull_bar, 1);
@@ -135,8 +187,10 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
   if (warp == 0 && lane == 0) {
     ptx::prefetch_tmap(&tm_rows);
     ptx::prefetch_tmap(&tm_row_scales);
-    ptx::prefetch_tmap(&tm_cols);
-    ptx::prefetch_tmap(&tm_col_scales);
+    if (!FLOAT_A) {
+      ptx::prefetch_tmap(&tm_cols);
+      ptx::prefetch_tmap(&tm_col_scales);
+    }
   }
   if (warp == 1) {
     ptx::tmem_alloc(ptx::smem_u32(tmem_slot), S::TMEM);
@@ -158,14 +212,14 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
           break;
         }
         const uint32_t fb = full_bar(stage), dst = base + stage * S::STAGE;
-        ptx::mbar_arrive_expect_tx(fb, S::STAGE);
+        ptx::mbar_arrive_expect_tx(fb, FLOAT_A ? ROW_CODES + 2 * SCALE_TILE : S::STAGE);
         ptx::tma_load_2d(dst, &tm_rows, int32_t(kb * STAGE_K_BYTES), int32_t(tn * ROWS), fb);
-        ptx::tma_load_2d(dst + ROW_CODES, &tm_cols, int32_t(kb * STAGE_K_BYTES), int32_t(tm * BN), fb);
         const uint32_t scales = dst + ROW_CODES + S::COL_CODES;
         ptx::tma_load_3d(scales, &tm_row_scales, 0, int32_t(kb * 2), int32_t(tn), fb);
-        // a tile narrower than 128 is the only one along M
-        ptx::tma_load_3d(scales + 2 * SCALE_TILE, &tm_col_scales, 0, int32_t(kb * 2),
-                         BN == 128 ? int32_t(tm) : 0, fb);
+        if (!FLOAT_A) {
+          ptx::tma_load_2d(dst + ROW_CODES, &tm_cols, int32_t(kb * STAGE_K_BYTES), int32_t(tm * BN), fb);
+          ptx::tma_load_3d(scales + 2 * SCALE_TILE, &tm_col_scales, 0, int32_t(kb * 2), int32_t(tm * BN / 128), fb);
+        }
         if (++stage == STAGES) {
           stage = 0;
           phase ^= 1u;
@@ -177,6 +231,9 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
     // The whole warp runs the loop and one lane issues: what the instructions take stays in
     // uniform registers.
     constexpr uint32_t idesc0 = ptx::make_idesc_mxf4(ROWS, BN, 0), idesc1 = ptx::make_idesc_mxf4(ROWS, BN, 1);
+    // A column of TMEM holds the scales of 32 rows: where in its tile of 128 this tile's begin.  The
+    // address has to be even, which is why tiles of 32 rows come alone along M.
+    const uint32_t scale_column = tm * BN % 128 / 32;
     uint32_t stage = 0, phase = 0;
     for (uint32_t kb = kb0; kb < kb1; ++kb) {
       const uint32_t in_chunk = (kb - kb0) % CHUNK;
@@ -199,7 +256,7 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
         for (uint32_t k = 0; k < STEPS; ++k)
           if (k < steps)
             ptx::mma_mxf4<false>(tmem, da + k * 2, db + k * 2, (k & 1) ? idesc1 : idesc0, ts + (k >> 1) * 4,
-                                 ts + 8 + (k >> 1) * 4, (in_chunk || k) ? 1u : 0u);
+                                 ts + 8 + (k >> 1) * 4 + scale_column, (in_chunk || k) ? 1u : 0u);
         ptx::mma_commit(empty_bar(stage));
         if (in_chunk + 1 == CHUNK || kb + 1 == kb1) ptx::mma_commit(tfull_bar);
       }
@@ -218,7 +275,29 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
     const uint32_t chunks = (kb1 - kb0 + CHUNK - 1) / CHUNK;
     float sum[BN / 32][32];
     bool ok = true;
+    // each of the four warps quantises every fourth stage; the floats of its next one are on
+    // their way meanwhile
+    static_assert(CHUNK % 4 == 0, "a chunk is whole rounds of the warps");
+    const uint32_t turn = warp - 2;
+    float v[FLOAT_ROWS][8];
+    if (FLOAT_A && kb0 + turn < kb1) load_floats(p, lane, kb0 + turn, v);
     for (uint32_t ch = 0; ch < chunks; ++ch) {
+      if (FLOAT_A) {
+        // a chunk's stages first, then its sums: the MMAs of a chunk wait for nothing else
+        const uint32_t end = min(kb0 + (ch + 1) * CHUNK, kb1);
+        for (uint32_t kb = kb0 + ch * CHUNK + turn; kb < end; kb += 4) {
+          const uint32_t i = kb - kb0, qstage = i % STAGES;
+          if (!__all_sync(0xffffffffu, ptx::mbar_wait(empty_bar(qstage), (i / STAGES & 1u) ^ 1u, abort_flag))) {
+            if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 1, 0x200u | qstage, tile, kb);
+          }
+          uint8_t* codes = smem_raw + pad + qstage * S::STAGE + ROW_CODES;
+          quantize_stage(p, lane, v, codes, codes + S::COL_CODES + 2 * SCALE_TILE);
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(full_bar(qstage));
+          if (kb + 4 < kb1) load_floats(p, lane, kb + 4, v);
+        }
+      }
       ok = __all_sync(0xffffffffu, ptx::mbar_wait(tfull_bar, ch & 1u, abort_flag));
       if (!ok) {
         if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 3, 0, tile, ch);
@@ -532,14 +611,14 @@ bool allow_smem(uint32_t bytes) {
   return done[dev & 63];
 }
 
-template <int BN, int STAGES, int CLASS>
+template <int BN, int STAGES, int CLASS, bool FLOAT_A = false>
 const char* launch_single(const Mxfp4Product& q, const Mxfp4Layout& la, const Mxfp4Layout& lb, const Params& p,
                           cudaStream_t stream) {
-  CUtensorMap rows, row_scales, cols, col_scales;
-  if (!code_map(&rows, q.b, lb, ROWS) || !scale_map(&row_scales, q.b, lb, 1) || !code_map(&cols, q.a, la, BN) ||
-      !scale_map(&col_scales, q.a, la, 1))
+  CUtensorMap rows, row_scales, cols{}, col_scales{};
+  if (!code_map(&rows, q.b, lb, ROWS) || !scale_map(&row_scales, q.b, lb, 1) ||
+      (!FLOAT_A && (!code_map(&cols, q.a, la, BN) || !scale_map(&col_scales, q.a, la, 1))))
     return "cuTensorMapEncodeTiled failed";
-  constexpr auto kern = mxfp4_single_kernel<BN, STAGES, CLASS>;
+  constexpr auto kern = mxfp4_single_kernel<BN, STAGES, CLASS, FLOAT_A>;
   constexpr uint32_t smem = SingleShape<BN, STAGES>::SMEM;
   static_assert(smem <= SMEM_LIMIT, "shared memory");
   if (!allow_smem<kern>(smem)) return "cudaFuncSetAttribute(max dynamic shared memory) failed";
@@ -582,26 +661,40 @@ const char* launch_class(const Mxfp4Product& q, GemmStatus* status, int sm_count
   p.status = status;
   const uint64_t pair_tiles = ((q.N + 255) / 256) * ((q.M + 255) / 256);
   if (pair_tiles >= (1ull << 30)) return "too many tiles";
-  if (pair_tiles >= 64) {
+  // Few pair tiles leave SMs idle: 1024^3 (16 tiles) takes 8.0 us on pairs and 4.3 us on single CTAs,
+  // 512 x 4096 x 4096 (32) 11.9 and 9.5, 2048^3 (64) 9.8 and 12.5, 1024 x 4096 x 4096 (64) 12.2 and
+  // 17.7.  And up to 128 rows half of each pair tile would be empty.
+  if (q.M > 128 && pair_tiles >= 48) {
     p.tiles_n = uint32_t((q.N + 255) / 256);
     p.tiles_m = uint32_t((q.M + 255) / 256);
     p.num_tiles = uint32_t(pair_tiles);
     return launch_pair<CLASS>(q, la, lb, p, sm_count, stream);
   }
-  const uint32_t bn = q.M <= 32 ? 32 : q.M <= 64 ? 64 : 128;
+  // (tiles of 128 rows were slower than those of 64 at every size that comes here)
+  const uint32_t bn = q.M <= 32 ? 32 : 64;
   p.tiles_n = uint32_t((q.N + ROWS - 1) / ROWS);
   p.tiles_m = uint32_t((q.M + bn - 1) / bn);
   p.num_tiles = p.tiles_n * p.tiles_m;
-  // few tiles: share each one's K among the CTAs of a cluster
-  const uint32_t splits = std::min({std::max(1u, uint32_t(sm_count) / p.num_tiles), p.kblocks, MAX_SPLITS});
+  // Few tiles: share each one's K among the CTAs of a cluster, where that saves more than the 2 us
+  // (32 columns) or 4 us (64) that the exchange of the sums costs; a stage takes about 0.3 us.  1 x 4096
+  // x 4096: 7.4 us whole, 5.5 us in 4 shares, 12.3 us in 8; 256 x 4096 x 4096: 8.9 us whole, 10.4 us in 2.
+  const uint32_t least = bn == 32 ? 4 : 16;
+  const uint32_t splits = std::max(1u, std::min({uint32_t(sm_count) / p.num_tiles, p.kblocks / least, MAX_SPLITS}));
   p.kb_per_split = (p.kblocks + splits - 1) / splits;
   p.splits = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;
-  return bn == 32   ? launch_single<32, 6, CLASS>(q, la, lb, p, stream)
-         : bn == 64 ? launch_single<64, 4, CLASS>(q, la, lb, p, stream)
-                    : launch_single<128, 4, CLASS>(q, la, lb, p, stream);
+  if (q.a_float) {
+    p.x = q.a_float;
+    p.K = uint32_t(q.K);
+    p.x_vec = (q.K & 3) == 0 && (reinterpret_cast<uintptr_t>(q.a_float) & 15u) == 0;
+    return launch_single<32, 6, CLASS, true>(q, la, lb, p, stream);
+  }
+  return bn == 32 ? launch_single<32, 6, CLASS>(q, la, lb, p, stream)
+                  : launch_single<64, 4, CLASS>(q, la, lb, p, stream);
 }
 
 }  // namespace
+
+bool mxfp4_takes_float(uint64_t rows) { return rows <= FLOAT_ROWS; }
 
 const char* launch_mxfp4_product(const Mxfp4Product& q, GemmStatus* status, int sm_count, cudaStream_t stream) {
   if (q.act == ACT_RELU) return launch_class<RELU>(q, status, sm_count, stream);
