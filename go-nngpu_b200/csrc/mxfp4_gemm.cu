@@ -8,9 +8,10 @@
 // and its alignment, and a batch of a few rows wastes columns of a narrow tile and not rows of a
 // tall one.
 //
-// Shared memory holds stages of 256 of K: 128 bytes of codes per row, fetched by TMA with the
-// 128-byte swizzle, and the scales of 128 rows as two tiles of 512 bytes, which tcgen05.cp moves
-// into TMEM right before the MMAs that read them.  Each stage has its own place for scales in
+// Shared memory holds stages of two k blocks of 256: 128 bytes of codes per row and block, fetched by
+// TMA with the 128-byte swizzle (both blocks in one box where the rows are whole blocks: 256
+// contiguous bytes a row), and the scales of 128 rows as four tiles of 512 bytes, which tcgen05.cp
+// moves into TMEM right before the MMAs that read them.  Each stage has its own place for scales in
 // TMEM: it is written again only after the stage's barrier has seen the MMAs retire.
 #include <algorithm>
 #include <cstring>
@@ -28,23 +29,26 @@ namespace gonn {
 namespace {
 
 constexpr uint32_t ROWS = 128;                 // rows of B in a CTA's tile
-constexpr uint32_t STAGE_K_BYTES = 128;        // code bytes of a row in a stage: 256 of K
-constexpr uint32_t STEPS = 4;                  // MMAs (64 of K) a stage
-constexpr uint32_t ROW_CODES = ROWS * STAGE_K_BYTES;
+constexpr uint32_t BLOCK_BYTES = 128;          // code bytes of a row in a k block: 256 of K
+constexpr uint32_t SUB = 2;                    // k blocks a stage
+constexpr uint32_t STEPS = 4;                  // MMAs (64 of K) a k block
+constexpr uint32_t ROW_CODES = ROWS * BLOCK_BYTES;  // of one k block
 constexpr uint32_t SCALE_TILE = 512;           // scales of 128 rows x 128 of K
+constexpr uint32_t SCALES = 2 * SUB;           // scale tiles of 128 rows in a stage
 constexpr uint32_t SMEM_LIMIT = 227 * 1024;
 // The tensor core adds into its accumulators with truncation, so the error grows with the number
 // of MMAs: on blocks whose scales differ by 2^4 (one standard deviation) 1.8e-7 relative at K =
 // 4096, 6.0e-7 at 8192, 3.8e-6 at 16384, against 1.6e-7, 4.5e-7 and 1.2e-6 of float32 sums.  After
 // this many stages (4096 of K) the accumulators are therefore added to sums in registers, with
 // rounding to nearest, and start again.
-constexpr uint32_t CHUNK = 16;
+constexpr uint32_t CHUNK = 8;
 
 struct Params {
   uint32_t M, N;          // rows of A (columns of the tile), rows of B (rows of the tile)
   uint32_t tiles_n, tiles_m, num_tiles;
-  uint32_t kblocks, ksteps;          // stages and MMAs along K
-  uint32_t splits, kb_per_split;     // single-CTA kernel: CTAs (of one cluster) that share a tile's K
+  uint32_t kblocks, ksteps, stages;  // k blocks, MMAs and stages along K
+  uint32_t splits, per_split;        // single-CTA kernel: CTAs (of one cluster) that share a tile's K, stages each
+  uint32_t rows_grouped, cols_grouped;  // both k blocks of a stage come in one box
   float* c;
   const float* bias;
   int act;
@@ -84,6 +88,23 @@ __device__ __forceinline__ uint64_t code_desc(uint32_t addr) {
   return ptx::smem_desc(2, 16, 1024) | uint64_t(addr >> 4);
 }
 
+// The codes of one operand's tile for a stage.
+template <bool PAIR>
+__device__ __forceinline__ void load_codes(uint32_t dst, const CUtensorMap* m, uint32_t grouped, uint32_t stage,
+                                           uint32_t row, uint32_t tile_bytes, uint32_t bar) {
+  if (grouped) {
+    if (PAIR) ptx::tma_load_3d_pair(dst, m, 0, int32_t(row), int32_t(stage * SUB), bar);
+    else ptx::tma_load_3d(dst, m, 0, int32_t(row), int32_t(stage * SUB), bar);
+    return;
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < SUB; ++j) {
+    const int32_t k = int32_t((stage * SUB + j) * BLOCK_BYTES);
+    if (PAIR) ptx::tma_load_2d_pair(dst + j * tile_bytes, m, k, int32_t(row), bar);
+    else ptx::tma_load_2d(dst + j * tile_bytes, m, k, int32_t(row), bar);
+  }
+}
+
 // ---- one CTA per tile of 128 outputs x BN batch rows, or a cluster that shares its K ------
 // Warp 0 loads, warp 1 issues the MMAs, warps 2-5 read the accumulators out.  A product with few
 // tiles gives each tile to a cluster of up to 4 CTAs: each multiplies its share of K, leaves its
@@ -99,15 +120,18 @@ constexpr uint32_t MAX_SPLITS = 4;
 
 template <int BN, int STAGES>
 struct SingleShape {
-  static constexpr uint32_t COL_CODES = BN * STAGE_K_BYTES;
-  static constexpr uint32_t STAGE = ROW_CODES + COL_CODES + 4 * SCALE_TILE;
+  static constexpr uint32_t COL_CODES = BN * BLOCK_BYTES;
+  static constexpr uint32_t COLS_AT = SUB * ROW_CODES, ROW_SCALES_AT = COLS_AT + SUB * COL_CODES,
+                            COL_SCALES_AT = ROW_SCALES_AT + SCALES * SCALE_TILE,
+                            STAGE = COL_SCALES_AT + SCALES * SCALE_TILE;
   static constexpr uint32_t SMEM = STAGES * STAGE + 1024 + 256;
-  static constexpr uint32_t USED = BN + STAGES * 16;
+  static constexpr uint32_t STAGE_COLS = 2 * SCALES * 4;  // of TMEM, for scales
+  static constexpr uint32_t USED = BN + STAGES * STAGE_COLS;
   static constexpr uint32_t TMEM = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
   static_assert(STAGES * STAGE >= BN * ROWS * 4, "the stages hold the sums of a share");
 };
 
-// This lane's 8 floats of every row for the stage kb.
+// This lane's 8 floats of every row for the k block kb.
 __device__ __forceinline__ void load_floats(const Params& p, uint32_t lane, uint32_t kb, float (&v)[FLOAT_ROWS][8]) {
   const uint32_t k = kb * 256u + lane * 8u;
 #pragma unroll
@@ -124,9 +148,9 @@ __device__ __forceinline__ void load_floats(const Params& p, uint32_t lane, uint
     }
   }
 }
-// Quantises them into a stage: the same codes and scales as launch_mxfp4_quantize, the codes at
+// Quantises them into a stage's k block: the same codes and scales as launch_mxfp4_quantize, the codes at
 // their place in the 128-byte swizzle (16-byte chunks XOR-ed with the row).
-__device__ __forceinline__ void quantize_stage(const Params& p, uint32_t lane, const float (&v)[FLOAT_ROWS][8],
+__device__ __forceinline__ void quantize_block(const Params& p, uint32_t lane, const float (&v)[FLOAT_ROWS][8],
                                                uint8_t* codes, uint8_t* scales) {
 #pragma unroll
   for (uint32_t m = 0; m < FLOAT_ROWS; ++m) {
@@ -142,7 +166,7 @@ __device__ __forceinline__ void quantize_stage(const Params& p, uint32_t lane, c
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) word |= mxfp4::encode2(v[m][2 * j] * f, v[m][2 * j + 1] * f) << (8 * j);
     if (byte == mxfp4::kScaleNan) word = 0;
-    *reinterpret_cast<uint32_t*>(codes + m * STAGE_K_BYTES + (((lane >> 2) ^ (m & 7u)) << 4) + (lane & 3u) * 4) = word;
+    *reinterpret_cast<uint32_t*>(codes + m * BLOCK_BYTES + (((lane >> 2) ^ (m & 7u)) << 4) + (lane & 3u) * 4) = word;
     uint32_t four = 0;
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) four |= __shfl_sync(0xffffffffu, byte, (lane & 16u) + j * 4) << (8 * j);
@@ -171,11 +195,11 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tile = blockIdx.x / p.splits, split = blockIdx.x - tile * p.splits;
   const uint32_t tn = tile % p.tiles_n, tm = tile / p.tiles_n;
-  const uint32_t kb0 = split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.kblocks);
+  const uint32_t st0 = split * p.per_split, st1 = min(st0 + p.per_split, p.stages);
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < STAGES; ++s) {
-      ptx::mbar_init(full_bar(s), FLOAT_A ? 2 : 1);  // the loader, and the quantising warp
+      ptx::mbar_init(full_bar(s), FLOAT_A ? 1 + SUB : 1);  // the loader, and a quantising warp per k block
       ptx::mbar_init(empty_bar(s), 1);
     }
     ptx::mbar_init(tfull_bar, 1);
@@ -206,19 +230,18 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
   if (warp == 0) {
     if (lane == 0) {
       uint32_t stage = 0, phase = 0;
-      for (uint32_t kb = kb0; kb < kb1; ++kb) {
+      for (uint32_t st = st0; st < st1; ++st) {
         if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
-          if (first_to_give_up(abort_flag)) report(p.status, 1, stage, tile, kb);
+          if (first_to_give_up(abort_flag)) report(p.status, 1, stage, tile, st);
           break;
         }
         const uint32_t fb = full_bar(stage), dst = base + stage * S::STAGE;
-        ptx::mbar_arrive_expect_tx(fb, FLOAT_A ? ROW_CODES + 2 * SCALE_TILE : S::STAGE);
-        ptx::tma_load_2d(dst, &tm_rows, int32_t(kb * STAGE_K_BYTES), int32_t(tn * ROWS), fb);
-        const uint32_t scales = dst + ROW_CODES + S::COL_CODES;
-        ptx::tma_load_3d(scales, &tm_row_scales, 0, int32_t(kb * 2), int32_t(tn), fb);
+        ptx::mbar_arrive_expect_tx(fb, FLOAT_A ? SUB * ROW_CODES + SCALES * SCALE_TILE : S::STAGE);
+        load_codes<false>(dst, &tm_rows, p.rows_grouped, st, tn * ROWS, ROW_CODES, fb);
+        ptx::tma_load_3d(dst + S::ROW_SCALES_AT, &tm_row_scales, 0, int32_t(st * SCALES), int32_t(tn), fb);
         if (!FLOAT_A) {
-          ptx::tma_load_2d(dst + ROW_CODES, &tm_cols, int32_t(kb * STAGE_K_BYTES), int32_t(tm * BN), fb);
-          ptx::tma_load_3d(scales + 2 * SCALE_TILE, &tm_col_scales, 0, int32_t(kb * 2), int32_t(tm * BN / 128), fb);
+          load_codes<false>(dst + S::COLS_AT, &tm_cols, p.cols_grouped, st, tm * BN, S::COL_CODES, fb);
+          ptx::tma_load_3d(dst + S::COL_SCALES_AT, &tm_col_scales, 0, int32_t(st * SCALES), int32_t(tm * BN / 128), fb);
         }
         if (++stage == STAGES) {
           stage = 0;
@@ -235,30 +258,33 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
     // address has to be even, which is why tiles of 32 rows come alone along M.
     const uint32_t scale_column = tm * BN % 128 / 32;
     uint32_t stage = 0, phase = 0;
-    for (uint32_t kb = kb0; kb < kb1; ++kb) {
-      const uint32_t in_chunk = (kb - kb0) % CHUNK;
+    for (uint32_t st = st0; st < st1; ++st) {
+      const uint32_t in_chunk = (st - st0) % CHUNK;
       bool ok = true;
-      if (in_chunk == 0) ok = ptx::mbar_wait(tempty_bar, ((kb - kb0) / CHUNK & 1u) ^ 1u, abort_flag);
+      if (in_chunk == 0) ok = ptx::mbar_wait(tempty_bar, ((st - st0) / CHUNK & 1u) ^ 1u, abort_flag);
       ok = ok && ptx::mbar_wait(full_bar(stage), phase, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) {
-        if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 2, stage, tile, kb);
+        if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 2, stage, tile, st);
         break;
       }
       ptx::tc_fence_after();
-      const uint32_t src = base + stage * S::STAGE, scales = src + ROW_CODES + S::COL_CODES;
-      const uint32_t ts = tmem + BN + stage * 16;
-      const uint64_t da = code_desc(src), db = code_desc(src + ROW_CODES), ds = scale_desc(scales);
-      const uint32_t steps = min(STEPS, p.ksteps - kb * STEPS);
+      const uint32_t src = base + stage * S::STAGE;
+      const uint32_t ts = tmem + BN + stage * S::STAGE_COLS;
+      const uint64_t da = code_desc(src), db = code_desc(src + S::COLS_AT), ds = scale_desc(src + S::ROW_SCALES_AT);
+      const uint32_t steps = min(SUB * STEPS, p.ksteps - st * SUB * STEPS);
       if (ptx::elect_one()) {
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) ptx::tmem_cp_scales<false>(ts + j * 4, ds + j * (SCALE_TILE >> 4));
+        for (uint32_t j = 0; j < 2 * SCALES; ++j)  // the rows' tiles, then the columns'
+          ptx::tmem_cp_scales<false>(ts + j * 4, ds + j * (SCALE_TILE >> 4));
 #pragma unroll
-        for (uint32_t k = 0; k < STEPS; ++k)
+        for (uint32_t k = 0; k < SUB * STEPS; ++k)
           if (k < steps)
-            ptx::mma_mxf4<false>(tmem, da + k * 2, db + k * 2, (k & 1) ? idesc1 : idesc0, ts + (k >> 1) * 4,
-                                 ts + 8 + (k >> 1) * 4 + scale_column, (in_chunk || k) ? 1u : 0u);
+            ptx::mma_mxf4<false>(tmem, da + (k / STEPS) * (ROW_CODES >> 4) + (k % STEPS) * 2,
+                                 db + (k / STEPS) * (S::COL_CODES >> 4) + (k % STEPS) * 2, (k & 1) ? idesc1 : idesc0,
+                                 ts + (k >> 1) * 4, ts + SCALES * 4 + (k >> 1) * 4 + scale_column,
+                                 (in_chunk || k) ? 1u : 0u);
         ptx::mma_commit(empty_bar(stage));
-        if (in_chunk + 1 == CHUNK || kb + 1 == kb1) ptx::mma_commit(tfull_bar);
+        if (in_chunk + 1 == CHUNK || st + 1 == st1) ptx::mma_commit(tfull_bar);
       }
       __syncwarp();
       if (++stage == STAGES) {
@@ -272,30 +298,31 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
     const uint64_t n = uint64_t(tn) * ROWS + r;
     const uint32_t m0 = tm * BN, cols = min(uint32_t(BN), p.M - m0);
     const uint32_t taddr = tmem + ((quarter * 32u) << 16);
-    const uint32_t chunks = (kb1 - kb0 + CHUNK - 1) / CHUNK;
+    const uint32_t chunks = (st1 - st0 + CHUNK - 1) / CHUNK;
     float sum[BN / 32][32];
     bool ok = true;
-    // each of the four warps quantises every fourth stage; the floats of its next one are on
+    // each of the four warps quantises every fourth k block; the floats of its next one are on
     // their way meanwhile
-    static_assert(CHUNK % 4 == 0, "a chunk is whole rounds of the warps");
+    static_assert(CHUNK * SUB % 4 == 0, "a chunk is whole rounds of the warps");
     const uint32_t turn = warp - 2;
     float v[FLOAT_ROWS][8];
-    if (FLOAT_A && kb0 + turn < kb1) load_floats(p, lane, kb0 + turn, v);
+    if (FLOAT_A) load_floats(p, lane, st0 * SUB + turn, v);
     for (uint32_t ch = 0; ch < chunks; ++ch) {
       if (FLOAT_A) {
         // a chunk's stages first, then its sums: the MMAs of a chunk wait for nothing else
-        const uint32_t end = min(kb0 + (ch + 1) * CHUNK, kb1);
-        for (uint32_t kb = kb0 + ch * CHUNK + turn; kb < end; kb += 4) {
-          const uint32_t i = kb - kb0, qstage = i % STAGES;
-          if (!__all_sync(0xffffffffu, ptx::mbar_wait(empty_bar(qstage), (i / STAGES & 1u) ^ 1u, abort_flag))) {
-            if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 1, 0x200u | qstage, tile, kb);
+        const uint32_t end = min(st0 + (ch + 1) * CHUNK, st1) * SUB;
+        for (uint32_t kb = (st0 + ch * CHUNK) * SUB + turn; kb < end; kb += 4) {
+          const uint32_t i = kb / SUB - st0, stage = i % STAGES;
+          if (!__all_sync(0xffffffffu, ptx::mbar_wait(empty_bar(stage), (i / STAGES & 1u) ^ 1u, abort_flag))) {
+            if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 1, 0x200u | stage, tile, kb);
           }
-          uint8_t* codes = smem_raw + pad + qstage * S::STAGE + ROW_CODES;
-          quantize_stage(p, lane, v, codes, codes + S::COL_CODES + 2 * SCALE_TILE);
+          uint8_t* at = smem_raw + pad + stage * S::STAGE;  // (past the end of K: zeros)
+          quantize_block(p, lane, v, at + S::COLS_AT + kb % SUB * S::COL_CODES,
+                         at + S::COL_SCALES_AT + kb % SUB * 2 * SCALE_TILE);
           ptx::fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(full_bar(qstage));
-          if (kb + 4 < kb1) load_floats(p, lane, kb + 4, v);
+          if (lane == 0) ptx::mbar_arrive(full_bar(stage));
+          load_floats(p, lane, kb + 4, v);
         }
       }
       ok = __all_sync(0xffffffffu, ptx::mbar_wait(tfull_bar, ch & 1u, abort_flag));
@@ -386,10 +413,13 @@ mxfp4_single_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_co
 // MMAs wait only for the read, while its loads have been running all the time.
 constexpr uint32_t PAIR_THREADS = 320;
 constexpr uint32_t PAIR_COLS = 256;
-constexpr uint32_t PAIR_STAGE = 2 * ROW_CODES + 6 * SCALE_TILE;
-constexpr uint32_t PAIR_STAGES = 6;
+constexpr uint32_t PAIR_COLS_AT = SUB * ROW_CODES, PAIR_ROW_SCALES_AT = 2 * SUB * ROW_CODES,
+                   PAIR_COL_SCALES_AT = PAIR_ROW_SCALES_AT + SCALES * SCALE_TILE,
+                   PAIR_STAGE = PAIR_COL_SCALES_AT + 2 * SCALES * SCALE_TILE;
+constexpr uint32_t PAIR_STAGES = 3;
+constexpr uint32_t PAIR_STAGE_COLS = 3 * SCALES * 4;  // of TMEM, for scales
 constexpr uint32_t PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + 1024 + 256;
-static_assert(PAIR_SMEM <= SMEM_LIMIT && PAIR_COLS + PAIR_STAGES * 24 <= 512, "pair kernel resources");
+static_assert(PAIR_SMEM <= SMEM_LIMIT && PAIR_COLS + PAIR_STAGES * PAIR_STAGE_COLS <= 512, "pair kernel resources");
 
 __device__ __forceinline__ void pair_tile(const Params& p, uint32_t t, uint32_t& tn, uint32_t& tm) {
   // groups of 8 tiles of B sweep A together
@@ -457,20 +487,19 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_cons
       for (uint32_t t = pair; alive && t < p.num_tiles; t += pairs) {
         uint32_t tn, tm;
         pair_tile(p, t, tn, tm);
-        for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
+        for (uint32_t st = 0; st < p.stages; ++st) {
           if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u, abort_flag)) {
-            if (first_to_give_up(abort_flag)) report(p.status, 1, stage, t, kb);
+            if (first_to_give_up(abort_flag)) report(p.status, 1, stage, t, st);
             alive = false;
             break;
           }
           if (leader) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * PAIR_STAGE);
           const uint32_t fb = ptx::mapa_shared(full_bar(stage), 0), dst = base + stage * PAIR_STAGE;
-          ptx::tma_load_2d_pair(dst, &tm_rows, int32_t(kb * STAGE_K_BYTES), int32_t((tn * 2 + rank) * ROWS), fb);
-          ptx::tma_load_2d_pair(dst + ROW_CODES, &tm_cols, int32_t(kb * STAGE_K_BYTES),
-                                int32_t((tm * 2 + rank) * ROWS), fb);
-          const uint32_t scales = dst + 2 * ROW_CODES;
-          ptx::tma_load_3d_pair(scales, &tm_row_scales, 0, int32_t(kb * 2), int32_t(tn * 2 + rank), fb);
-          ptx::tma_load_3d_pair(scales + 2 * SCALE_TILE, &tm_col_scales, 0, int32_t(kb * 2), int32_t(tm * 2), fb);
+          load_codes<true>(dst, &tm_rows, p.rows_grouped, st, (tn * 2 + rank) * ROWS, ROW_CODES, fb);
+          load_codes<true>(dst + PAIR_COLS_AT, &tm_cols, p.cols_grouped, st, (tm * 2 + rank) * ROWS, ROW_CODES, fb);
+          ptx::tma_load_3d_pair(dst + PAIR_ROW_SCALES_AT, &tm_row_scales, 0, int32_t(st * SCALES),
+                                int32_t(tn * 2 + rank), fb);
+          ptx::tma_load_3d_pair(dst + PAIR_COL_SCALES_AT, &tm_col_scales, 0, int32_t(st * SCALES), int32_t(tm * 2), fb);
           if (++stage == PAIR_STAGES) {
             stage = 0;
             phase ^= 1u;
@@ -488,7 +517,7 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_cons
       bool alive = true;
       for (uint32_t t = pair; alive && t < p.num_tiles; t += pairs) {
         uint32_t in_chunk = 0;
-        for (uint32_t kb = 0; kb < p.kblocks; ++kb) {
+        for (uint32_t st = 0; st < p.stages; ++st) {
           bool ok = true;
           if (in_chunk == 0) {
             ok = ptx::mbar_wait(tempty_bar, drained, abort_flag);
@@ -496,31 +525,34 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_cons
           }
           ok = ok && ptx::mbar_wait(full_bar(stage), phase, abort_flag);
           if (!__all_sync(0xffffffffu, ok)) {
-            if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 2, stage, t, kb);
+            if (lane == 0 && first_to_give_up(abort_flag)) report(p.status, 2, stage, t, st);
             alive = false;
             break;
           }
           ptx::tc_fence_after();
           const uint32_t src = base + stage * PAIR_STAGE;
-          // per stage: 2 x 4 columns for the rows' scales, 2 x 8 for the columns' (128 + 128 rows)
-          const uint32_t ts = tmem + PAIR_COLS + stage * 24;
-          const uint64_t da = code_desc(src), db = code_desc(src + ROW_CODES), ds = scale_desc(src + 2 * ROW_CODES);
-          const uint32_t steps = min(STEPS, p.ksteps - kb * STEPS);
+          // per stage: 4 columns for each of the rows' four scale tiles, 8 (128 + 128 rows) for each
+          // of the columns' four
+          const uint32_t ts = tmem + PAIR_COLS + stage * PAIR_STAGE_COLS, tc = ts + SCALES * 4;
+          const uint64_t da = code_desc(src), db = code_desc(src + PAIR_COLS_AT),
+                         ds = scale_desc(src + PAIR_ROW_SCALES_AT), dc = scale_desc(src + PAIR_COL_SCALES_AT);
+          const uint32_t steps = min(SUB * STEPS, p.ksteps - st * SUB * STEPS);
           if (ptx::elect_one()) {
 #pragma unroll
-            for (uint32_t k = 0; k < 2; ++k) {
+            for (uint32_t k = 0; k < SCALES; ++k) {
               ptx::tmem_cp_scales<true>(ts + k * 4, ds + k * (SCALE_TILE >> 4));
 #pragma unroll
               for (uint32_t h = 0; h < 2; ++h)
-                ptx::tmem_cp_scales<true>(ts + 8 + k * 8 + h * 4, ds + (2 + h * 2 + k) * (SCALE_TILE >> 4));
+                ptx::tmem_cp_scales<true>(tc + k * 8 + h * 4, dc + (h * SCALES + k) * (SCALE_TILE >> 4));
             }
 #pragma unroll
-            for (uint32_t k = 0; k < STEPS; ++k)
+            for (uint32_t k = 0; k < SUB * STEPS; ++k)
               if (k < steps)
-                ptx::mma_mxf4<true>(tmem, da + k * 2, db + k * 2, (k & 1) ? idesc1 : idesc0, ts + (k >> 1) * 4,
-                                    ts + 8 + (k >> 1) * 8, (in_chunk || k) ? 1u : 0u);
+                ptx::mma_mxf4<true>(tmem, da + (k / STEPS) * (ROW_CODES >> 4) + (k % STEPS) * 2,
+                                    db + (k / STEPS) * (ROW_CODES >> 4) + (k % STEPS) * 2, (k & 1) ? idesc1 : idesc0,
+                                    ts + (k >> 1) * 4, tc + (k >> 1) * 8, (in_chunk || k) ? 1u : 0u);
             ptx::mma_commit_pair(empty_bar(stage), 3);
-            if (in_chunk + 1 == CHUNK || kb + 1 == p.kblocks) ptx::mma_commit_pair(tfull_bar, 3);
+            if (in_chunk + 1 == CHUNK || st + 1 == p.stages) ptx::mma_commit_pair(tfull_bar, 3);
           }
           __syncwarp();
           if (++in_chunk == CHUNK) in_chunk = 0;
@@ -534,7 +566,7 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_cons
   } else {
     const uint32_t quarter = warp & 3u, half = (warp - 2u) >> 2;
     const uint32_t taddr = tmem + ((quarter * 32u) << 16) + half * 128u;
-    const uint32_t chunks = (p.kblocks + CHUNK - 1) / CHUNK;
+    const uint32_t chunks = (p.stages + CHUNK - 1) / CHUNK;
     uint32_t filled = 0;
     for (uint32_t t = pair; t < p.num_tiles; t += pairs) {
       uint32_t tn, tm;
@@ -585,18 +617,28 @@ mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tm_rows, const __grid_cons
 }
 
 // ---- host side -----------------------------------------------------------------------
-// Codes as a byte matrix: boxes of 128 bytes x `box_rows` rows.
-bool code_map(CUtensorMap* map, const void* packed, const Mxfp4Layout& l, uint32_t box_rows) {
+// Codes as a byte matrix: boxes of 128 bytes x `box_rows` rows; or, for rows of whole k blocks, as
+// [k block, row, 128 bytes] with both k blocks of a stage in one box (*grouped).
+bool code_map(CUtensorMap* map, const void* packed, const Mxfp4Layout& l, uint32_t box_rows, uint32_t* grouped) {
+  *grouped = 0;
+  if (l.row_bytes % BLOCK_BYTES == 0) {
+    const uint64_t dims[3] = {BLOCK_BYTES, l.rows, l.row_bytes / BLOCK_BYTES}, strides[2] = {l.row_bytes, BLOCK_BYTES};
+    const uint32_t box[3] = {BLOCK_BYTES, box_rows, SUB};
+    // (the driver may refuse strides in this order)
+    *grouped = encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, packed, dims, strides, box,
+                                 CU_TENSOR_MAP_SWIZZLE_128B);
+    if (*grouped) return true;
+  }
   const uint64_t dims[2] = {l.row_bytes, l.rows}, strides[1] = {l.row_bytes};
-  const uint32_t box[2] = {STAGE_K_BYTES, box_rows};
+  const uint32_t box[2] = {BLOCK_BYTES, box_rows};
   return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, packed, dims, strides, box,
                            CU_TENSOR_MAP_SWIZZLE_128B);
 }
-// Scale tiles of 512 bytes: boxes of 2 along K x `tall` along the rows.
+// Scale tiles of 512 bytes: boxes of a stage's four along K x `tall` along the rows.
 bool scale_map(CUtensorMap* map, const void* packed, const Mxfp4Layout& l, uint32_t tall) {
   const uint64_t dims[3] = {SCALE_TILE / 4, l.groups, (l.rows + 127) / 128};
   const uint64_t strides[2] = {SCALE_TILE, l.groups * SCALE_TILE};
-  const uint32_t box[3] = {SCALE_TILE / 4, 2, tall};
+  const uint32_t box[3] = {SCALE_TILE / 4, SCALES, tall};
   return encode_tensor_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3,
                            static_cast<const uint8_t*>(packed) + l.scale_offset, dims, strides, box,
                            CU_TENSOR_MAP_SWIZZLE_NONE);
@@ -612,11 +654,11 @@ bool allow_smem(uint32_t bytes) {
 }
 
 template <int BN, int STAGES, int CLASS, bool FLOAT_A = false>
-const char* launch_single(const Mxfp4Product& q, const Mxfp4Layout& la, const Mxfp4Layout& lb, const Params& p,
+const char* launch_single(const Mxfp4Product& q, const Mxfp4Layout& la, const Mxfp4Layout& lb, Params p,
                           cudaStream_t stream) {
   CUtensorMap rows, row_scales, cols{}, col_scales{};
-  if (!code_map(&rows, q.b, lb, ROWS) || !scale_map(&row_scales, q.b, lb, 1) ||
-      (!FLOAT_A && (!code_map(&cols, q.a, la, BN) || !scale_map(&col_scales, q.a, la, 1))))
+  if (!code_map(&rows, q.b, lb, ROWS, &p.rows_grouped) || !scale_map(&row_scales, q.b, lb, 1) ||
+      (!FLOAT_A && (!code_map(&cols, q.a, la, BN, &p.cols_grouped) || !scale_map(&col_scales, q.a, la, 1))))
     return "cuTensorMapEncodeTiled failed";
   constexpr auto kern = mxfp4_single_kernel<BN, STAGES, CLASS, FLOAT_A>;
   constexpr uint32_t smem = SingleShape<BN, STAGES>::SMEM;
@@ -629,10 +671,11 @@ const char* launch_single(const Mxfp4Product& q, const Mxfp4Layout& la, const Mx
 }
 
 template <int CLASS>
-const char* launch_pair(const Mxfp4Product& q, const Mxfp4Layout& la, const Mxfp4Layout& lb, const Params& p,
+const char* launch_pair(const Mxfp4Product& q, const Mxfp4Layout& la, const Mxfp4Layout& lb, Params p,
                         int sm_count, cudaStream_t stream) {
   CUtensorMap rows, row_scales, cols, col_scales;
-  if (!code_map(&rows, q.b, lb, ROWS) || !scale_map(&row_scales, q.b, lb, 1) || !code_map(&cols, q.a, la, ROWS) ||
+  if (!code_map(&rows, q.b, lb, ROWS, &p.rows_grouped) || !scale_map(&row_scales, q.b, lb, 1) ||
+      !code_map(&cols, q.a, la, ROWS, &p.cols_grouped) ||
       !scale_map(&col_scales, q.a, la, 2))
     return "cuTensorMapEncodeTiled failed";
   constexpr auto kern = mxfp4_pair_kernel<CLASS>;
@@ -650,10 +693,11 @@ const char* launch_class(const Mxfp4Product& q, GemmStatus* status, int sm_count
   Params p{};
   p.M = uint32_t(q.M);
   p.N = uint32_t(q.N);
-  p.kblocks = uint32_t((lb.row_bytes + STAGE_K_BYTES - 1) / STAGE_K_BYTES);
+  p.kblocks = uint32_t((lb.row_bytes + BLOCK_BYTES - 1) / BLOCK_BYTES);
   p.ksteps = uint32_t((lb.blocks + 1) / 2);
+  p.stages = (p.kblocks + SUB - 1) / SUB;
   p.splits = 1;
-  p.kb_per_split = p.kblocks;
+  p.per_split = p.stages;
   p.c = q.c;
   p.bias = q.bias;
   p.act = q.act;
@@ -680,16 +724,16 @@ const char* launch_class(const Mxfp4Product& q, GemmStatus* status, int sm_count
   // x 4096: 7.4 us whole, 5.5 us in 4 shares, 12.3 us in 8; 256 x 4096 x 4096: 8.9 us whole, 10.4 us in 2.
   const uint32_t least = bn == 32 ? 4 : 16;
   const uint32_t splits = std::max(1u, std::min({uint32_t(sm_count) / p.num_tiles, p.kblocks / least, MAX_SPLITS}));
-  p.kb_per_split = (p.kblocks + splits - 1) / splits;
-  p.splits = (p.kblocks + p.kb_per_split - 1) / p.kb_per_split;
+  p.per_split = (p.stages + splits - 1) / splits;
+  p.splits = (p.stages + p.per_split - 1) / p.per_split;
   if (q.a_float) {
     p.x = q.a_float;
     p.K = uint32_t(q.K);
     p.x_vec = (q.K & 3) == 0 && (reinterpret_cast<uintptr_t>(q.a_float) & 15u) == 0;
-    return launch_single<32, 6, CLASS, true>(q, la, lb, p, stream);
+    return launch_single<32, 4, CLASS, true>(q, la, lb, p, stream);
   }
-  return bn == 32 ? launch_single<32, 6, CLASS>(q, la, lb, p, stream)
-                  : launch_single<64, 4, CLASS>(q, la, lb, p, stream);
+  return bn == 32 ? launch_single<32, 4, CLASS>(q, la, lb, p, stream)
+                  : launch_single<64, 2, CLASS>(q, la, lb, p, stream);
 }
 
 }  // namespace
