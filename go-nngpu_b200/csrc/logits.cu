@@ -322,14 +322,22 @@ __device__ __forceinline__ void add_one(RowStats& r, float x, float c) {
 // is one fused multiply-add, x c - b with b = m c rounded (the same b for all elements, so its
 // rounding is a common factor, which result() takes out again); logits beyond 1e37, where the
 // products could overflow, take the difference first (`far`).
+//
+// m is a reference and need not be the maximum: it is the largest logit of the warp's first stage,
+// and moves only when one comes whose exponential would be above 2^58 (the sums are then still far
+// from overflow).  With the reference at each thread's running maximum some lane of
+// a warp moved it at nearly every stage, which made a stage take 1400 clocks instead of 900.
 template <Sum SUM>
 struct Stream {
-  float m = -INFINITY, b = 0.f, bt = 0.f;
+  const float slack;
+  float m = -INFINITY, top = -INFINITY, b = 0.f, bt = 0.f;
   float2 s = make_float2(0.f, 0.f), u = make_float2(0.f, 0.f);
   bool far = false;
 
   // scale of S itself; Plain: log2(e) / T
   static __device__ __forceinline__ float scale(float c) { return SUM == Sum::Plain ? c : kLog2e; }
+
+  __device__ __forceinline__ explicit Stream(float c) : slack(58.f / (tempered(SUM) ? fmaxf(c, kLog2e) : scale(c))) {}
 
   __device__ __forceinline__ void raise(float most, float c) {
     const float k = scale(c), ref = reference(most);
@@ -389,13 +397,15 @@ struct Stream {
     return e;
   }
 
-  // Adds a thread's logits of a stage and leaves their exponentials, relative to the maximum m as
-  // it is then, in their place.  Returns their maximum.
+  // Adds a thread's logits of a stage and leaves their exponentials, relative to m as it is then, in
+  // their place.  Returns their maximum.
   __device__ __forceinline__ float add(float4 (&v)[QUADS], float c) {
     float most = max4(v[0]);
 #pragma unroll
     for (uint32_t j = 1; j < QUADS; ++j) most = fmaxf(most, max4(v[j]));
-    if (most > m) raise(most, c);
+    // (the whole warp moves together: its lanes hold logits of one row)
+    if (__any_sync(0xffffffffu, most > m + slack)) raise(fmaxf(m, order_value(__reduce_max_sync(0xffffffffu, order_bits(most)))), c);
+    top = fmaxf(top, most);
 #pragma unroll
     for (uint32_t j = 0; j < QUADS; ++j) {
       const float2 a = add_pair(v[j].x, v[j].y, c), z = add_pair(v[j].z, v[j].w, c);
@@ -414,6 +424,7 @@ struct Stream {
     r.s = (s.x + s.y) * f;
     if (SUM == Sum::Entropy) r.u = ((u.x + u.y) - off * (s.x + s.y)) * f * 0.6931471805599453f;
     if (tempered(SUM)) r.u = (u.x + u.y) * exp2f(-off_t);
+    rescale<SUM>(r, fmaxf(m, top), c);  // (m is one of the row's logits too)
     return r;
   }
 };
@@ -488,19 +499,33 @@ __device__ void keep_largest(Selection& s, uint32_t n, uint32_t want) {
   adders_sync<BLOCK>();
 }
 
-// The first floor from the threads' maxima: 17 bits of it.
-__device__ void first_floor(Selection& s, float most, uint32_t want) {
-  const uint32_t bits = order_bits(most);
-  uint32_t floor = 0;
-  for (int bit = 31; bit >= 15; --bit) {
-    const uint32_t trial = floor | (1u << bit);
-    const uint32_t above = adders_count<BLOCK>(bits >= trial);
-    if (above >= want) floor = trial;
-    if (above == want) break;
-  }
-  if (threadIdx.x == 0) {
-    s.floor = uint64_t(floor) << 32;
-    s.count = 0;
+// The first floor from the threads' maxima, 18 bits of it: one warp looks for the largest bound
+// with `want` maxima at or above it, two bits a round, with the three counts of a round in one
+// word.  (All threads counting together, a barrier a bit, took 2100 clocks of a row's 27000.)  `maxima`:
+// room for BLOCK words.
+__device__ void first_floor(Selection& s, uint32_t* maxima, float most, uint32_t want) {
+  maxima[threadIdx.x] = order_bits(most);
+  adders_sync<BLOCK>();
+  if (threadIdx.x < 32) {
+    uint32_t mine[BLOCK / 32];
+#pragma unroll
+    for (uint32_t i = 0; i < BLOCK / 32; ++i) mine[i] = maxima[i * 32 + threadIdx.x];
+    uint32_t floor = 0;
+    for (int bit = 30; bit >= 14; bit -= 2) {
+      uint32_t above = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < BLOCK / 32; ++i)
+#pragma unroll
+        for (uint32_t k = 0; k < 3; ++k) above += uint32_t(mine[i] >= (floor | ((k + 1) << bit))) << (10 * k);
+      above = __reduce_add_sync(0xffffffffu, above);
+      if ((above >> 20) >= want) floor |= 3u << bit;
+      else if ((above >> 10 & 1023u) >= want) floor |= 2u << bit;
+      else if ((above & 1023u) >= want) floor |= 1u << bit;
+    }
+    if (threadIdx.x == 0) {
+      s.floor = uint64_t(floor) << 32;
+      s.count = 0;
+    }
   }
   adders_sync<BLOCK>();
 }
@@ -509,7 +534,7 @@ __device__ void first_floor(Selection& s, float most, uint32_t want) {
 __device__ __forceinline__ float floor_value(uint64_t floor) {
   return uint32_t(floor >> 32) <= kMaskedBits ? -INFINITY : key_value(floor);
 }
-constexpr uint32_t STEP = 4;   // stages between two looks at how many keys there are
+constexpr uint32_t STEP = 16;  // stages between two looks at how many keys there are
 constexpr uint32_t FIRST = 2;  // stages that the first floor is taken from
 // Which of a thread's 16 logits from piece `q` may lie above the floor, a bit each.
 __device__ __forceinline__ uint32_t above_floor(const Part& p, uint32_t q, const float4 (&v)[QUADS], float low) {
@@ -523,10 +548,11 @@ __device__ __forceinline__ uint32_t above_floor(const Part& p, uint32_t q, const
   return hits;
 }
 
-// What a thread could not store since the last look (`waiting`: a bit for each logit of the step,
-// `outside`: the one outside the pieces), and whether it saw the buffer fill up.
+// Where a thread stands since the last look: the first of its logits of the step that found no room
+// (`left`, 16 to a stage; the count only grows between two looks, so none after it did either),
+// whether that is so of the logit outside the pieces, and whether it saw the buffer fill up.
 struct Offer {
-  uint64_t waiting = 0;
+  uint32_t left = 0xffffffffu;
   bool outside = false, over = false;
 };
 
@@ -546,33 +572,38 @@ __device__ __forceinline__ bool store_key(Selection& s, uint64_t floor, float x,
 // memory.
 __device__ __forceinline__ void offer_stage(Selection& s, const Part& p, uint32_t q, uint32_t k, const float4* stage,
                                             uint32_t hits, uint64_t floor, uint32_t want, Offer& o) {
-  while (hits) {
-    const uint32_t bit = hits & (0u - hits), i = 31u - uint32_t(__clz(int(bit)));
+  while (hits && o.left == 0xffffffffu) {
+    const uint32_t i = uint32_t(__ffs(int(hits))) - 1u;
     const uint32_t piece = (i >> 2) * BLOCK + threadIdx.x;
     const float x = reinterpret_cast<const float*>(stage + piece)[i & 3u];
-    if (!store_key(s, floor, x, p.lead + (q + piece) * 4u + (i & 3u), want, o)) o.waiting |= uint64_t(bit) << (16 * k);
-    hits ^= bit;
+    if (!store_key(s, floor, x, p.lead + (q + piece) * 4u + (i & 3u), want, o)) o.left = k * 16u + i;
+    hits &= hits - 1u;
   }
 }
 
-// The look after a step that began at piece `q`: throws out the surplus when there is one, and
-// stores what had found no room (from the row itself: that is rare).  All adding threads call it.
-__device__ __forceinline__ void settle(Selection& s, const float* x, const Part& p, uint32_t q, int extra,
-                                       uint32_t want, Offer& o) {
+// The look after a step of `stages` stages from piece `q`: throws out the surplus when there is one,
+// and goes on with what had found no room (from the row itself: that is rare).  All adding threads
+// call it.
+__device__ __forceinline__ void settle(Selection& s, const float* x, const Part& p, uint32_t q, uint32_t stages,
+                                       int extra, uint32_t want, Offer& o) {
   while (adders_or<BLOCK>(o.over)) {
     keep_largest(s, min(s.count, Selection::CAP), want);
-    if (!adders_or<BLOCK>(o.waiting != 0 || o.outside)) break;
+    if (!adders_or<BLOCK>(o.left != 0xffffffffu || o.outside)) break;
     o.over = false;
     const uint64_t floor = s.floor;
-    uint64_t again = o.waiting;
-    o.waiting = 0;
+    const float low = floor_value(floor);
     if (o.outside) o.outside = !store_key(s, floor, x[extra], uint32_t(extra), want, o);
-    while (again) {
-      const uint64_t bit = again & (0ull - again);
-      const uint32_t i = 63u - uint32_t(__clzll(static_cast<long long>(bit)));
-      const uint32_t index = p.lead + (q + (i >> 2) * BLOCK + threadIdx.x) * 4u + (i & 3u);
-      if (!store_key(s, floor, x[index], index, want, o)) o.waiting |= bit;
-      again ^= bit;
+    uint32_t i = o.left;
+    o.left = 0xffffffffu;
+    for (; i < stages * 16u; ++i) {
+      const uint32_t piece = q + (i >> 4) * kStage<BLOCK> + (i >> 2 & 3u) * BLOCK + threadIdx.x;
+      if (piece >= p.q1) continue;
+      const uint32_t index = p.lead + piece * 4u + (i & 3u);
+      const float v = x[index];
+      if (v >= low && !store_key(s, floor, v, index, want, o)) {
+        o.left = i;
+        break;
+      }
     }
   }
   o = Offer{};
@@ -681,7 +712,7 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
       const Part p = part_of(x, vocab, rank, shares);
       const int extra_at = extra_of(p);
       const float extra = extra_at >= 0 ? x[extra_at] : -INFINITY;
-      Stream<Sum::Entropy> stream;
+      Stream<Sum::Entropy> stream(kLog2e);
       Offer mine;
       uint32_t q = p.q0;
       if (TOP) {  // the first stages stay until there is a floor
@@ -694,7 +725,10 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
           most = fmaxf(most, stream.add(v, kLog2e));
           at.next();
         }
-        first_floor(sel, most, a.top_n);
+        // the place of this row's result: the server has read the one of two rows ago
+        w.wait(&freed[i & 1], ((i >> 1) & 1u) ^ 1u, 0x21u);
+        static_assert(!TOP || sizeof(sorted[0]) >= BLOCK * 4, "room for the maxima");
+        first_floor(sel, reinterpret_cast<uint32_t*>(sorted[i & 1]), most, a.top_n);
         const uint64_t floor = sel.floor;
         const float low = floor_value(floor);
         if (extra_at >= 0 && extra >= low)
@@ -711,7 +745,7 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
           leave_stage<T>(bars, again);
           again.next();
         }
-        settle(sel, x, p, q, extra_at, a.top_n, mine);
+        settle(sel, x, p, q, FIRST, extra_at, a.top_n, mine);
         q += FIRST * kStage<T>;
       }
       while (q < p.q1 || (!TOP && q == p.q0)) {
@@ -730,13 +764,13 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
           leave_stage<T>(bars, at);
           at.next();
         }
-        if (TOP) settle(sel, x, p, q, -1, a.top_n, mine);
+        if (TOP) settle(sel, x, p, q, STEP, -1, a.top_n, mine);
         q += STEP * kStage<T>;
       }
       RowStats r = stream.result(kLog2e);
       add_one<Sum::Entropy>(r, extra, 0.f);
       r = block_merge<Sum::Entropy, T>(r, 0.f, merged[i & 1]);
-      w.wait(&freed[i & 1], ((i >> 1) & 1u) ^ 1u, 0x21u);
+      if (!TOP) w.wait(&freed[i & 1], ((i >> 1) & 1u) ^ 1u, 0x21u);
       uint32_t found = 0;
       if (TOP) found = sort_selection(sel, sorted[i & 1], a.top_n);
       if (threadIdx.x == 0) result[i & 1] = r;
@@ -1032,7 +1066,8 @@ __device__ __forceinline__ void grad_stage(const GradFactors& f, float4 (&v)[QUA
     v[j] = f.empty ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(a.x, a.y, b.x, b.y);
   }
 }
-// The same from the exponentials that Stream::add left when its maximum was m (<= the row's).
+// The same from the exponentials that Stream::add left when its reference was m (<= the row's
+// maximum).
 template <Sum SUM>
 __device__ __forceinline__ void scale_stage(const GradFactors& f, float4 (&v)[QUADS], float m, float c) {
   const float ref = reference(m);
@@ -1185,7 +1220,7 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
       if (PASS == DistillPass::Backward) {
         r = saved_stats(a, row);
       } else {
-        Stream<SUM> stream;
+        Stream<SUM> stream(c);
         uint32_t q = p.q0;
         do {
           float4 v[QUADS];
