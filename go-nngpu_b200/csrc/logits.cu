@@ -788,30 +788,42 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
     __syncthreads();
     ptx::cluster_sync_all();  // every block's results are in place
     if (rank == 0 && warp < WARPS) {
-      RowStats r = result[0];
-      const uint32_t at = ptx::smem_u32(&result[0]);
-      uint32_t n = 0;
+      // All peers are asked at once, a lane each (a word from another block's shared memory takes
+      // up to a thousand clocks).
+      const uint32_t lane = threadIdx.x & 31, peer = min(lane, shares - 1);
+      const uint32_t at = ptx::mapa_shared(ptx::smem_u32(&result[0]), peer);
+      RowStats r;
+      r.m = ptx::ld_shared_cluster(at);
+      r.s = ptx::ld_shared_cluster(at + 4);
+      r.u = ptx::ld_shared_cluster(at + 8);
+      if (lane >= shares) r = RowStats{};
+      rescale<Sum::Entropy>(r, order_value(__reduce_max_sync(0xffffffffu, order_bits(r.m))), 0.f);
+      r.s = warp_sum(r.s);
+      r.u = warp_sum(r.u);
       if (TOP) {  // the blocks' own alternatives, at most 8 x 128, behind one another
-        n = sel.count;
-        if (threadIdx.x < n) sel.key[threadIdx.x] = sorted[0][threadIdx.x];
-      }
-      for (uint32_t k = 1; k < shares; ++k) {
-        RowStats other;
-        other.m = ptx::ld_shared_cluster(ptx::mapa_shared(at, k));
-        other.s = ptx::ld_shared_cluster(ptx::mapa_shared(at + 4, k));
-        other.u = ptx::ld_shared_cluster(ptx::mapa_shared(at + 8, k));
-        merge<Sum::Entropy>(r, other, 0.f);
-        if (TOP) {
-          const uint32_t theirs = ptx::ld_shared_cluster_u32(ptx::mapa_shared(ptx::smem_u32(&sel.count), k));
-          if (threadIdx.x < theirs)
-            sel.key[n + threadIdx.x] =
-                ptx::ld_shared_cluster_u64(ptx::mapa_shared(ptx::smem_u32(&sorted[0][threadIdx.x]), k));
-          n += theirs;
+        uint32_t theirs = ptx::ld_shared_cluster_u32(ptx::mapa_shared(ptx::smem_u32(&sel.count), peer));
+        if (lane >= shares) theirs = 0;
+        uint32_t before = 0;  // keys of the peers below this lane's
+        for (uint32_t k = 0; k + 1 < shares; ++k) {
+          const uint32_t n = __shfl_sync(0xffffffffu, theirs, k);
+          if (k < lane) before += n;
         }
-      }
-      if (TOP) {
+        const uint32_t all = __shfl_sync(0xffffffffu, before + theirs, shares - 1);
+        uint64_t key[kMaxTop * MAX_SHARE / T];
+        uint32_t to[kMaxTop * MAX_SHARE / T];
+#pragma unroll
+        for (uint32_t i = 0; i < kMaxTop * MAX_SHARE / T; ++i) {
+          const uint32_t from = (i * T + threadIdx.x) / kMaxTop, k = threadIdx.x % kMaxTop;
+          const uint32_t n = __shfl_sync(0xffffffffu, theirs, from), base = __shfl_sync(0xffffffffu, before, from);
+          const bool there = from < shares && k < n;
+          to[i] = there ? base + k : 0xffffffffu;
+          if (there) key[i] = ptx::ld_shared_cluster_u64(ptx::mapa_shared(ptx::smem_u32(&sorted[0][k]), from));
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kMaxTop * MAX_SHARE / T; ++i)
+          if (to[i] != 0xffffffffu) sel.key[to[i]] = key[i];
         adders_sync<T>();
-        if (threadIdx.x == 0) sel.count = n;
+        if (threadIdx.x == 0) sel.count = all;
         sort_selection(sel, sorted[1], a.top_n);
         adders_sync<T>();
       }
