@@ -219,7 +219,7 @@ __device__ __forceinline__ int extra_of(const Part& p) {
 __device__ __forceinline__ float4 masked_quad() { return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
 
 // ---- the ring ------------------------------------------------------------------------------
-// full[s]: the feeder's arrival and the stage's bytes; empty[s]: the adding warps.
+// full[s]: the feeder's arrival and the stage's bytes; empty[s]: the adding warps (or the storing one).
 template <int T>
 constexpr uint32_t kStage = QUADS * T;  // pieces of a stage: 16 or 32 KB
 template <int T>
@@ -227,10 +227,10 @@ constexpr uint32_t kStages = T == WIDE ? 6 : 4;  // 192 KB and one block an SM, 
 template <int T>
 struct RingBars {
   uint64_t full[kStages<T>], empty[kStages<T>];
-  __device__ void init() {
+  __device__ void init(uint32_t leavers) {
     for (uint32_t i = 0; i < kStages<T>; ++i) {
       ptx::mbar_init(ptx::smem_u32(&full[i]), 1);
-      ptx::mbar_init(ptx::smem_u32(&empty[i]), T / 32);
+      ptx::mbar_init(ptx::smem_u32(&empty[i]), leavers);
     }
   }
 };
@@ -673,7 +673,7 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
   const uint32_t warp = threadIdx.x >> 5, rank = blockIdx.x % shares, vocab = uint32_t(a.vocab);
   const uint64_t first_row = blockIdx.x / shares, step = gridDim.x / shares;
   if (threadIdx.x == 0) {
-    bars.init();
+    bars.init(WARPS);
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(ptx::smem_u32(&ready[i]), WARPS);
       ptx::mbar_init(ptx::smem_u32(&freed[i]), 1);
@@ -1142,15 +1142,21 @@ __device__ __forceinline__ void save_stats(const DistillArgs& a, uint64_t row, c
 // The serving warp reads a row's targets while the row before it is being added (tfull, tempty),
 // writes its loss (done) and corrects the gradient at the targets (written).  The blocks of a
 // cluster exchange their statistics by writing them into each other's shared memory (peers).
+//
+// BULK: the gradient takes the exponentials' place in the ring and a storing warp sends each stage
+// off with a bulk copy (stored[s] says that it is there); the next row is added meanwhile.  (16-byte
+// stores of the adding warps left an SM at 20 bytes a clock and took 6200 of a row's 13500 clocks.)
 template <DistillPass PASS>
 constexpr int kAdders = PASS == DistillPass::Step ? WIDE : BLOCK;
-template <DistillPass PASS, Sum SUM>
-__global__ void __launch_bounds__(kAdders<PASS> + 64, PASS == DistillPass::Step ? 1 : 3)
+template <DistillPass PASS>
+constexpr int kRingThreads = kAdders<PASS> + (PASS == DistillPass::Step ? 96 : 64);
+template <DistillPass PASS, Sum SUM, bool BULK>
+__global__ void __launch_bounds__(kRingThreads<PASS>, PASS == DistillPass::Step ? 1 : 3)
 distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
   constexpr int T = kAdders<PASS>, WARPS = T / 32;
   extern __shared__ float4 ring[];
   __shared__ RingBars<T> bars;
-  __shared__ uint64_t tfull[2], tempty[2], done[2], written[2], peers[2];
+  __shared__ uint64_t tfull[2], tempty[2], done[2], written[2], peers[2], stored[BULK ? kStages<T> : 1];
   __shared__ uint32_t abort_word;
   __shared__ RowStats result[2], merged[2][WARPS], parts[2][MAX_SHARE];
   __shared__ float kept_at[PASS == DistillPass::Step ? kStages<T> : 1][PASS == DistillPass::Step ? T : 1];
@@ -1160,12 +1166,13 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
   const uint64_t first_row = blockIdx.x / shares, step = gridDim.x / shares;
   const float c = kLog2e / a.temperature;
   if (threadIdx.x == 0) {
-    bars.init();
+    bars.init(BULK ? 1 : WARPS);
+    for (uint32_t i = 0; BULK && i < kStages<T>; ++i) ptx::mbar_init(ptx::smem_u32(&stored[i]), WARPS);
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(ptx::smem_u32(&tfull[i]), 1);
       ptx::mbar_init(ptx::smem_u32(&tempty[i]), WARPS);
       ptx::mbar_init(ptx::smem_u32(&done[i]), 1);
-      ptx::mbar_init(ptx::smem_u32(&written[i]), WARPS);
+      ptx::mbar_init(ptx::smem_u32(&written[i]), BULK ? 1 : WARPS);
       ptx::mbar_init(ptx::smem_u32(&peers[i]), shares);
     }
     abort_word = 0;
@@ -1218,6 +1225,37 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
       }
       __syncwarp();
     }
+  } else if (warp > WARPS + 1) {  // storer
+    if (BULK && lane == 0) {
+      RingAt<T> at, sent;  // the next stage to send, the first whose memory may still be read
+      bool sending = false;
+      uint32_t i = 0;
+      for (uint64_t row = first_row; row < a.rows; row += step, ++i) {
+        const Part p = part_of(a.x + row * a.ld, vocab, rank, shares);
+        float4* gq = reinterpret_cast<float4*>(a.grad + row * a.ld_grad + p.lead);
+        uint32_t q = p.q0;
+        do {
+          w.wait(&stored[at.slot], at.phase, 0x40u | at.slot);
+          const uint32_t n = min(kStage<T>, p.q1 - q);
+          if (n) ptx::bulk_store(gq + q, ptx::smem_u32(ring + at.slot * kStage<T>), n * 16);
+          ptx::bulk_commit();
+          if (sending) {
+            ptx::bulk_wait_read<1>();
+            arrive(&bars.empty[sent.slot]);
+            sent.next();
+          }
+          sending = true;
+          at.next();
+          q += kStage<T>;
+        } while (q < p.q1);
+        ptx::bulk_wait<0>();  // the row is in memory: its targets may be corrected
+        arrive(&bars.empty[sent.slot]);
+        sent.next();
+        sending = false;
+        arrive(&written[i & 1]);
+      }
+    }
+    __syncwarp();
   } else {  // adders
     RingAt<T> at;
     uint32_t i = 0;
@@ -1293,9 +1331,19 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
             read_stage<T>(p, q, ring + start.slot * kStage<T>, v);
             if (SUM == Sum::Tempered) grad_stage<SUM>(f, v, c);
             else scale_stage<SUM>(f, v, kept_at[start.slot][threadIdx.x], c);
-            // the exponentials were written here: they come before the copy that fills the stage next
-            if (SUM != Sum::Tempered) ptx::fence_proxy_async_smem();
-            leave_stage<T>(bars, start);
+            if (BULK) {
+              float4* to = ring + start.slot * kStage<T> + threadIdx.x;
+#pragma unroll
+              for (uint32_t j = 0; j < QUADS; ++j) to[j * T] = v[j];
+            }
+            // what was written here comes before the copy that sends the stage off, or fills it
+            if (BULK || SUM != Sum::Tempered) ptx::fence_proxy_async_smem();
+            if (BULK) {
+              __syncwarp();
+              if (lane == 0) arrive(&stored[start.slot]);
+            } else {
+              leave_stage<T>(bars, start);
+            }
             start.next();
           } else {
             take_stage<T>(p, q, ring, bars, at, w, v);
@@ -1303,7 +1351,9 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
             at.next();
             grad_stage<SUM>(f, v, c);
           }
-          if (vec && q + kStage<T> <= p.q1) {
+          if (BULK) {
+            // sent by the storing warp
+          } else if (vec && q + kStage<T> <= p.q1) {
 #pragma unroll
             for (uint32_t j = 0; j < QUADS; ++j) __stcs(gq + q + threadIdx.x + j * T, v[j]);
           } else {
@@ -1329,7 +1379,7 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
       }
       __syncwarp();
       if (lane == 0) {
-        if (PASS != DistillPass::Forward) arrive(&written[turn]);
+        if (PASS != DistillPass::Forward && !BULK) arrive(&written[turn]);
         arrive(&tempty[turn]);
       }
     }
@@ -1394,7 +1444,7 @@ uint32_t rows_grid(uint64_t rows) { return uint32_t((rows + ROWS_BLOCK / 32 - 1)
 // once: a cluster lies within one GPC, so that is fewer than the SMs would hold, and one more would
 // start when the first are done (the step over 1024 x 128000 took 479 us with 37 clusters of 4 on
 // 148 SMs, 263 us with those that fit).
-template <auto KERN, int T>
+template <auto KERN, int T, int THREADS = T + 64>
 cudaError_t launch_ring(uint64_t rows, uint32_t shares, cudaStream_t stream, auto... args) {
   constexpr size_t smem = size_t(kStages<T>) * kStage<T> * 16;
   static int fit[64][MAX_SHARE + 1] = {};  // per kernel and device: clusters that run at once
@@ -1405,7 +1455,7 @@ cudaError_t launch_ring(uint64_t rows, uint32_t shares, cudaStream_t stream, aut
     cudaError_t e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(shares);
-    cfg.blockDim = dim3(T + 64);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1420,7 +1470,7 @@ cudaError_t launch_ring(uint64_t rows, uint32_t shares, cudaStream_t stream, aut
     at_once = n;
   }
   const uint64_t clusters = std::min<uint64_t>(rows, at_once);
-  return launch_kernel_cluster(KERN, shares, dim3(uint32_t(clusters) * shares), dim3(T + 64), smem, stream, args...);
+  return launch_kernel_cluster(KERN, shares, dim3(uint32_t(clusters) * shares), dim3(THREADS), smem, stream, args...);
 }
 
 template <DistillPass PASS, Sum SUM>
@@ -1435,13 +1485,20 @@ cudaError_t launch_distill_sum(const DistillArgs& a, int sm_count, cudaStream_t 
   uint32_t shares = shares_for(a.rows, a.vocab, sm_count);
   constexpr int T = kAdders<PASS>;
   if (PASS != DistillPass::Step)
-    return launch_ring<distill_ring_kernel<PASS, SUM>, T>(a.rows, shares, stream, a, shares, false);
+    return launch_ring<distill_ring_kernel<PASS, SUM, false>, T>(a.rows, shares, stream, a, shares, false);
   // a part takes at most 4 of the 6 stages, so that loads run while it is kept, or all of them where
   // 8 blocks are not enough for that
   auto part_stages = [&](uint32_t n) { return (a.vocab / 4 / n + 1 + kStage<T> - 1) / kStage<T>; };
   while (shares < MAX_SHARE && part_stages(shares) > 4) shares *= 2;
   const bool keep = part_stages(shares) <= kStages<T>;
-  return launch_ring<distill_ring_kernel<PASS, SUM>, T>(a.rows, shares, stream, a, shares, keep);
+  constexpr int THREADS = kRingThreads<PASS>;
+  // bulk stores need the rows of both matrices at the same distance from a 16-byte boundary
+  const bool bulk = keep && ((reinterpret_cast<uintptr_t>(a.grad) ^ reinterpret_cast<uintptr_t>(a.x)) & 15u) == 0 &&
+                    (a.ld_grad - a.ld) % 4 == 0;
+  if (PASS == DistillPass::Step && bulk)
+    return launch_ring<distill_ring_kernel<PASS, SUM, PASS == DistillPass::Step>, T, THREADS>(a.rows, shares, stream, a,
+                                                                                            shares, keep);
+  return launch_ring<distill_ring_kernel<PASS, SUM, false>, T, THREADS>(a.rows, shares, stream, a, shares, keep);
 }
 
 template <DistillPass PASS>

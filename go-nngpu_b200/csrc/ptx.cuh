@@ -112,6 +112,22 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
+// The same shared -> global, in the issuing thread's current group of stores.  What was written to
+// shared memory by ordinary stores has to be fenced (fence_proxy_async_smem) first.
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t smem_src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// At most N of this thread's groups have not read their shared memory yet / are not complete.
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bulk_wait() {
+  asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory");
+}
 // 3-D tiled load (used for MN-major operands: all 128-byte-wide slabs of a tile in one box).
 __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* m, int32_t c0,
                                             int32_t c1, int32_t c2, uint32_t bar) {
