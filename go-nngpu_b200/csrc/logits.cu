@@ -127,15 +127,6 @@ __device__ __forceinline__ void add(RowStats& r, float x, float ref, float c) {
   if (tempered(SUM)) r.u += exp2_ftz(d * c);
 }
 
-template <Sum SUM>
-__device__ __forceinline__ void merge(RowStats& a, RowStats b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  rescale<SUM>(a, m, c);
-  rescale<SUM>(b, m, c);
-  a.s += b.s;
-  a.u += b.u;
-}
-
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -325,8 +316,8 @@ __device__ __forceinline__ void add_one(RowStats& r, float x, float c) {
 //
 // m is a reference and need not be the maximum: it is the largest logit of the warp's first stage,
 // and moves only when one comes whose exponential would be above 2^58 (the sums are then still far
-// from overflow).  With the reference at each thread's running maximum some lane of
-// a warp moved it at nearly every stage, which made a stage take 1400 clocks instead of 900.
+// from overflow).  With the reference at each thread's running maximum some lane of a warp moved it
+// at nearly every stage (1021 x 50001, top 5: 53 us instead of 50).
 template <Sum SUM>
 struct Stream {
   const float slack;
@@ -926,6 +917,8 @@ struct Targets {
   float take[kMaxTop + 1];  // q_k, then 1 for the label
   float x_at[kMaxTop + 1];  // the student's logit there
   float log_q[kMaxTop];
+  float scale;              // of the row's gradient
+  float saved[3];           // the statistics that the forward pass has left: m, u, s (Backward)
   float soft;               // 1: there is a teacher, 0: there is none, NaN: it is spoiled
 };
 
@@ -990,6 +983,7 @@ __device__ void read_targets(const DistillArgs& a, uint64_t row, const float* x,
     t.index[a.top_n] = label;
     t.take[a.top_n] = 1.f;
     t.x_at[a.top_n] = x_label;
+    t.scale = a.grad_loss ? a.grad_scale * a.grad_loss[row] : a.grad_scale;
     // a NaN among the teacher's logits spoils the whole row, not only the tokens it names
     t.soft = total == 0.f ? 0.f : total == total ? 1.f : NAN;
   }
@@ -1023,10 +1017,10 @@ struct GradFactors {
   bool empty, far;
 };
 template <Sum SUM>
-__device__ __forceinline__ GradFactors grad_factors(const DistillArgs& a, uint64_t row, const RowStats& r, float soft,
-                                                    int label, float c) {
+__device__ __forceinline__ GradFactors grad_factors(const DistillArgs& a, const RowStats& r, const Targets& t, float c) {
   GradFactors f;
-  const float scale = a.grad_loss ? a.grad_scale * a.grad_loss[row] : a.grad_scale;
+  const float scale = t.scale, soft = t.soft;
+  const int label = t.index[a.top_n];
   f.empty = r.m == -INFINITY && r.s == 0.f && r.u == 0.f;
   f.m = reference(r.m);
   f.far = !(fabsf(f.m) < 1e37f);
@@ -1096,22 +1090,34 @@ __device__ __forceinline__ void scale_stage(const GradFactors& f, float4 (&v)[QU
   }
 }
 
-// The places that the teacher and the label name, among [first, end): the first entry that names
-// a place takes away what all of them do there, in their order.  Called by one warp.
+// Takes the targets' part from the gradient at the places that they name, among [first, end).
+// Called by one warp.  Entries that name the same place are added up before they are taken off
+// where they are in one group of 32, and are taken off one group after the other where they are not
+// (same-address reductions of a warp stay in order): the result does not depend on timing.  The
+// reductions leave without waiting for the gradient to come back; with loads, and a loop over all
+// entries for those that name a place again, this took 10000 to 17000 clocks for 65 entries, longer
+// than all else that happens to a block's part of a row.
 __device__ void take_targets(const DistillArgs& a, float* g, const Targets& t, const GradFactors& f, uint32_t first,
                              uint32_t end) {
   if (f.empty) return;
-  const uint32_t n = a.top_n + 1;
-  for (uint32_t k = threadIdx.x & 31; k < n; k += 32) {
-    const int index = t.index[k];
-    bool lead = index >= int(first) && uint32_t(index) < end;
-#pragma unroll 8
-    for (uint32_t j = 0; j < k; ++j) lead = lead && t.index[j] != index;
-    if (!lead) continue;
-    float v = g[index];
-#pragma unroll 8
-    for (uint32_t j = k; j < n; ++j) v -= t.index[j] == index ? t.take[j] * (j == a.top_n ? f.hard : f.soft) : 0.f;
-    g[index] = v;
+  const uint32_t n = a.top_n + 1, lane = threadIdx.x & 31;
+  for (uint32_t k0 = 0; k0 < n; k0 += 32) {
+    const uint32_t k = k0 + lane;
+    const int index = k < n ? t.index[k] : -1;
+    const bool here = index >= int(first) && uint32_t(index) < end;
+    float by = here ? t.take[k] * (k == a.top_n ? f.hard : f.soft) : 0.f;
+    const uint32_t same = __match_any_sync(0xffffffffu, here ? index : -1 - int(lane));
+    const bool lead = uint32_t(__ffs(int(same))) == lane + 1;
+    if (!__all_sync(0xffffffffu, lead)) {
+      float sum = 0.f;
+      for (uint32_t j = 0; j < 32; ++j) {
+        const float other = __shfl_sync(0xffffffffu, by, int(j));
+        if ((same >> j) & 1u) sum += other;
+      }
+      by = sum;
+    }
+    if (here && lead) ptx::red_add(g + index, -by);
+    __syncwarp();
   }
 }
 
@@ -1133,34 +1139,39 @@ __device__ __forceinline__ void save_stats(const DistillArgs& a, uint64_t row, c
   a.stats[row * 3 + 2] = r.s;
 }
 
-// Long rows.  In the step a block keeps its part of a row in the ring until the gradient has been
-// written from there (`keep`); what is left of the ring holds the first stages of the next row
-// meanwhile.  (Reading the row twice, with the rows in flight small enough for L2, took 1.6 times
-// as long: the clusters that takes spent their time waiting for one another.)  Only rows too long
-// for 8 blocks' rings are read twice.
+// Long rows.  The step reads a row twice, the second time from L2 (see launch_step).  Parts of a row
+// that leave room in the ring for the next row's first stages are read once (`keep`): their
+// exponentials wait in the ring for the gradient.  (2048 x 32000: 100 us, read twice 104; in 2 to 8
+// blocks' rings, 4096 x 128000 took 823 to 1142 us, read twice 683.)
 //
-// The serving warp reads a row's targets while the row before it is being added (tfull, tempty),
-// writes its loss (done) and corrects the gradient at the targets (written).  The blocks of a
-// cluster exchange their statistics by writing them into each other's shared memory (peers).
+// The serving warps read a row's targets while rows before it are being added (tfull, tempty), write
+// its loss (done) and correct the gradient at the targets (written); with two of them in the step,
+// each may take as long as two rows.  The blocks of a cluster send each other their statistics
+// (peers).
 //
-// BULK: the gradient takes the exponentials' place in the ring and a storing warp sends each stage
-// off with a bulk copy (stored[s] says that it is there); the next row is added meanwhile.  (16-byte
-// stores of the adding warps left an SM at 20 bytes a clock and took 6200 of a row's 13500 clocks.)
+// BULK: the gradient takes the logits' place in the ring and a storing warp sends each stage off
+// with a bulk copy (stored[s] says that it is there) while the next is added; it also gives back
+// the stages of the first reading.  (16-byte stores of the adding warps left an SM at 20 bytes a
+// clock and took 6200 of a row's 13500 clocks.)  `written` comes when the next row's first stage
+// does: until then the row's bytes had time to arrive.
 template <DistillPass PASS>
-constexpr int kAdders = PASS == DistillPass::Step ? WIDE : BLOCK;
-template <DistillPass PASS>
-constexpr int kRingThreads = kAdders<PASS> + (PASS == DistillPass::Step ? 96 : 64);
-template <DistillPass PASS, Sum SUM, bool BULK>
-__global__ void __launch_bounds__(kRingThreads<PASS>, PASS == DistillPass::Step ? 1 : 3)
+constexpr int kServers = PASS == DistillPass::Step ? 2 : 1;  // warps that take care of the targets
+template <DistillPass PASS, int T>
+constexpr int kRingThreads = T + 32 + 32 * kServers<PASS> + (PASS == DistillPass::Step ? 32 : 0);
+template <DistillPass PASS, int T>
+constexpr int kRingBlocks = PASS != DistillPass::Step ? 3 : T == WIDE ? 1 : 2;  // an SM
+template <DistillPass PASS, Sum SUM, bool BULK, int T>
+__global__ void __launch_bounds__((kRingThreads<PASS, T>), (kRingBlocks<PASS, T>))
 distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
-  constexpr int T = kAdders<PASS>, WARPS = T / 32;
+  constexpr int WARPS = T / 32, SERVERS = kServers<PASS>, SLOTS = 2 * SERVERS;
   extern __shared__ float4 ring[];
   __shared__ RingBars<T> bars;
-  __shared__ uint64_t tfull[2], tempty[2], done[2], written[2], peers[2], stored[BULK ? kStages<T> : 1];
+  __shared__ uint64_t tfull[SLOTS], tempty[SLOTS], done[SLOTS], written[SLOTS], peers[2], stored[BULK ? kStages<T> : 1];
   __shared__ uint32_t abort_word;
-  __shared__ RowStats result[2], merged[2][WARPS], parts[2][MAX_SHARE];
+  __shared__ RowStats result[SLOTS], merged[2][WARPS];
+  __shared__ float4 parts[2][MAX_SHARE];  // of a row: m, s, u of every block
   __shared__ float kept_at[PASS == DistillPass::Step ? kStages<T> : 1][PASS == DistillPass::Step ? T : 1];
-  __shared__ Targets targets[2];
+  __shared__ Targets targets[SLOTS];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % shares;
   const uint32_t vocab = uint32_t(a.vocab);
   const uint64_t first_row = blockIdx.x / shares, step = gridDim.x / shares;
@@ -1168,13 +1179,13 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
   if (threadIdx.x == 0) {
     bars.init(BULK ? 1 : WARPS);
     for (uint32_t i = 0; BULK && i < kStages<T>; ++i) ptx::mbar_init(ptx::smem_u32(&stored[i]), WARPS);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < SLOTS; ++i) {
       ptx::mbar_init(ptx::smem_u32(&tfull[i]), 1);
       ptx::mbar_init(ptx::smem_u32(&tempty[i]), WARPS);
       ptx::mbar_init(ptx::smem_u32(&done[i]), 1);
       ptx::mbar_init(ptx::smem_u32(&written[i]), BULK ? 1 : WARPS);
-      ptx::mbar_init(ptx::smem_u32(&peers[i]), shares);
     }
+    for (int i = 0; i < 2; ++i) ptx::mbar_init(ptx::smem_u32(&peers[i]), 1);
     abort_word = 0;
     ptx::fence_mbar_init();
     ptx::fence_proxy_async_smem();
@@ -1195,19 +1206,27 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
       }
     }
     __syncwarp();
-  } else if (warp == WARPS + 1) {  // server
-    uint32_t i = 0;
-    auto publish = [&](uint32_t k, uint64_t row) {
-      w.wait(&tempty[k & 1], ((k >> 1) & 1u) ^ 1u, 0x30u);
-      if (PASS != DistillPass::Forward || rank == 0)
-        read_targets<PASS != DistillPass::Backward>(a, row, a.x + row * a.ld, rank == 0, targets[k & 1]);
+  } else if (warp > WARPS && warp <= WARPS + SERVERS) {  // servers, each with every SERVERS-th row
+    const uint32_t me = warp - WARPS - 1;
+    auto publish = [&](uint32_t k) {
+      const uint64_t row = first_row + uint64_t(k) * step;
+      if (row >= a.rows) return;
+      w.wait(&tempty[k % SLOTS], ((k / SLOTS) & 1u) ^ 1u, 0x30u);
+      if (PASS == DistillPass::Backward) {
+        read_targets<false>(a, row, a.x + row * a.ld, rank == 0, targets[k % SLOTS]);
+        if (lane < 3) targets[k % SLOTS].saved[lane] = a.stats_in[row * 3 + lane];
+      }
+      else if (rank == 0) read_targets<true>(a, row, a.x + row * a.ld, true, targets[k % SLOTS]);
+      else if (PASS == DistillPass::Step) read_targets<false>(a, row, a.x + row * a.ld, false, targets[k % SLOTS]);
       __syncwarp();
-      if (lane == 0) arrive(&tfull[k & 1]);
+      if (lane == 0) arrive(&tfull[k % SLOTS]);
     };
-    if (first_row < a.rows) publish(0, first_row);
-    for (uint64_t row = first_row; row < a.rows; row += step, ++i) {
-      if (row + step < a.rows) publish(i + 1, row + step);
-      const uint32_t turn = i & 1, phase = (i >> 1) & 1u;
+    publish(me);
+    for (uint32_t i = me;; i += SERVERS) {
+      const uint64_t row = first_row + uint64_t(i) * step;
+      if (row >= a.rows) break;
+      publish(i + SERVERS);
+      const uint32_t turn = i % SLOTS, phase = (i / SLOTS) & 1u;
       w.wait(&done[turn], phase, 0x31u);
       const RowStats r = result[turn];
       if (PASS != DistillPass::Backward && rank == 0) {
@@ -1218,41 +1237,61 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
         }
       }
       if (PASS != DistillPass::Forward) {
-        const GradFactors f = grad_factors<SUM>(a, row, r, targets[turn].soft, targets[turn].index[a.top_n], c);
+        const GradFactors f = grad_factors<SUM>(a, r, targets[turn], c);
         const Part p = part_of(a.x + row * a.ld, vocab, rank, shares);
         w.wait(&written[turn], phase, 0x34u);
         take_targets(a, a.grad + row * a.ld_grad, targets[turn], f, p.first, p.end);
       }
       __syncwarp();
     }
-  } else if (warp > WARPS + 1) {  // storer
+  } else if (warp > WARPS + SERVERS) {  // storer
     if (BULK && lane == 0) {
-      RingAt<T> at, sent;  // the next stage to send, the first whose memory may still be read
-      bool sending = false;
+      RingAt<T> at;
+      int sent = -1;  // a stage whose memory may still be read
       uint32_t i = 0;
       for (uint64_t row = first_row; row < a.rows; row += step, ++i) {
         const Part p = part_of(a.x + row * a.ld, vocab, rank, shares);
         float4* gq = reinterpret_cast<float4*>(a.grad + row * a.ld_grad + p.lead);
+        bool first = i > 0;
+        if (!keep) {  // the stages of the first reading have only to be given back
+          uint32_t q = p.q0;
+          do {
+            w.wait(&stored[at.slot], at.phase, 0x50u | at.slot);
+            if (first) {
+              ptx::bulk_wait<0>();
+              arrive(&bars.empty[sent]);
+              arrive(&written[(i - 1) % SLOTS]);
+              sent = -1;
+              first = false;
+            }
+            arrive(&bars.empty[at.slot]);
+            at.next();
+            q += kStage<T>;
+          } while (q < p.q1);
+        }
         uint32_t q = p.q0;
         do {
           w.wait(&stored[at.slot], at.phase, 0x40u | at.slot);
           const uint32_t n = min(kStage<T>, p.q1 - q);
           if (n) ptx::bulk_store(gq + q, ptx::smem_u32(ring + at.slot * kStage<T>), n * 16);
           ptx::bulk_commit();
-          if (sending) {
+          if (sent >= 0) {
             ptx::bulk_wait_read<1>();
-            arrive(&bars.empty[sent.slot]);
-            sent.next();
+            arrive(&bars.empty[sent]);
           }
-          sending = true;
+          if (first) {
+            ptx::bulk_wait<1>();  // the row before is in memory: its targets may be corrected
+            arrive(&written[(i - 1) % SLOTS]);
+            first = false;
+          }
+          sent = int(at.slot);
           at.next();
           q += kStage<T>;
         } while (q < p.q1);
-        ptx::bulk_wait<0>();  // the row is in memory: its targets may be corrected
-        arrive(&bars.empty[sent.slot]);
-        sent.next();
-        sending = false;
-        arrive(&written[i & 1]);
+      }
+      if (i) {
+        ptx::bulk_wait<0>();
+        arrive(&written[(i - 1) % SLOTS]);
       }
     }
     __syncwarp();
@@ -1261,15 +1300,13 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
     uint32_t i = 0;
     for (uint64_t row = first_row; row < a.rows; row += step, ++i) {
       RingAt<T> start = at;
-      const uint32_t turn = i & 1, phase = (i >> 1) & 1u;
+      const uint32_t turn = i % SLOTS, phase = (i / SLOTS) & 1u;
       const float* x = a.x + row * a.ld;
       const Part p = part_of(x, vocab, rank, shares);
       const int extra_at = extra_of(p);
       const float extra = extra_at >= 0 ? x[extra_at] : -INFINITY;
       RowStats r;
-      if (PASS == DistillPass::Backward) {
-        r = saved_stats(a, row);
-      } else {
+      if (PASS != DistillPass::Backward) {
         Stream<SUM> stream(c);
         uint32_t q = p.q0;
         do {
@@ -1284,6 +1321,9 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
               for (uint32_t j = 0; j < QUADS; ++j) to[j * T] = v[j];
               kept_at[at.slot][threadIdx.x] = stream.m;
             }
+          } else if (BULK) {
+            __syncwarp();
+            if (lane == 0) arrive(&stored[at.slot]);
           } else {
             leave_stage<T>(bars, at);
           }
@@ -1292,24 +1332,33 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
         } while (q < p.q1);
         r = stream.result(c);
         add_one<SUM>(r, extra, c);
-        r = block_merge<SUM, T>(r, c, merged[turn]);
+        r = block_merge<SUM, T>(r, c, merged[i & 1]);
       }
       // From here on the targets have been read, in every block of the cluster once its
       // statistics have arrived: the row may be overwritten.  The wait also says that the server
-      // is done with the result of two rows ago.
+      // is done with the result of SLOTS rows ago.
       w.wait(&tfull[turn], phase, 0x32u);
-      if (PASS != DistillPass::Backward) {
+      if (PASS == DistillPass::Backward) {
+        r.m = targets[turn].saved[0];
+        r.u = targets[turn].saved[1];
+        r.s = targets[turn].saved[2];
+      } else {
         if (shares > 1) {
-          if (threadIdx.x < shares) {
-            const uint32_t to = ptx::mapa_shared(ptx::smem_u32(&parts[turn][rank]), threadIdx.x);
-            ptx::st_shared_cluster(to, r.m);
-            ptx::st_shared_cluster(to + 4, r.s);
-            ptx::st_shared_cluster(to + 8, r.u);
-            ptx::mbar_arrive_cluster(ptx::mapa_shared(ptx::smem_u32(&peers[turn]), threadIdx.x));
+          const uint32_t bar = ptx::smem_u32(&peers[i & 1]);
+          if (threadIdx.x == 0) ptx::mbar_arrive_expect_tx(bar, shares * 16);
+          if (threadIdx.x < shares)
+            ptx::st_async(ptx::mapa_shared(ptx::smem_u32(&parts[i & 1][rank]), threadIdx.x),
+                          make_float4(r.m, r.s, r.u, 0.f), ptx::mapa_shared(bar, threadIdx.x));
+          w.wait_cluster(&peers[i & 1], (i >> 1) & 1u, 0x33u);
+          const float4 part = parts[i & 1][lane & (shares - 1)];
+          r.m = part.x;
+          r.s = part.y;
+          r.u = part.z;
+          rescale<SUM>(r, order_value(__reduce_max_sync(0xffffffffu, order_bits(r.m))), c);
+          for (uint32_t o = shares / 2; o > 0; o >>= 1) {
+            r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+            if (SUM != Sum::Plain) r.u += __shfl_xor_sync(0xffffffffu, r.u, o);
           }
-          w.wait_cluster(&peers[turn], phase, 0x33u);
-          r = parts[turn][0];
-          for (uint32_t k = 1; k < shares; ++k) merge<SUM>(r, parts[turn][k], c);
         }
         complete<SUM>(r);
       }
@@ -1318,7 +1367,7 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
         arrive(&done[turn]);
       }
       if (PASS != DistillPass::Forward) {
-        const GradFactors f = grad_factors<SUM>(a, row, r, targets[turn].soft, targets[turn].index[a.top_n], c);
+        const GradFactors f = grad_factors<SUM>(a, r, targets[turn], c);
         float* g = a.grad + row * a.ld_grad;
         if (extra_at >= 0) g[extra_at] = grad_at<SUM>(f, extra, c);
         // the same distance to a 16-byte boundary in both rows: 16-byte stores
@@ -1327,30 +1376,31 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
         uint32_t q = p.q0;
         do {
           float4 v[QUADS];
-          if (PASS == DistillPass::Step && keep) {
+          const bool kept = PASS == DistillPass::Step && keep;
+          RingAt<T>& now_at = kept ? start : at;
+          if (kept) {
             read_stage<T>(p, q, ring + start.slot * kStage<T>, v);
             if (SUM == Sum::Tempered) grad_stage<SUM>(f, v, c);
             else scale_stage<SUM>(f, v, kept_at[start.slot][threadIdx.x], c);
-            if (BULK) {
-              float4* to = ring + start.slot * kStage<T> + threadIdx.x;
-#pragma unroll
-              for (uint32_t j = 0; j < QUADS; ++j) to[j * T] = v[j];
-            }
-            // what was written here comes before the copy that sends the stage off, or fills it
-            if (BULK || SUM != Sum::Tempered) ptx::fence_proxy_async_smem();
-            if (BULK) {
-              __syncwarp();
-              if (lane == 0) arrive(&stored[start.slot]);
-            } else {
-              leave_stage<T>(bars, start);
-            }
-            start.next();
           } else {
             take_stage<T>(p, q, ring, bars, at, w, v);
-            leave_stage<T>(bars, at);
-            at.next();
+            if (!BULK) leave_stage<T>(bars, at);
             grad_stage<SUM>(f, v, c);
           }
+          if (BULK) {
+            float4* to = ring + now_at.slot * kStage<T> + threadIdx.x;
+#pragma unroll
+            for (uint32_t j = 0; j < QUADS; ++j) to[j * T] = v[j];
+          }
+          // what was written here comes before the copy that sends the stage off, or fills it
+          if (BULK || (kept && SUM != Sum::Tempered)) ptx::fence_proxy_async_smem();
+          if (BULK) {
+            __syncwarp();
+            if (lane == 0) arrive(&stored[now_at.slot]);
+          } else if (kept) {
+            leave_stage<T>(bars, start);
+          }
+          now_at.next();
           if (BULK) {
             // sent by the storing warp
           } else if (vec && q + kStage<T> <= p.q1) {
@@ -1418,7 +1468,7 @@ __global__ void __launch_bounds__(ROWS_BLOCK) distill_warp_kernel(const DistillA
     }
   }
   if (PASS != DistillPass::Forward) {
-    const GradFactors f = grad_factors<SUM>(a, row, r, targets[warp].soft, targets[warp].index[a.top_n], c);
+    const GradFactors f = grad_factors<SUM>(a, r, targets[warp], c);
     float* g = a.grad + row * a.ld_grad;
     __syncwarp();
 #pragma unroll
@@ -1473,6 +1523,29 @@ cudaError_t launch_ring(uint64_t rows, uint32_t shares, cudaStream_t stream, aut
   return launch_kernel_cluster(KERN, shares, dim3(uint32_t(clusters) * shares), dim3(THREADS), smem, stream, args...);
 }
 
+// The step over long rows with T adding threads a block.  What is read twice should come from L2 the
+// second time, so the rows in flight are kept below kInFlight by giving a row to more blocks
+// (4096 x 128000, one block a row and 76 MB in flight: 940 us; two and 38 MB: 683; four and 19 MB:
+// 801, since each row costs a block some 3000 clocks besides its logits).
+constexpr uint64_t kInFlight = 48ull << 20;
+template <Sum SUM, int T>
+cudaError_t launch_step(const DistillArgs& a, int sm_count, cudaStream_t stream) {
+  constexpr DistillPass PASS = DistillPass::Step;
+  uint32_t shares = shares_for(a.rows, a.vocab, sm_count);
+  auto in_flight = [&] {
+    return std::min<uint64_t>(a.rows, uint64_t(sm_count) * kRingBlocks<PASS, T> / shares) * a.vocab * 4;
+  };
+  while (shares < MAX_SHARE && in_flight() > kInFlight) shares *= 2;
+  // a part that leaves the next row's loads two stages of the ring is kept there
+  const bool keep = a.vocab / 4 / shares + 1 <= (kStages<T> - 2) * kStage<T>;
+  // bulk stores need the rows of both matrices at the same distance from a 16-byte boundary
+  const bool bulk = ((reinterpret_cast<uintptr_t>(a.grad) ^ reinterpret_cast<uintptr_t>(a.x)) & 15u) == 0 &&
+                    (a.ld_grad - a.ld) % 4 == 0;
+  constexpr int THREADS = kRingThreads<PASS, T>;
+  return bulk ? launch_ring<distill_ring_kernel<PASS, SUM, true, T>, T, THREADS>(a.rows, shares, stream, a, shares, keep)
+              : launch_ring<distill_ring_kernel<PASS, SUM, false, T>, T, THREADS>(a.rows, shares, stream, a, shares, keep);
+}
+
 template <DistillPass PASS, Sum SUM>
 cudaError_t launch_distill_sum(const DistillArgs& a, int sm_count, cudaStream_t stream) {
   if (a.vocab <= WARP_ROW) {
@@ -1482,23 +1555,16 @@ cudaError_t launch_distill_sum(const DistillArgs& a, int sm_count, cudaStream_t 
                                  : distill_warp_kernel<PASS, SUM, 32>;
     return launch_kernel(kern, dim3(rows_grid(a.rows)), dim3(ROWS_BLOCK), 0, stream, a);
   }
-  uint32_t shares = shares_for(a.rows, a.vocab, sm_count);
-  constexpr int T = kAdders<PASS>;
-  if (PASS != DistillPass::Step)
-    return launch_ring<distill_ring_kernel<PASS, SUM, false>, T>(a.rows, shares, stream, a, shares, false);
-  // a part takes at most 4 of the 6 stages, so that loads run while it is kept, or all of them where
-  // 8 blocks are not enough for that
-  auto part_stages = [&](uint32_t n) { return (a.vocab / 4 / n + 1 + kStage<T> - 1) / kStage<T>; };
-  while (shares < MAX_SHARE && part_stages(shares) > 4) shares *= 2;
-  const bool keep = part_stages(shares) <= kStages<T>;
-  constexpr int THREADS = kRingThreads<PASS>;
-  // bulk stores need the rows of both matrices at the same distance from a 16-byte boundary
-  const bool bulk = keep && ((reinterpret_cast<uintptr_t>(a.grad) ^ reinterpret_cast<uintptr_t>(a.x)) & 15u) == 0 &&
-                    (a.ld_grad - a.ld) % 4 == 0;
-  if (PASS == DistillPass::Step && bulk)
-    return launch_ring<distill_ring_kernel<PASS, SUM, PASS == DistillPass::Step>, T, THREADS>(a.rows, shares, stream, a,
-                                                                                            shares, keep);
-  return launch_ring<distill_ring_kernel<PASS, SUM, false>, T, THREADS>(a.rows, shares, stream, a, shares, keep);
+  if constexpr (PASS == DistillPass::Step) {
+    // Two narrow blocks an SM hide each other's waits between rows, a wide one has more of them in
+    // flight: 2000 x 8000 41 and 55 us, x 12000 53 and 64, x 16000 68 and 66, x 24000 88 and 82.
+    return a.vocab <= 3 * 4 * kStage<BLOCK> ? launch_step<SUM, BLOCK>(a, sm_count, stream)
+                                            : launch_step<SUM, WIDE>(a, sm_count, stream);
+  } else {
+    const uint32_t shares = shares_for(a.rows, a.vocab, sm_count);
+    return launch_ring<distill_ring_kernel<PASS, SUM, false, BLOCK>, BLOCK, kRingThreads<PASS, BLOCK>>(
+        a.rows, shares, stream, a, shares, false);
+  }
 }
 
 template <DistillPass PASS>
