@@ -70,21 +70,6 @@ __device__ __forceinline__ bool adders_or(bool v) {
       : "memory");
   return r != 0;
 }
-template <int T>
-__device__ __forceinline__ uint32_t adders_count(bool v) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t"
-      ".reg .pred P;\n\t"
-      "setp.ne.u32 P, %1, 0;\n\t"
-      "bar.red.popc.u32 %0, 1, %2, P;\n\t"
-      "}\n"
-      : "=r"(r)
-      : "r"(uint32_t(v)), "n"(T)
-      : "memory");
-  return r;
-}
-
 // ---- statistics of (part of) a row ------------------------------------------------------
 // What is summed beside S: nothing; U for the entropy; or the tempered sum e^((x-m)/T), with
 // `c` = log2(e) / T.  With T = 2 or 4, e^(x-m) is the tempered exponential squared once or twice: one
@@ -431,9 +416,10 @@ constexpr uint32_t kMaskedBits = 0x007fffffu;  // order_bits(-inf); below it onl
 
 // The largest `want` keys a block has met.  A key is kept when it lies above a floor that is known
 // to have `want` keys above it.  The first floor comes from the threads' maxima of their first 32
-// logits (as many of those as wanted lie above it, so as many logits do); when more than about
-// twice the wanted keys are kept, the surplus is thrown out and the floor rises to the exact
-// want-th key, which in ordinary rows happens each time the logits seen have tripled.
+// logits (as many of those as wanted lie above it, so as many logits do).  Before the
+// buffer can have filled up (in rows without an order), the threads look whether there are more than
+// kCrowd keys; then the surplus is thrown out and the floor rises.  (With a look every 16 stages
+// the buffer did fill up: 2048 x 64000, top 128, 349 us instead of 193.)
 struct Selection {
   static constexpr uint32_t CAP = 1024;
   uint64_t key[CAP];
@@ -442,22 +428,15 @@ struct Selection {
   uint32_t part[2][BLOCK / 32];
 };
 
-// Sum over the block of a count; `turn` alternates so that one barrier a call is enough.
-__device__ __forceinline__ uint32_t block_count(Selection& s, uint32_t n, uint32_t& turn) {
-  n = __reduce_add_sync(0xffffffffu, n);
-  if ((threadIdx.x & 31) == 0) s.part[turn][threadIdx.x >> 5] = n;
-  adders_sync<BLOCK>();
-  uint32_t all = 0;
-#pragma unroll
-  for (int w = 0; w < BLOCK / 32; ++w) all += s.part[turn][w];
-  turn ^= 1u;
-  return all;
-}
+constexpr uint32_t kCrowd = 2 * kMaxTop + 64;  // more keys than that are thinned out
 
-// Throws out all but the `want` largest of the n > want keys (all different): bit by bit, the
-// largest floor that still has `want` keys at or above it.  Ends with a barrier.
-__device__ void keep_largest(Selection& s, uint32_t n, uint32_t want) {
-  constexpr uint32_t PER = Selection::CAP / BLOCK;
+// Throws out the smallest of the n > want + want / 2 + 16 keys (all different): the `want` largest
+// stay and up to want / 2 + 16 more.  All threads look for a bound, two bits a round, with a barrier
+// a round; they stop at the first that leaves few enough.  (The exact bound, a bit a round, took
+// 11000 clocks of a row's 50000; this takes about 2500.)  Ends with a barrier.
+__device__ __noinline__ void keep_largest(Selection& s, uint32_t n, uint32_t want) {
+  constexpr uint32_t PER = Selection::CAP / BLOCK, WARPS = BLOCK / 32;
+  const uint32_t most = want + want / 2 + 16;
   uint64_t mine[PER];
 #pragma unroll
   for (uint32_t i = 0; i < PER; ++i) {
@@ -466,18 +445,29 @@ __device__ void keep_largest(Selection& s, uint32_t n, uint32_t want) {
   }
   uint64_t floor = 0;
   uint32_t turn = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t trial = floor | (1ull << bit);
+  for (int bit = 62; bit >= 0; bit -= 2) {
+    // keys at or above the three bounds, 10 bits each: a warp has at most 128 keys
     uint32_t above = 0;
-    if (n <= BLOCK) {
-      above = adders_count<BLOCK>(mine[0] >= trial);
-    } else {
 #pragma unroll
-      for (uint32_t i = 0; i < PER; ++i) above += mine[i] >= trial;
-      above = block_count(s, above, turn);
+    for (uint32_t i = 0; i < PER; ++i)
+#pragma unroll
+      for (uint32_t k = 0; k < 3; ++k) above += uint32_t(mine[i] >= (floor | (uint64_t(k + 1) << bit))) << (10 * k);
+    above = __reduce_add_sync(0xffffffffu, above);
+    if ((threadIdx.x & 31) == 0) s.part[turn][threadIdx.x >> 5] = above;
+    adders_sync<BLOCK>();
+    uint32_t c1 = 0, c2 = 0, c3 = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < WARPS; ++w) {
+      above = s.part[turn][w];
+      c1 += above & 1023u;
+      c2 += above >> 10 & 1023u;
+      c3 += above >> 20;
     }
-    if (above >= want) floor = trial;
-    if (above == want) break;
+    turn ^= 1u;
+    const uint32_t digit = c3 >= want ? 3u : c2 >= want ? 2u : c1 >= want ? 1u : 0u;
+    floor |= uint64_t(digit) << bit;
+    const uint32_t left = digit == 3 ? c3 : digit == 2 ? c2 : c1;
+    if (digit && left <= most) break;
   }
   if (threadIdx.x == 0) {
     s.count = 0;
@@ -492,8 +482,8 @@ __device__ void keep_largest(Selection& s, uint32_t n, uint32_t want) {
 
 // The first floor from the threads' maxima, 18 bits of it: one warp looks for the largest bound
 // with `want` maxima at or above it, two bits a round, with the three counts of a round in one
-// word.  (All threads counting together, a barrier a bit, took 2100 clocks of a row's 27000.)  `maxima`:
-// room for BLOCK words.
+// word.  (All threads counting together, a barrier a bit, took 2100 clocks of a row's 27000.)
+// `maxima`: room for BLOCK words.
 __device__ void first_floor(Selection& s, uint32_t* maxima, float most, uint32_t want) {
   maxima[threadIdx.x] = order_bits(most);
   adders_sync<BLOCK>();
@@ -509,9 +499,9 @@ __device__ void first_floor(Selection& s, uint32_t* maxima, float most, uint32_t
 #pragma unroll
         for (uint32_t k = 0; k < 3; ++k) above += uint32_t(mine[i] >= (floor | ((k + 1) << bit))) << (10 * k);
       above = __reduce_add_sync(0xffffffffu, above);
-      if ((above >> 20) >= want) floor |= 3u << bit;
-      else if ((above >> 10 & 1023u) >= want) floor |= 2u << bit;
-      else if ((above & 1023u) >= want) floor |= 1u << bit;
+      const uint32_t c1 = above & 1023u, c2 = above >> 10 & 1023u, c3 = above >> 20;
+      const uint32_t digit = c3 >= want ? 3u : c2 >= want ? 2u : c1 >= want ? 1u : 0u;
+      floor |= digit << bit;
     }
     if (threadIdx.x == 0) {
       s.floor = uint64_t(floor) << 32;
@@ -525,8 +515,8 @@ __device__ void first_floor(Selection& s, uint32_t* maxima, float most, uint32_t
 __device__ __forceinline__ float floor_value(uint64_t floor) {
   return uint32_t(floor >> 32) <= kMaskedBits ? -INFINITY : key_value(floor);
 }
-constexpr uint32_t STEP = 16;  // stages between two looks at how many keys there are
 constexpr uint32_t FIRST = 2;  // stages that the first floor is taken from
+
 // Which of a thread's 16 logits from piece `q` may lie above the floor, a bit each.
 __device__ __forceinline__ uint32_t above_floor(const Part& p, uint32_t q, const float4 (&v)[QUADS], float low) {
   uint32_t hits = 0;
@@ -548,12 +538,11 @@ struct Offer {
 };
 
 // Stores a logit's key unless it lies below the floor; false when there is no room.
-__device__ __forceinline__ bool store_key(Selection& s, uint64_t floor, float x, uint32_t index, uint32_t want,
-                                          Offer& o) {
+__device__ __forceinline__ bool store_key(Selection& s, uint64_t floor, float x, uint32_t index, Offer& o) {
   const uint64_t key = order_key(x, index);
   if (key < floor) return true;
   const uint32_t at = atomicAdd(&s.count, 1u);
-  o.over = o.over || at >= 2 * want + 64;
+  o.over = o.over || at >= kCrowd;
   if (at >= Selection::CAP) return false;
   s.key[at] = key;
   return true;
@@ -562,28 +551,29 @@ __device__ __forceinline__ bool store_key(Selection& s, uint64_t floor, float x,
 // Offers the marked ones of a thread's logits of the k-th stage of a step, which is still in shared
 // memory.
 __device__ __forceinline__ void offer_stage(Selection& s, const Part& p, uint32_t q, uint32_t k, const float4* stage,
-                                            uint32_t hits, uint64_t floor, uint32_t want, Offer& o) {
+                                            uint32_t hits, uint64_t floor, Offer& o) {
   while (hits && o.left == 0xffffffffu) {
     const uint32_t i = uint32_t(__ffs(int(hits))) - 1u;
     const uint32_t piece = (i >> 2) * BLOCK + threadIdx.x;
     const float x = reinterpret_cast<const float*>(stage + piece)[i & 3u];
-    if (!store_key(s, floor, x, p.lead + (q + piece) * 4u + (i & 3u), want, o)) o.left = k * 16u + i;
+    if (!store_key(s, floor, x, p.lead + (q + piece) * 4u + (i & 3u), o)) o.left = k * 16u + i;
     hits &= hits - 1u;
   }
 }
 
 // The look after a step of `stages` stages from piece `q`: throws out the surplus when there is one,
-// and goes on with what had found no room (from the row itself: that is rare).  All adding threads
-// call it.
+// and goes on with what had found no room (from the row itself: that is rare).  At the row's end a
+// surplus that the sort can do with may stay.  All adding threads call it.
 __device__ __forceinline__ void settle(Selection& s, const float* x, const Part& p, uint32_t q, uint32_t stages,
-                                       int extra, uint32_t want, Offer& o) {
+                                       int extra, uint32_t want, bool last, Offer& o) {
+  if (last) o.over = o.left != 0xffffffffu || o.outside;
   while (adders_or<BLOCK>(o.over)) {
     keep_largest(s, min(s.count, Selection::CAP), want);
     if (!adders_or<BLOCK>(o.left != 0xffffffffu || o.outside)) break;
     o.over = false;
     const uint64_t floor = s.floor;
     const float low = floor_value(floor);
-    if (o.outside) o.outside = !store_key(s, floor, x[extra], uint32_t(extra), want, o);
+    if (o.outside) o.outside = !store_key(s, floor, x[extra], uint32_t(extra), o);
     uint32_t i = o.left;
     o.left = 0xffffffffu;
     for (; i < stages * 16u; ++i) {
@@ -591,7 +581,7 @@ __device__ __forceinline__ void settle(Selection& s, const float* x, const Part&
       if (piece >= p.q1) continue;
       const uint32_t index = p.lead + piece * 4u + (i & 3u);
       const float v = x[index];
-      if (v >= low && !store_key(s, floor, v, index, want, o)) {
+      if (v >= low && !store_key(s, floor, v, index, o)) {
         o.left = i;
         break;
       }
@@ -605,9 +595,9 @@ __device__ __forceinline__ void settle(Selection& s, const float* x, const Part&
 __device__ uint32_t sort_selection(Selection& s, uint64_t* sorted, uint32_t want) {
   adders_sync<BLOCK>();
   uint32_t n = s.count;
-  if (n > 2 * kMaxTop + 64) {  // the alternatives of several blocks
+  if (n > kCrowd) {  // the alternatives of several blocks
     keep_largest(s, n, want);
-    n = want;
+    n = s.count;
   }
   // a key's place is the number of keys above it
   for (uint32_t i = threadIdx.x; i < n; i += BLOCK) {
@@ -723,7 +713,7 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
         const uint64_t floor = sel.floor;
         const float low = floor_value(floor);
         if (extra_at >= 0 && extra >= low)
-          mine.outside = !store_key(sel, floor, extra, uint32_t(extra_at), a.top_n, mine);
+          mine.outside = !store_key(sel, floor, extra, uint32_t(extra_at), mine);
 #pragma unroll 1
         for (uint32_t k = 0; k < FIRST && (k == 0 || q + k * kStage<T> < p.q1); ++k) {
           const float4* stage = ring + again.slot * kStage<T>;
@@ -731,32 +721,37 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
             float4 v[QUADS];
             read_stage<T>(p, q + k * kStage<T>, stage, v);
             const uint32_t hits = above_floor(p, q + k * kStage<T>, v, low);
-            offer_stage(sel, p, q + k * kStage<T>, k, stage, hits, floor, a.top_n, mine);
+            offer_stage(sel, p, q + k * kStage<T>, k, stage, hits, floor, mine);
           }
           leave_stage<T>(bars, again);
           again.next();
         }
-        settle(sel, x, p, q, FIRST, extra_at, a.top_n, mine);
+        settle(sel, x, p, q, FIRST, extra_at, a.top_n, q + FIRST * kStage<T> >= p.q1, mine);
         q += FIRST * kStage<T>;
       }
+      // stages of the next step: as many as bring at most about half of CAP keys, and at least three
+      // times as many as have been seen (`want` is at most 128)
+      const uint32_t grow = TOP ? Selection::CAP / 2 / a.top_n - 1 : 1;
+      uint32_t stages = FIRST * grow;
       while (q < p.q1 || (!TOP && q == p.q0)) {
         const uint64_t floor = TOP ? sel.floor : 0;
         const float low = TOP ? floor_value(floor) : INFINITY;
 #pragma unroll 1
-        for (uint32_t k = 0; k < STEP && (k == 0 || q + k * kStage<T> < p.q1); ++k) {
+        for (uint32_t k = 0; k < stages && (k == 0 || q + k * kStage<T> < p.q1); ++k) {
           float4 v[QUADS];
           take_stage<T>(p, q + k * kStage<T>, ring, bars, at, w, v);
           if (stream.add(v, kLog2e) >= low && TOP) {
             const float4* stage = ring + at.slot * kStage<T>;
             read_stage<T>(p, q + k * kStage<T>, stage, v);
             const uint32_t hits = above_floor(p, q + k * kStage<T>, v, low);
-            offer_stage(sel, p, q + k * kStage<T>, k, stage, hits, floor, a.top_n, mine);
+            offer_stage(sel, p, q + k * kStage<T>, k, stage, hits, floor, mine);
           }
           leave_stage<T>(bars, at);
           at.next();
         }
-        if (TOP) settle(sel, x, p, q, STEP, -1, a.top_n, mine);
-        q += STEP * kStage<T>;
+        if (TOP) settle(sel, x, p, q, stages, -1, a.top_n, q + stages * kStage<T> >= p.q1, mine);
+        q += stages * kStage<T>;
+        stages = min((q - p.q0) / kStage<T> * grow, 1u << 20);
       }
       RowStats r = stream.result(kLog2e);
       add_one<Sum::Entropy>(r, extra, 0.f);
