@@ -1843,8 +1843,8 @@ bool overlap(const Use& a, const Use& b) {
   const char *pa = reinterpret_cast<const char*>(a.b->dptr), *pb = reinterpret_cast<const char*>(b.b->dptr);
   return pa < pb + b.bytes && pb < pa + a.bytes;
 }
-// -2: buffers on different devices, -3: an output overlaps an input or another output, -1: no
-// device, -6: an upload failed, 0: inputs are resident.  NULL handles are skipped.
+// -2: buffers on different devices, -3: an output overlaps an input or another output, or a buffer
+// does not start on 4 bytes, -1: no device, -6: an upload failed, 0: inputs are resident.  NULL handles are skipped.
 int prepare_buffers(const char* what, std::initializer_list<Use> ins, std::initializer_list<Use> outs,
                     CError* err) {
   const int dev = ins.begin()->b->device;
@@ -1853,6 +1853,12 @@ int prepare_buffers(const char* what, std::initializer_list<Use> ins, std::initi
       if (u.b && u.b->device != dev) {
         set_error(err, "%s: buffers live on different devices.", what);
         return -2;
+      }
+  for (const auto* list : {&ins, &outs})
+    for (const Use& u : *list)
+      if (u.b && (reinterpret_cast<uintptr_t>(u.b->dptr) & 3u)) {  // wrapped memory
+        set_error(err, "%s: a buffer does not start on 4 bytes.", what);
+        return -3;
       }
   for (const Use* o = outs.begin(); o != outs.end(); ++o) {
     bool bad = false;
@@ -2232,10 +2238,19 @@ int mxfp4_product(const char* what, GPUPtr aPtr, bool a_float, long m, GPUPtr bP
   p.act = act;
   p.act_param = act_param;
   void* scratch = nullptr;
-  if (a_float && gonn::mxfp4_takes_float(uint64_t(m))) {
+  if (a_float && m <= gonn::kMxfp4FloatRows) {
     p.a = nullptr;
     p.a_float = a->dptr;
   } else if (a_float) {
+    // A graph would go on using the scratch after it has gone back to the cache, on whatever stream
+    // it is replayed.
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(d.stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+      cudaGetLastError();
+      set_error(err, "%s: more than %d rows take library scratch, which a captured graph cannot hold; capture "
+                     "gonngpu_mxfp4_quantize and gonngpu_mxfp4_matmul instead.", what, gonn::kMxfp4FloatRows);
+      return -5;
+    }
     if (pool_alloc(c->device, &scratch, la.bytes) != cudaSuccess) {
       cudaGetLastError();
       set_error(err, "%s: could not allocate the packed operand.", what);

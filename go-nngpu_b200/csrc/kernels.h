@@ -208,9 +208,11 @@ cudaError_t launch_mxfp4_quantize(const float* src, uint64_t rows, uint64_t cols
 // packed matrix [rows, cols] -> float32 (dense).
 cudaError_t launch_mxfp4_dequantize(const void* packed, uint64_t rows, uint64_t cols, float* dst,
                                     cudaStream_t stream);
+// A product quantises that many float32 rows of A itself.
+constexpr int kMxfp4FloatRows = 8;
 struct Mxfp4Product {
   const void* a = nullptr;  // packed [M, K], or
-  const float* a_float = nullptr;  // float32 [M, K], for as few rows as mxfp4_takes_float allows
+  const float* a_float = nullptr;  // float32 [M, K] in its place, M <= kMxfp4FloatRows
   const void* b = nullptr;  // packed [N, K]
   uint64_t M = 0, N = 0, K = 0;
   float* c = nullptr;           // [M, N] float32, dense
@@ -218,8 +220,6 @@ struct Mxfp4Product {
   int act = ACT_NONE;
   float act_param = 0.f;
 };
-// True when a product with that many rows of A quantises them itself.
-bool mxfp4_takes_float(uint64_t rows);
 // C = act(A . B^T + bias).  Returns nullptr on success, else a static message.
 const char* launch_mxfp4_product(const Mxfp4Product& p, GemmStatus* status, int sm_count, cudaStream_t stream);
 

@@ -1430,8 +1430,8 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
     }
   }
   __syncthreads();
+  if (shares > 1) ptx::cluster_sync_all();  // no block leaves while another may still write to it
   wait_out(&abort_word);
-  // (a peer's last message has been waited for: nobody writes here any more)
 }
 
 // Short rows, one warp each.

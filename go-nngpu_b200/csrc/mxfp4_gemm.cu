@@ -115,7 +115,7 @@ __device__ __forceinline__ void load_codes(uint32_t dst, const CUtensorMap* m, u
 // by, quantise it stage by stage into the place where the tensor core looks for its codes and
 // scales: one launch instead of two.  (Every CTA does all of it, which is why it stops at 8 rows.)
 constexpr uint32_t SINGLE_THREADS = 192;
-constexpr uint32_t FLOAT_ROWS = 8;
+constexpr uint32_t FLOAT_ROWS = kMxfp4FloatRows;
 constexpr uint32_t MAX_SPLITS = 4;
 
 template <int BN, int STAGES>
@@ -737,8 +737,6 @@ const char* launch_class(const Mxfp4Product& q, GemmStatus* status, int sm_count
 }
 
 }  // namespace
-
-bool mxfp4_takes_float(uint64_t rows) { return rows <= FLOAT_ROWS; }
 
 const char* launch_mxfp4_product(const Mxfp4Product& q, GemmStatus* status, int sm_count, cudaStream_t stream) {
   if (q.act == ACT_RELU) return launch_class<RELU>(q, status, sm_count, stream);

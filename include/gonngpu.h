@@ -393,9 +393,9 @@ GONNGPU_API int gonngpu_linear_backward(GPUPtr x, GPUPtr w, GPUPtr dy, GPUPtr ac
  * +inf gives NaN (alternatives: token -1).  Token numbers below 0 mean "none"; one that is not
  * below vocab is treated as none (a log probability: NaN) and reported: -3, by
  * this call in blocking mode, else by gonngpu_synchronize.  Result buffers must
- * not overlap other buffers of the call.  Errors: -1 device, -2 bad or missing
- * buffer, -3 dimensions, sizes, parameters or token numbers, -4 launch, -6
- * execution. */
+ * not overlap other buffers of the call; wrapped memory starts on 4 bytes.
+ * Errors: -1 device, -2 bad or missing buffer, -3 dimensions, sizes, parameters
+ * or token numbers, -4 launch, -6 execution. */
 
 /* At most this many alternatives, or teacher logits, per row. */
 #define GONNGPU_MAX_TOP 128
@@ -475,7 +475,9 @@ GONNGPU_API int gonngpu_mxfp4_matmul(GPUPtr a, long m, GPUPtr b, long n, long k,
                          int activation_type, float activation_param, GPUPtr c, CError *err);
 /* The 4-bit form of perform_fused_linear_activation: x [batch, in_size] float32 is
  * quantised (blocks along in_size) and multiplied by packed weights [out_size,
- * in_size]; y [batch, out_size] float32. */
+ * in_size]; y [batch, out_size] float32.  Up to 8 rows are quantised inside the
+ * product; more take library scratch, so that the call is refused (-5) while the
+ * library's stream is being captured into a graph. */
 GONNGPU_API int gonngpu_mxfp4_linear(GPUPtr x, long batch, long in_size, GPUPtr weights, long out_size,
                          GPUPtr bias, int activation_type, float activation_param, GPUPtr y,
                          CError *err);
