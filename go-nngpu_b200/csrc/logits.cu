@@ -279,7 +279,10 @@ __device__ __forceinline__ void take_stage(const Part& p, uint32_t q, const floa
   w.wait(&bars.full[at.slot], at.phase, at.slot);
   read_stage<T>(p, q, ring + at.slot * kStage<T>, v);
 }
-// The warp does not need the stage any more.
+// The warp does not need the stage any more.  What it has read must have been used by something that
+// cannot move behind the arrival (a vote, a store): the arrival can overtake loads under way, and the
+// next copy then lands in front of them (one backward pass in ten over 2048 x 32000 had 256 bytes of a
+// row from the next copy).
 template <int T>
 __device__ __forceinline__ void leave_stage(RingBars<T>& bars, const RingAt<T>& at) {
   __syncwarp();
@@ -1379,7 +1382,6 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
             else scale_stage<SUM>(f, v, kept_at[start.slot][threadIdx.x], c);
           } else {
             take_stage<T>(p, q, ring, bars, at, w, v);
-            if (!BULK) leave_stage<T>(bars, at);
             grad_stage<SUM>(f, v, c);
           }
           if (BULK) {
@@ -1392,10 +1394,7 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
           if (BULK) {
             __syncwarp();
             if (lane == 0) arrive(&stored[now_at.slot]);
-          } else if (kept) {
-            leave_stage<T>(bars, start);
           }
-          now_at.next();
           if (BULK) {
             // sent by the storing warp
           } else if (vec && q + kStage<T> <= p.q1) {
@@ -1419,6 +1418,8 @@ distill_ring_kernel(const DistillArgs a, uint32_t shares, bool keep) {
               }
             }
           }
+          if (!BULK) leave_stage<T>(bars, now_at);  // after the stores, which wait for what was read
+          now_at.next();
           q += kStage<T>;
         } while (q < p.q1);
       }

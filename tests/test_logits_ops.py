@@ -478,3 +478,41 @@ def test_results_repeat_bit_for_bit(gpu):
             assert np.array_equal(first[0], again[0]) and np.array_equal(first[2], again[2])
             for a, b in zip(lp, run_logprobs(gpu, x, tokens, 16)):
                 assert np.array_equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["backward", "step", "forward", "logprobs"])
+def test_long_runs_repeat_bit_for_bit(gpu, kind):
+    """Rings under load, pass after pass: a stage that is given back before it has been read shows here."""
+    rows, vocab, top, g = 2048, 32000, 16, gpu
+    rng = np.random.default_rng(5)
+    x = some_logits(rng, rows, vocab, masked=True)
+    tokens, z, labels = some_teacher(rng, x, top)
+    bx, bz = g.Buffer.from_host(x), g.Buffer.from_host(z)
+    bt, bl = g.Buffer.from_host_int32(tokens), g.Buffer.from_host_int32(labels)
+    loss, stats, grad = g.Buffer.empty(rows * 4), g.Buffer.empty(rows * 12), g.Buffer.empty(rows * vocab * 4)
+    tt, tl = g.Buffer.empty(rows * top * 4), g.Buffer.empty(rows * top * 4)
+    args = (bx, rows, vocab, bt, bz, top, bl, 2.0, 0.5)
+    g.distill_forward(*args, loss=loss, stats=stats)
+
+    def run():
+        if kind == "backward":
+            g.distill_backward(*args, stats=stats, grad=grad)
+            return grad.retrieve((rows, vocab))
+        if kind == "step":
+            g.distill_step(*args, loss=loss, grad=grad)
+            return grad.retrieve((rows, vocab))
+        if kind == "forward":
+            g.distill_forward(*args, loss=loss, stats=stats)
+            return stats.retrieve((rows, 3))
+        g.token_logprobs(bx, rows, vocab, tokens=bl, n_tokens=1, logprobs=loss, top_n=top, top_tokens=tt,
+                         top_logprobs=tl)
+        return np.concatenate([loss.retrieve((rows, 1)), tl.retrieve((rows, top))], axis=1)
+
+    first = run()
+    for _ in range(40):
+        assert np.array_equal(run(), first, equal_nan=True)
+    if kind in ("backward", "step"):
+        for r in range(0, rows, 256):
+            want = distill64(x[r:r + 8], tokens[r:r + 8], z[r:r + 8], labels[r:r + 8], 2.0, 0.5, np.ones(8))
+            assert close(first[r:r + 8], want[1], want[3])
