@@ -11,8 +11,8 @@
 //
 // Short rows (up to 1024 logits) are held in the registers of one warp.  Longer ones go through a
 // ring of shared-memory stages of 4096 or 8192 logits: one warp of a block feeds it with bulk copies,
-// ahead of the eight or sixteen warps that add (T threads), and into the next row; another warp takes care of what is little
-// and slow, the tokens, targets and results of a row.  Few long rows are shared by the up to 8 blocks
+// ahead of the eight or sixteen warps that add (T threads), and into the next row; another one or two
+// take care of what is little and slow, the tokens, targets and results of a row.  Few long rows are shared by the up to 8 blocks
 // of a cluster.  All merges have a fixed order: results repeat bit for bit.
 #include <algorithm>
 
@@ -27,7 +27,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int BLOCK = 256;                          // adding threads of a ring kernel, and
-constexpr int WIDE = 512;                           // of the step, which has an SM to itself
+constexpr int WIDE = 512;                           // of the step over wide rows
 constexpr int ROWS_BLOCK = 256;                     // threads of a kernel with a warp per row
 constexpr uint32_t QUADS = 4;                       // 16-byte pieces of an adding thread in one stage
 constexpr uint32_t WARP_ROW = 1024;                 // longest row that one warp holds
@@ -199,7 +199,7 @@ __device__ __forceinline__ float4 masked_quad() { return make_float4(-INFINITY, 
 template <int T>
 constexpr uint32_t kStage = QUADS * T;  // pieces of a stage: 16 or 32 KB
 template <int T>
-constexpr uint32_t kStages = T == WIDE ? 6 : 4;  // 192 KB and one block an SM, or 64 KB and three
+constexpr uint32_t kStages = T == WIDE ? 6 : 4;  // 192 KB and one block an SM, or 64 KB and two or three
 template <int T>
 struct RingBars {
   uint64_t full[kStages<T>], empty[kStages<T>];

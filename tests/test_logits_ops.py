@@ -516,3 +516,26 @@ def test_long_runs_repeat_bit_for_bit(gpu, kind):
         for r in range(0, rows, 256):
             want = distill64(x[r:r + 8], tokens[r:r + 8], z[r:r + 8], labels[r:r + 8], 2.0, 0.5, np.ones(8))
             assert close(first[r:r + 8], want[1], want[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,t", [(200, 130001, 1.0), (400, 40000, 2.0), (320, 70003, 1.5), (700, 9000, 4.0)])
+def test_steps_that_read_rows_twice(gpu, rows, vocab, t):
+    """In place, beside the logits, and with rows at another distance from 16 bytes: the same gradient."""
+    rng = np.random.default_rng(vocab)
+    x = some_logits(rng, rows, vocab)
+    tokens, z, labels = some_teacher(rng, x, 20)
+    tokens[:, 7] = tokens[:, 3]
+    labels[::3] = tokens[::3, 5]
+    loss, _, grad = run_distill(gpu, "step", x, tokens, z, labels, t, 0.5)
+    again, _, inside = run_distill(gpu, "step", x, tokens, z, labels, t, 0.5, in_place=True)
+    assert np.array_equal(loss, again) and np.array_equal(grad, inside)
+    bx, bt, bz, bl = (gpu.Buffer.from_host(x), gpu.Buffer.from_host_int32(tokens), gpu.Buffer.from_host(z),
+                      gpu.Buffer.from_host_int32(labels))
+    out, apart = gpu.Buffer.empty(rows * 4), gpu.Buffer.empty(rows * (vocab + 1) * 4)
+    gpu.distill_step(bx, rows, vocab, bt, bz, 20, bl, t, 0.5, loss=out, grad=apart, ld_grad=vocab + 1)
+    assert np.array_equal(out.retrieve((rows,)), loss)
+    assert np.array_equal(apart.retrieve((rows, vocab + 1))[:, :vocab], grad)
+    some = np.array([0, 1, rows // 2, rows - 1])
+    want = distill64(x[some], tokens[some], z[some], labels[some], t, 0.5, np.ones(4))
+    assert close(loss[some], want[0], want[2]) and close(grad[some], want[1], want[3])
