@@ -743,9 +743,11 @@ logprobs_ring_kernel(const LogprobArgs a, uint32_t shares) {
         for (uint32_t k = 0; k < stages && (k == 0 || q + k * kStage<T> < p.q1); ++k) {
           float4 v[QUADS];
           take_stage<T>(p, q + k * kStage<T>, ring, bars, at, w, v);
-          if (stream.add(v, kLog2e) >= low && TOP) {
+          float4 raw[QUADS];
+#pragma unroll
+          for (uint32_t j = 0; j < QUADS; ++j) raw[j] = v[j];
+          if (stream.add(raw, kLog2e) >= low && TOP) {
             const float4* stage = ring + at.slot * kStage<T>;
-            read_stage<T>(p, q + k * kStage<T>, stage, v);
             const uint32_t hits = above_floor(p, q + k * kStage<T>, v, low);
             offer_stage(sel, p, q + k * kStage<T>, k, stage, hits, floor, mine);
           }
